@@ -33,7 +33,7 @@ extern "C" {
 #define W8A8_ECUDA 3    /* the CUDA launch failed (cudaGetLastError) */
 #define W8A8_ESCRATCH 4 /* the scratch buffer is smaller than required */
 
-#define W8A8_ABI_VERSION 6
+#define W8A8_ABI_VERSION 7
 #define W8A8_MAX_ROWS 16 /* query rows per call (decode: 1, prefill chunk: 16) */
 
 /* ABI version (W8A8_ABI_VERSION) and a message for a status code. */
@@ -67,7 +67,8 @@ int w8a8_embed(const int32_t* tokens, int rows, const int8_t* emb_q, const float
  * copy did not land within its bounded wait; bit 3: the same for an MoE weight
  * tile; bit 4: a tensor-core GEMM pipeline wait; bit 5: a tensor-parallel
  * exchange wait gave up; bit 6: w8a8_moe_ffn_rows found more pairs of one
- * expert than rows, routing that is not Top-k, and skipped the excess).
+ * expert than rows, routing that is not Top-k, and skipped the excess; bit 7:
+ * a w8a8_kvb_* row or length past the cache's capacity, skipped).
  * Synchronous with the device.
  * Plays the role of the overlay's sticky list status (llm/sa_funcsim.py:62-66,
  * firmware/rt/rt_fw.c:53-60). */
@@ -474,6 +475,87 @@ int w8a8_quant_rows_posted(const float* x, const uint32_t* amax_bits, int rows, 
                            void* stream);
 int w8a8_dequant_resid(const int32_t* acc, const float* s_x, const float* s_w, int rows, int n, const float* resid,
                        float* y, void* stream);
+
+/* ------------------------------------------------------------------------
+ * A KV cache held in 8 bits with dynamic scales: one fp32 scale per (slot, KV
+ * head, block of tokens) for K and one for V; the value held is code * scale.
+ * No counterpart in the reference, whose cache scales are calibrated before
+ * the run (hf_generic.py:466-491) and fixed; here the scales follow the data,
+ * any capacity is taken, and a slot can be cut to its heaviest tokens. The
+ * arithmetic is plain fp32 (not the overlay's SFU): rows come in and go out in
+ * fp32, bf16 or fp16.
+ *
+ * Layout: codes [slots][kv_heads][capacity][head_dim] for K and for V, scales
+ * [slots][kv_heads][capacity / block]; consecutive slots are slot_stride codes
+ * and scale_stride scales apart (so that one layer of a [slots, layers, ...]
+ * cache can be passed). head_dim a multiple of 16, at most W8A8_KVB_MAX_HEAD_DIM;
+ * block 16, 32, 64 or 128; capacity a multiple of block. Blocks at or past a
+ * slot's length are never read.
+ *
+ * Rows of several sequences lie one behind the other: slot b's are
+ * start[b] .. start[b + 1] - 1 (start: [slots + 1] int32 on the device, or NULL:
+ * one row per slot, rows = slots), and its row i is the token at cache position
+ * pos[b] + i (pos: [slots] int32 on the device, negative: an idle slot). Rows
+ * behind the last sequence are left alone, rows past the capacity skipped
+ * (error bit 7). Keys and queries come with their position encoding applied.
+ * Distinct slots never share memory: calls on distinct slots may overlap. */
+#define W8A8_F32 0
+#define W8A8_BF16 1
+#define W8A8_F16 2
+#define W8A8_KVB_MAX_HEAD_DIM 256
+
+typedef struct {
+    int8_t* k;                 /* codes, 16-byte aligned */
+    int8_t* v;
+    float* k_scale;
+    float* v_scale;
+    int slots, kv_heads, capacity, head_dim, block;
+    int64_t slot_stride;       /* codes between slots, a multiple of 16 */
+    int64_t scale_stride;      /* scales between slots */
+} W8A8KvBlocks;
+
+/* Write rows k, v [rows][kv_heads][head_dim] (k_stride / v_stride elements
+ * between rows: slices of a fused qkv row) of type `dtype`. Per touched block
+ * s' = max(s, max|new| * F(1/127)) (s = 0 without older tokens in it), new
+ * codes = rint(x / s'), older codes = rint((q * s) / s') when s' grew; a block
+ * that holds only zeros has scale 0. NaN is written as 0, an infinity as the
+ * largest finite value. */
+int w8a8_kvb_append(const W8A8KvBlocks* cache, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                    int dtype, int rows, const int32_t* pos, const int32_t* start, void* stream);
+
+/* The values the cache holds: k, v [rows][kv_heads][head_dim] of type `dtype`;
+ * rows of idle slots and rows past the capacity are zero. */
+int w8a8_kvb_read(const W8A8KvBlocks* cache, int rows, const int32_t* pos, const int32_t* start, void* k, void* v,
+                  int dtype, void* stream);
+
+/* Attention of rows q [rows][heads][head_dim] (q_stride elements between rows)
+ * over their slot's tokens up to and with their own position (appended
+ * before): out [rows][heads][head_dim] = softmax(scale * q . k) v, zero for
+ * idle slots and rows past the capacity. heads a multiple of kv_heads. mass (or
+ * NULL): [slots][kv_heads][capacity], each token's probabilities, summed over
+ * the rows and the query heads of its KV head, are added. start NULL: one row
+ * per slot (decode). scratch: w8a8_kvb_attn_scratch_bytes() bytes (16-byte
+ * aligned, contents irrelevant), not shared by calls that can overlap. */
+size_t w8a8_kvb_attn_scratch_bytes(const W8A8KvBlocks* cache, int heads, int rows, int one_row_per_slot,
+                                   int with_mass);
+int w8a8_kvb_attn(const W8A8KvBlocks* cache, const void* q, int64_t q_stride, int dtype, int heads, int rows,
+                  const int32_t* pos, const int32_t* start, float scale, void* out, float* mass, void* scratch,
+                  size_t scratch_bytes, void* stream);
+
+/* Cut every slot to its `keep` most attended tokens: of a slot holding
+ * n = count[b] > keep tokens the first `sink`, the last `recent` and, of those
+ * between, the keep - sink - recent with the largest mass stay (equal weights:
+ * the lower position; NaN counts as -infinity), in their order, at positions
+ * 0 .. keep - 1; each block is requantized to its largest value (codes
+ * rint((q * s) / s'), s' = max|q * s| * F(1/127)). A slot with n <= keep stays
+ * as it is. dst NULL: in place (dst_mass is then ignored, mass is written);
+ * else the result goes to dst / dst_mass (no overlap with cache / mass; its
+ * capacity at least keep) and the source stays. kept [slots][kv_heads][keep]:
+ * each place's former position, -1 past the new length; count_out [slots]
+ * (not count itself): the new lengths min(n, keep). The mass of the places past
+ * the new length, up to n, is set to 0. */
+int w8a8_kvb_evict(const W8A8KvBlocks* cache, float* mass, const int32_t* count, int keep, int sink, int recent,
+                   const W8A8KvBlocks* dst, float* dst_mass, int32_t* kept, int32_t* count_out, void* stream);
 
 #ifdef __cplusplus
 }

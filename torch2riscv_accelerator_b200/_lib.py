@@ -12,7 +12,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("W8A8_B200_LIB") or os.path.join(HERE, "libw8a8_b200.so")
 
 W8A8_OK, W8A8_EINVAL, W8A8_EALIGN, W8A8_ECUDA, W8A8_ESCRATCH = 0, 1, 2, 3, 4
-ABI_VERSION = 6
+ABI_VERSION = 7
 ACT_SILU, ACT_GELU_TANH = 0, 1
 TP_MAX_RANKS, TP_ROWS, TP_CTAS, TP_HEADER = 8, 4, 512, 256
 TP_STORE, TP_PARTIAL, TP_SWIGLU = 0, 1, 2
@@ -27,6 +27,12 @@ class W8A8AttnArgs(C.Structure):
                 ("scratch", C.c_void_p), ("scratch_bytes", C.c_size_t), ("att_amax", C.c_void_p),
                 ("k_scale", C.c_void_p), ("inv_sk_ch", C.c_void_p), ("inv_sv_ch", C.c_void_p),
                 ("a_v_ch", C.c_void_p)]
+
+
+class W8A8KvBlocks(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("slots", C.c_int), ("kv_heads", C.c_int), ("capacity", C.c_int), ("head_dim", C.c_int),
+                ("block", C.c_int), ("slot_stride", C.c_int64), ("scale_stride", C.c_int64)]
 
 
 class W8A8TpComm(C.Structure):
@@ -113,6 +119,11 @@ PROTOTYPES = {
     "w8a8_row_amax": (I, [P, I, I, P, P]),
     "w8a8_quant_rows_posted": (I, [P, P, I, I, P, P, P]),
     "w8a8_dequant_resid": (I, [P, P, P, I, I, P, P, P]),
+    "w8a8_kvb_append": (I, [C.POINTER(W8A8KvBlocks), P, L, P, L, I, I, P, P, P]),
+    "w8a8_kvb_read": (I, [C.POINTER(W8A8KvBlocks), I, P, P, P, P, I, P]),
+    "w8a8_kvb_attn_scratch_bytes": (Z, [C.POINTER(W8A8KvBlocks), I, I, I, I]),
+    "w8a8_kvb_attn": (I, [C.POINTER(W8A8KvBlocks), P, L, I, I, I, P, P, F, P, P, P, Z, P]),
+    "w8a8_kvb_evict": (I, [C.POINTER(W8A8KvBlocks), P, P, I, I, I, C.POINTER(W8A8KvBlocks), P, P, P, P]),
 }
 
 _LIB = None

@@ -5,6 +5,7 @@
 #include <mutex>
 
 #include "../../include/w8a8.h"
+#include "kvb.cuh"
 #include "trace.cuh"
 #include "w8a8_internal.h"
 
@@ -90,7 +91,7 @@ int w8a8_error_flags(uint32_t* flags) {
     unsigned int v = 0;
     int st = cuda_status(read_clear_errors(&v));
     *flags = v | gemv_read_clear_errors() | attn_read_clear_errors() | moe_read_clear_errors() |
-             gemm_read_clear_errors();
+             gemm_read_clear_errors() | kvb_read_clear_errors() | kvb_attn_read_clear_errors();
     return st;
 }
 
@@ -692,6 +693,112 @@ int w8a8_tp_moe_combine(const W8A8TpComm* comm, const uint64_t* terms, int rows,
         !tp_block(comm, terms, W8A8_TP_MOE_WORDS(comm->ranks, top_k, dim)))
         return W8A8_EINVAL;
     return cuda_status(launch_moe_combine_ll(t, terms, rows, top_k, dim, resid, y, S(stream)));
+}
+
+// ------------------------------------------------- block-scaled 8-bit KV cache
+static int kvb_cache(const W8A8KvBlocks* c, KvbCache* o) {
+    if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale || c->slots <= 0 || c->slots > 65535 || c->kv_heads <= 0 ||
+        c->kv_heads > 65535 || c->capacity <= 0 || c->capacity > (1 << 30) || c->head_dim <= 0 ||
+        c->head_dim > W8A8_KVB_MAX_HEAD_DIM)
+        return W8A8_EINVAL;
+    if (c->block != 16 && c->block != 32 && c->block != 64 && c->block != 128) return W8A8_EINVAL;
+    if (c->capacity % c->block) return W8A8_EINVAL;
+    if (c->head_dim % 16 || !al16(c->k) || !al16(c->v) || c->slot_stride % 16) return W8A8_EALIGN;
+    if (((reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) & 3u) != 0)
+        return W8A8_EALIGN;
+    if (c->slots > 1 && (c->slot_stride < (int64_t)c->kv_heads * c->capacity * c->head_dim ||
+                         c->scale_stride < (int64_t)c->kv_heads * (c->capacity / c->block)))
+        return W8A8_EINVAL;
+    *o = KvbCache{c->k,        c->v,        c->k_scale, c->v_scale,     c->slots,       c->kv_heads,
+                  c->capacity, c->head_dim, c->block,   c->slot_stride, c->scale_stride};
+    return W8A8_OK;
+}
+
+static int kvb_rows(const KvbCache& c, int rows, const int32_t* pos, const int32_t* start, KvbRows* o) {
+    if (rows < 0 || !pos || (!start && rows != c.slots)) return W8A8_EINVAL;
+    *o = KvbRows{rows, pos, start};
+    return W8A8_OK;
+}
+
+static int kvb_type_bytes(int dtype) {
+    return dtype == W8A8_F32 ? 4 : dtype == W8A8_BF16 || dtype == W8A8_F16 ? 2 : 0;
+}
+
+int w8a8_kvb_append(const W8A8KvBlocks* cache, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                    int dtype, int rows, const int32_t* pos, const int32_t* start, void* stream) {
+    KvbAppendArgs a{};
+    int st = kvb_cache(cache, &a.c);
+    if (!st) st = kvb_rows(a.c, rows, pos, start, &a.r);
+    if (st) return st;
+    const int e = kvb_type_bytes(dtype);
+    const int64_t row = (int64_t)a.c.heads * a.c.hd;
+    if (!e || (rows > 0 && (!k || !v)) || (rows > 1 && (k_stride < row || v_stride < row))) return W8A8_EINVAL;
+    if (!al16(k) || !al16(v) || (k_stride * e) % 16 || (v_stride * e) % 16) return W8A8_EALIGN;
+    if (rows == 0) return W8A8_OK;
+    a.k = k, a.v = v, a.k_stride = k_stride, a.v_stride = v_stride, a.type = dtype;
+    return cuda_status(launch_kvb_append(a, S(stream)));
+}
+
+int w8a8_kvb_read(const W8A8KvBlocks* cache, int rows, const int32_t* pos, const int32_t* start, void* k, void* v,
+                  int dtype, void* stream) {
+    KvbReadArgs a{};
+    int st = kvb_cache(cache, &a.c);
+    if (!st) st = kvb_rows(a.c, rows, pos, start, &a.r);
+    if (st) return st;
+    if (!kvb_type_bytes(dtype) || (rows > 0 && (!k || !v))) return W8A8_EINVAL;
+    if (!al16(k) || !al16(v)) return W8A8_EALIGN;
+    if (rows == 0) return W8A8_OK;
+    a.k = k, a.v = v, a.type = dtype;
+    return cuda_status(launch_kvb_read(a, S(stream)));
+}
+
+size_t w8a8_kvb_attn_scratch_bytes(const W8A8KvBlocks* cache, int heads, int rows, int one_row_per_slot,
+                                   int with_mass) {
+    KvbCache c;
+    if (kvb_cache(cache, &c) || heads <= 0 || heads % c.heads || rows <= 0) return 0;
+    return kvb_attn_scratch(c, heads, rows, one_row_per_slot != 0, with_mass != 0);
+}
+
+int w8a8_kvb_attn(const W8A8KvBlocks* cache, const void* q, int64_t q_stride, int dtype, int heads, int rows,
+                  const int32_t* pos, const int32_t* start, float scale, void* out, float* mass, void* scratch,
+                  size_t scratch_bytes, void* stream) {
+    KvbAttnArgs a{};
+    int st = kvb_cache(cache, &a.c);
+    if (!st) st = kvb_rows(a.c, rows, pos, start, &a.r);
+    if (st) return st;
+    const int e = kvb_type_bytes(dtype);
+    if (!e || heads <= 0 || heads > 65535 || heads % a.c.heads || !(std::fabs(scale) <= 3.4e38f)) return W8A8_EINVAL;
+    if (rows > 0 && (!q || !out || (rows > 1 && q_stride < (int64_t)heads * a.c.hd))) return W8A8_EINVAL;
+    if (!al16(q) || !al16(out) || (q_stride * e) % 16 || !al16(scratch)) return W8A8_EALIGN;
+    if (rows == 0) return W8A8_OK;
+    const size_t need = kvb_attn_scratch(a.c, heads, rows, start == nullptr, mass != nullptr);
+    if (need && (!scratch || scratch_bytes < need)) return W8A8_ESCRATCH;
+    a.q = q, a.q_stride = q_stride, a.out = out, a.heads = heads, a.type = dtype, a.scale = scale, a.mass = mass;
+    a.scratch = scratch;
+    return cuda_status(launch_kvb_attn(a, S(stream)));
+}
+
+int w8a8_kvb_evict(const W8A8KvBlocks* cache, float* mass, const int32_t* count, int keep, int sink, int recent,
+                   const W8A8KvBlocks* dst, float* dst_mass, int32_t* kept, int32_t* count_out, void* stream) {
+    KvbEvictArgs a{};
+    int st = kvb_cache(cache, &a.src);
+    if (st) return st;
+    if (dst) {
+        st = kvb_cache(dst, &a.dst);
+        if (st) return st;
+        if (a.dst.slots != a.src.slots || a.dst.heads != a.src.heads || a.dst.hd != a.src.hd ||
+            a.dst.block != a.src.block || a.dst.k == a.src.k || a.dst.v == a.src.v || a.dst.ks == a.src.ks ||
+            a.dst.vs == a.src.vs || !dst_mass || dst_mass == mass)
+            return W8A8_EINVAL;
+    } else {
+        a.dst = a.src;
+    }
+    if (!mass || !count || !kept || !count_out || count == count_out || keep <= 0 || sink < 0 || recent < 0 ||
+        (int64_t)sink + recent > keep || keep > a.src.cap || keep > a.dst.cap)
+        return W8A8_EINVAL;
+    a.mass = mass, a.dst_mass = dst ? dst_mass : mass, a.in_place = dst == nullptr;
+    a.count = count, a.keep = keep, a.sink = sink, a.recent = recent, a.kept = kept, a.count_out = count_out;
+    return cuda_status(launch_kvb_evict(a, S(stream)));
 }
 
 }  // extern "C"

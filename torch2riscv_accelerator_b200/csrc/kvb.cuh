@@ -1,0 +1,158 @@
+// The block-scaled 8-bit KV cache (kvb.cu, kvb_attn.cu): codes int8
+// [slots][kv_heads][cap][hd] for K and V, one fp32 scale per (slot, KV head,
+// block of tokens): the value held is code * scale.
+#pragma once
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "pdl.cuh"
+
+namespace w8a8 {
+
+constexpr int kKvbMaxHd = 256;
+enum KvbType { KVB_F32 = 0, KVB_BF16 = 1, KVB_F16 = 2 };
+constexpr unsigned int kKvbErrCapacity = 128u;   // error bit 7: a row or a length past the capacity
+
+struct KvbCache {
+    int8_t* k;
+    int8_t* v;
+    float* ks;
+    float* vs;
+    int slots, heads, cap, hd, block;
+    int64_t slot_stride;                         // codes between slots
+    int64_t scale_stride;                        // scales between slots
+};
+
+// Rows of several sequences: slot b's are r0 .. r0 + n - 1, the first at cache
+// position pos[b]; start null: row b alone.
+struct KvbRows {
+    int rows;
+    const int32_t* pos;
+    const int32_t* start;
+};
+
+struct KvbSpan {
+    int r0, n, p;                                // first row, rows, position of the first (negative: idle)
+};
+
+// The offsets are data: clamped into [0, rows], so that no order of them
+// leads out of the row arrays.
+__device__ __forceinline__ KvbSpan kvb_span(const KvbRows& r, int b) {
+    KvbSpan s;
+    s.p = r.pos[b];
+    if (r.start) {
+        const int a = min(max(r.start[b], 0), r.rows), e = min(max(r.start[b + 1], 0), r.rows);
+        s.r0 = a, s.n = max(e - a, 0);
+    } else {
+        s.r0 = b, s.n = 1;
+    }
+    return s;
+}
+
+// The slot whose rows hold row r, or -1 (a row behind the last sequence):
+// the last b with start[b] <= r.
+__device__ __forceinline__ int kvb_slot_of(const KvbRows& w, int slots, int r) {
+    if (!w.start) return r;
+    int lo = 0, hi = slots;                      // start[lo] <= r < start[hi], if any
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (w.start[mid] <= r) lo = mid;
+        else hi = mid;
+    }
+    return w.start[lo] <= r && r < w.start[lo + 1] ? lo : -1;
+}
+
+struct KvbAppendArgs {
+    KvbCache c;
+    KvbRows r;
+    const void* k;
+    const void* v;
+    int64_t k_stride, v_stride;                  // elements between rows
+    int type;
+};
+struct KvbReadArgs {
+    KvbCache c;
+    KvbRows r;
+    void* k;
+    void* v;
+    int type;
+};
+struct KvbAttnArgs {
+    KvbCache c;
+    KvbRows r;
+    const void* q;                               // [rows][heads][hd], q_stride elements between rows
+    int64_t q_stride;
+    void* out;                                   // [rows][heads][hd]
+    int heads, type;
+    float scale;
+    float* mass;                                 // [slots][kv_heads][cap] or null
+    void* scratch;
+};
+struct KvbEvictArgs {
+    KvbCache src, dst;
+    const float* mass;                           // [slots][kv_heads][src.cap]
+    float* dst_mass;                             // [slots][kv_heads][dst.cap]
+    const int32_t* count;
+    int keep, sink, recent;
+    int32_t* kept;                               // [slots][kv_heads][keep]
+    int32_t* count_out;
+    int in_place;
+};
+
+cudaError_t launch_kvb_append(const KvbAppendArgs& a, cudaStream_t st);
+cudaError_t launch_kvb_read(const KvbReadArgs& a, cudaStream_t st);
+cudaError_t launch_kvb_evict(const KvbEvictArgs& a, cudaStream_t st);
+size_t kvb_attn_scratch(const KvbCache& c, int heads, int rows, bool one_row, bool mass);
+cudaError_t launch_kvb_attn(const KvbAttnArgs& a, cudaStream_t st);
+unsigned int kvb_read_clear_errors();
+unsigned int kvb_attn_read_clear_errors();
+
+template <typename T>
+__device__ __forceinline__ float kvb_f(T x);
+template <>
+__device__ __forceinline__ float kvb_f<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float kvb_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <>
+__device__ __forceinline__ float kvb_f<__half>(__half x) { return __half2float(x); }
+template <typename T>
+__device__ __forceinline__ T kvb_t(float x);
+template <>
+__device__ __forceinline__ float kvb_t<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 kvb_t<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half kvb_t<__half>(float x) { return __float2half_rn(x); }
+
+// 8 consecutive elements (16- or 32-byte aligned) as floats
+template <typename T>
+__device__ __forceinline__ void kvb_load8(const T* p, float* x) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    } else {
+        const uint4 a = *reinterpret_cast<const uint4*>(p);
+        T h[8];
+        *reinterpret_cast<uint4*>(h) = a;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = kvb_f<T>(h[i]);
+    }
+}
+
+// rint(num / den) saturated to +-127 as an int8 code, the quotient correctly
+// rounded before the rounding to an integer. The product with rcp ~ 1 / den is
+// within 3 ulp of the quotient (below 1e-4 for |quotient| <= 128), so only
+// values that close to a half need the division itself.
+__device__ __forceinline__ int kvb_code(float num, float den, float rcp) {
+    float y = __fmul_rn(num, rcp);
+    float q = rintf(y);
+    if (!(fabsf(fabsf(y - q) - 0.5f) > 1e-4f)) {
+        y = __fdiv_rn(num, den);
+        q = rintf(y);
+    }
+    return (int)fminf(fmaxf(q, -127.0f), 127.0f);
+}
+
+}  // namespace w8a8

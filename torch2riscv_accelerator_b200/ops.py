@@ -7,6 +7,7 @@ runs on the current torch CUDA stream and raises W8A8Error on a nonzero status.
 Tensors are passed as raw device pointers; torch only owns the memory.
 """
 import ctypes
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -66,7 +67,8 @@ def embed(tokens, emb_q, emb_s, out=None):
 
 
 def error_flags():
-    """Read and clear the device error flags (bit 0: an out-of-range token)."""
+    """Read and clear the device error flags (bit 0: an out-of-range token;
+    w8a8.h lists the others)."""
     v = ctypes.c_uint32(0)
     _lib.check("w8a8_error_flags", _lib.load().w8a8_error_flags(ctypes.byref(v)))
     return v.value
@@ -395,3 +397,208 @@ def dequant_resid(acc, s_x, s_w, out, resid=None):
                                                                    _p(out), _st()))
     return out
 
+
+
+# ------------------------------------------------- block-scaled 8-bit KV cache
+class KvBlocks(NamedTuple):
+    """One layer's cache in 8 bits with a scale per (slot, KV head, block of
+    tokens): codes k, v int8 [slots, kv_heads, capacity, head_dim] and scales
+    k_scale, v_scale fp32 [slots, kv_heads, capacity / block]; a value is
+    code * scale of its block. The kvb_ calls take any such 4-tuple; the slot
+    dimension may be strided (one layer of a [slots, layers, ...] cache)."""
+    k: torch.Tensor
+    k_scale: torch.Tensor
+    v: torch.Tensor
+    v_scale: torch.Tensor
+
+
+_KVB_TYPES = {F32: 0, torch.bfloat16: 1, torch.float16: 2}
+KVB_BLOCKS = (16, 32, 64, 128)
+
+
+def kvb_cache(slots, kv_heads, capacity, head_dim, block=64, device="cuda"):
+    """An empty cache; capacity is rounded up to whole blocks."""
+    if block not in KVB_BLOCKS:
+        raise ValueError(f"block {block}: one of {KVB_BLOCKS}")
+    blocks = -(-capacity // block)
+    codes = lambda: torch.zeros(slots, kv_heads, blocks * block, head_dim, dtype=I8, device=device)
+    scales = lambda: torch.zeros(slots, kv_heads, blocks, dtype=F32, device=device)
+    return KvBlocks(codes(), scales(), codes(), scales())
+
+
+def _kvb(cache, name="cache"):
+    """The checked W8A8KvBlocks of a cache."""
+    k, ks, v, vs = cache
+    S, H, T, D = k.shape
+    NB = ks.shape[2] if ks.dim() == 3 else 0
+    st, sc = k.stride(), ks.stride()
+    if k.dtype != I8 or v.dtype != I8 or ks.dtype != F32 or vs.dtype != F32:
+        raise ValueError(f"{name}: int8 codes and fp32 scales are required")
+    if v.shape != k.shape or ks.shape != (S, H, NB) or vs.shape != ks.shape or NB == 0 or T % NB:
+        raise ValueError(f"{name}: codes {tuple(k.shape)} / {tuple(v.shape)} and scales {tuple(ks.shape)} / "
+                         f"{tuple(vs.shape)} do not belong together")
+    if st[1:] != (T * D, D, 1) or sc[1:] != (NB, 1) or (S > 1 and (v.stride() != st or vs.stride() != sc)) or \
+            v.stride()[1:] != st[1:] or vs.stride()[1:] != sc[1:]:
+        raise ValueError(f"{name}: each slot's codes and scales must be contiguous, K's and V's alike")
+    dev = k.device
+    if dev.type != "cuda" or v.device != dev or ks.device != dev or vs.device != dev:
+        raise ValueError(f"{name}: CUDA tensors on one device are required")
+    return _lib.W8A8KvBlocks(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), S, H, T, D, T // NB, st[0],
+                             sc[0])
+
+
+def _kvb_index(t, n, dev, name):
+    if t.dtype != I32 or t.dim() != 1 or t.shape[0] != n or t.device != dev or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name}: a contiguous int32 [{n}] tensor on {dev} is required")
+
+
+def _kvb_rows(t, heads, hd, dev, name):
+    """(dtype code, elements between rows) of rows [rows, heads, hd] whose rows
+    are contiguous (a slice of a wider row is fine)."""
+    code = _KVB_TYPES.get(t.dtype)
+    if code is None or t.dim() != 3 or t.device != dev:
+        raise ValueError(f"{name}: fp32, bf16 or fp16 [rows, {heads}, {hd}] on {dev} is required")
+    st = t.stride()
+    if t.shape[2] != hd or (heads and t.shape[1] != heads) or st[2] != 1 or (t.shape[1] > 1 and st[1] != hd):
+        raise ValueError(f"{name}: [rows, {heads}, {hd}] with contiguous rows is required, got {tuple(t.shape)} "
+                         f"with strides {st}")
+    return code, st[0] if t.shape[0] > 1 else t.shape[1] * hd
+
+
+def _kvb_mass(t, k, name="mass"):
+    if t.dtype != F32 or t.shape != k.shape[:3] or not t.is_contiguous() or t.device != k.device:
+        raise ValueError(f"{name}: a contiguous fp32 {tuple(k.shape[:3])} tensor on {k.device} is required")
+
+
+def _kvb_call(fn, dev, *args):
+    """One C call on dev's current stream (the device made current for it)."""
+    i = dev.index
+    if i == torch.cuda.current_device():
+        rc = getattr(_lib.load(), fn)(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(dev):
+            rc = getattr(_lib.load(), fn)(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc:
+        _lib.check(fn, rc)
+
+
+def kvb_append(k, v, cache, pos, start=None):
+    """Rows k, v [rows, kv_heads, head_dim] into the cache: slot b's rows
+    start[b] .. start[b + 1] - 1 (start None: row b) at positions pos[b] on
+    (negative: an idle slot). A block's scale grows with its largest value; its
+    older codes are rescaled with it."""
+    c = _kvb(cache)
+    dev = cache[0].device
+    dt, ks = _kvb_rows(k, c.kv_heads, c.head_dim, dev, "k")
+    dv, vs = _kvb_rows(v, c.kv_heads, c.head_dim, dev, "v")
+    if dt != dv or k.shape[0] != v.shape[0]:
+        raise ValueError("k and v: the same type and number of rows are required")
+    _kvb_index(pos, c.slots, dev, "pos")
+    if start is not None:
+        _kvb_index(start, c.slots + 1, dev, "start")
+    _kvb_call("w8a8_kvb_append", dev, ctypes.byref(c), k.data_ptr(), ks, v.data_ptr(), vs, dt, k.shape[0],
+              pos.data_ptr(), None if start is None else start.data_ptr())
+
+
+def kvb_read(cache, pos, start, rows, dtype=F32, k=None, v=None):
+    """The values held at the rows' positions: k, v [rows, kv_heads, head_dim]
+    (zeros for idle slots; rows behind the last sequence are left alone)."""
+    c = _kvb(cache)
+    dev = cache[0].device
+    _kvb_index(pos, c.slots, dev, "pos")
+    if start is not None:
+        _kvb_index(start, c.slots + 1, dev, "start")
+    k = torch.empty(rows, c.kv_heads, c.head_dim, dtype=dtype, device=dev) if k is None else k
+    v = torch.empty(rows, c.kv_heads, c.head_dim, dtype=dtype, device=dev) if v is None else v
+    for t, name in ((k, "k"), (v, "v")):
+        if t.shape != (rows, c.kv_heads, c.head_dim) or not t.is_contiguous() or t.device != dev or t.dtype != dtype:
+            raise ValueError(f"{name}: a contiguous {dtype} {(rows, c.kv_heads, c.head_dim)} tensor is required")
+    if dtype not in _KVB_TYPES:
+        raise ValueError(f"dtype {dtype}: fp32, bf16 or fp16")
+    _kvb_call("w8a8_kvb_read", dev, ctypes.byref(c), rows, pos.data_ptr(),
+              None if start is None else start.data_ptr(), k.data_ptr(), v.data_ptr(), _KVB_TYPES[dtype])
+    return k, v
+
+
+def kvb_attn_scratch(cache, heads, rows, start=True, mass=False):
+    """Scratch for kvb_attn (start False) or kvb_attn_rows (True) calls of at
+    most `rows` rows; one per call that may overlap another."""
+    n = _lib.load().w8a8_kvb_attn_scratch_bytes(ctypes.byref(_kvb(cache)), heads, rows, int(not start), int(mass))
+    return torch.empty(n, dtype=torch.uint8, device=cache[0].device)
+
+
+def _kvb_attn(q, cache, pos, start, scale, mass, out, scratch):
+    c = _kvb(cache)
+    dev = cache[0].device
+    dt, qs = _kvb_rows(q, 0, c.head_dim, dev, "q")
+    rows, heads, hd = q.shape
+    _kvb_index(pos, c.slots, dev, "pos")
+    if start is not None:
+        _kvb_index(start, c.slots + 1, dev, "start")
+    if mass is not None:
+        _kvb_mass(mass, cache[0])
+    if out is None:
+        out = torch.empty((rows, heads, hd), dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev:
+        raise ValueError(f"out: a contiguous {q.dtype} {tuple(q.shape)} tensor is required")
+    if scratch is None:
+        n = _lib.load().w8a8_kvb_attn_scratch_bytes(ctypes.byref(c), heads, rows, int(start is None),
+                                                    int(mass is not None))
+        scratch = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    elif scratch.device != dev:
+        raise ValueError(f"scratch: a tensor on {dev} is required")
+    _kvb_call("w8a8_kvb_attn", dev, ctypes.byref(c), q.data_ptr(), qs, dt, heads, rows, pos.data_ptr(),
+              None if start is None else start.data_ptr(), hd ** -0.5 if scale is None else scale, out.data_ptr(),
+              None if mass is None else mass.data_ptr(), None if scratch is None else scratch.data_ptr(),
+              0 if scratch is None else scratch.numel())
+    return out
+
+
+def kvb_attn(q, cache, pos, scale=None, mass=None, out=None, scratch=None):
+    """Decode attention over the cache: row b of q [slots, heads, head_dim]
+    attends slot b's tokens 0 .. pos[b] (its own appended before); a negative
+    pos gives a zero row. scale: 1 / sqrt(head_dim) by default. mass (fp32
+    [slots, kv_heads, capacity]): each token's probabilities, summed over the
+    query heads of its KV head, are added to it. scratch: kvb_attn_scratch()
+    bytes of this call's own, or None to take them from torch's allocator."""
+    return _kvb_attn(q, cache, pos, None, scale, mass, out, scratch)
+
+
+def kvb_attn_rows(q, cache, pos, start, scale=None, mass=None, out=None, scratch=None):
+    """Prompt attention over the cache: slot b's rows start[b] .. start[b + 1]
+    - 1 of q [rows, heads, head_dim] stand at positions pos[b], pos[b] + 1, ...
+    and attend the tokens up to their own (all appended before). Rows behind
+    the last sequence are left as they are in `out`; the rest as kvb_attn."""
+    if start is None:
+        raise ValueError("start: an int32 [slots + 1] tensor is required")
+    return _kvb_attn(q, cache, pos, start, scale, mass, out, scratch)
+
+
+def kvb_evict(cache, mass, count, keep, sink=0, recent=0, dst=None, dst_mass=None):
+    """Cut every slot that holds more than `keep` tokens (count [slots]) to
+    `keep`: the first `sink`, the last `recent` and the heaviest by `mass` of
+    those between, moved together in their order; in place, or into dst /
+    dst_mass. Returns (kept [slots, kv_heads, keep] int32: each place's former
+    position, -1 past the new length; the new lengths [slots] int32)."""
+    c = _kvb(cache)
+    dev = cache[0].device
+    _kvb_mass(mass, cache[0])
+    _kvb_index(count, c.slots, dev, "count")
+    d = None
+    if dst is not None:
+        d = _kvb(dst, "dst")
+        if dst_mass is None:
+            raise ValueError("dst_mass: required with dst")
+        _kvb_mass(dst_mass, dst[0], "dst_mass")
+        if dst[0].device != dev:
+            raise ValueError(f"dst: a cache on {dev} is required")
+    elif dst_mass is not None:
+        raise ValueError("dst_mass: only with dst")
+    if not 0 < keep <= c.capacity:
+        raise ValueError(f"keep {keep}: 1 .. {c.capacity}")
+    kept = torch.empty(c.slots, c.kv_heads, keep, dtype=I32, device=dev)
+    left = torch.empty(c.slots, dtype=I32, device=dev)
+    _kvb_call("w8a8_kvb_evict", dev, ctypes.byref(c), mass.data_ptr(), count.data_ptr(), keep, sink, recent,
+              None if d is None else ctypes.byref(d), None if d is None else dst_mass.data_ptr(), kept.data_ptr(),
+              left.data_ptr())
+    return kept, left
