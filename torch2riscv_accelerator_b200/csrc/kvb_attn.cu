@@ -196,7 +196,11 @@ __device__ __forceinline__ int64_t step_scan(const KvbAttnArgs& a, int tile, int
     return x;
 }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool in) {
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// zeros instead of the source where it is not to be read
+__device__ __forceinline__ void cp16z(uint32_t dst, const void* src, bool in) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -228,21 +232,30 @@ __device__ __forceinline__ uint32_t halves_of(uint32_t x, uint32_t sel) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// A tile among the units: slot b, KV head h, head group gt, tile of the slot.
 struct StepIter {
-    int b, u, tile, tiles, len;
+    int b, h, gt, tile, tiles, len;
+    int64_t head;                                // first code of (b, h)
     __device__ __forceinline__ void load(const KvbAttnArgs& a, int tile_tokens) {
         len = step_len(a, b);
         tiles = (len + tile_tokens - 1) / tile_tokens;
+        head = b * a.c.slot_stride + (int64_t)h * a.c.cap * a.c.hd;
     }
-    __device__ __forceinline__ void next(const KvbAttnArgs& a, int units, int tile_tokens) {
-        if (++tile < tiles) return;
+    // the next unit; false past the last one
+    __device__ __forceinline__ bool next_unit(const KvbAttnArgs& a, int GT, int tile_tokens) {
         tile = 0;
-        if (++u < units) return;
-        u = 0;
+        if (++gt < GT) return true;
+        gt = 0;
+        if (++h < a.c.heads) {
+            head += (int64_t)a.c.cap * a.c.hd;
+            return true;
+        }
+        h = 0;
         do {
-            if (++b >= a.c.slots) return;
+            if (++b >= a.c.slots) return false;
             load(a, tile_tokens);
         } while (tiles == 0);
+        return true;
     }
 };
 
@@ -297,41 +310,70 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD>::CTAS) kvb_step_kernel(c
     __syncthreads();
     StepIter in, it;                             // the next tile to fetch, the tile at work
     it.b = s_b;
+    it.h = 0;
     it.load(a, C::TILE);
-    it.u = s_off / it.tiles, it.tile = s_off - it.u * it.tiles;
+    {
+        const int u = s_off / it.tiles;
+        it.tile = s_off - u * it.tiles;
+        it.h = u / GT, it.gt = u - it.h * GT;
+        it.head += (int64_t)it.h * a.c.cap * hd;
+    }
     in = it;
     int fetch = (int)(hi - lo), todo = fetch;
 
+    // Places in a stage without bank conflicts. K (a row's 16-byte chunk ch): the
+    // halves of odd rows' 128-byte lines are swapped, so that the two rows that
+    // eight lanes read together lie in different banks. V: ch ^ (row & 6), for
+    // eight lanes that read two neighbouring chunks of rows 0, 2, 4 and 6; with
+    // 64-byte rows two rows share a line and the line's number is folded in.
+    constexpr int RPI = 32 / CH;                 // rows per copy instruction of the warp
+    const int crow = lane / CH, ch = lane % CH;
+    const bool live_ch = ch * 16 < hd;
+    const uint32_t kdst = crow * HD + (HD == 64 ? ch : ch ^ ((crow & 1) << 2)) * 16;
+    const uint32_t vdst = HD == 64 ? (crow >> 1) * 128 + ((((crow & 1) * 4 + ch) ^ ((crow >> 1 & 3) << 1)) * 16)
+                                   : crow * HD + (ch ^ (crow & 6)) * 16;
+    const int lane_off = crow * hd + ch * 16;
     auto issue = [&](int stage) {
         if (fetch > 0) {
-            const uint32_t dst = smem_u32(ring + stage * C::STAGE);
-            const int h = in.u / GT, t0 = in.tile * C::TILE + warp * C::TOK;
-            const int64_t base = in.b * a.c.slot_stride + (int64_t)h * a.c.cap * hd;
+            const uint32_t dst = smem_u32(ring) + stage * C::STAGE;
+            const int t0 = in.tile * C::TILE + warp * C::TOK;
+            const int64_t at = in.head + (int64_t)t0 * hd + lane_off;
+            const int8_t *k = a.c.k + at, *v = a.c.v + at;
+            if (live_ch) {
+                if (t0 + C::TOK <= in.len) {
 #pragma unroll
-            for (int i = 0; i < C::TOK * CH / 32; ++i) {
-                const int idx = i * 32 + lane, row = idx / CH, ch = idx % CH, tok = t0 + row;
-                if (ch * 16 < hd) {
-                    const int64_t off = base + (int64_t)(tok < in.len ? tok : 0) * hd + ch * 16;
-                    // bank-conflict-free places: see the fragment loads below
-                    const int kc = HD == 64 ? ch : ch ^ ((row & 1) << 2);
-                    const int vrow = HD == 64 ? row >> 1 : row;
-                    const int vc = HD == 64 ? (((row & 1) * 4 + ch) ^ ((vrow & 3) << 1)) : ch ^ (row & 6);
-                    cp16(dst + row * HD + kc * 16, a.c.k + off, tok < in.len);
-                    cp16(dst + C::TOK * HD + vrow * (HD == 64 ? 128 : HD) + vc * 16, a.c.v + off, tok < in.len);
+                    for (int i = 0; i < C::TOK / RPI; ++i) {
+                        cp16(dst + kdst + i * RPI * HD, k + i * RPI * hd);
+                        cp16(dst + C::TOK * HD + i * RPI * HD + (vdst ^ (HD == 64 ? 0 : ((i * RPI) & 6) * 16)),
+                             v + i * RPI * hd);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < C::TOK / RPI; ++i) {
+                        const bool ok = t0 + i * RPI + crow < in.len;
+                        cp16z(dst + kdst + i * RPI * HD, ok ? k + i * RPI * hd : a.c.k, ok);
+                        cp16z(dst + C::TOK * HD + i * RPI * HD + (vdst ^ (HD == 64 ? 0 : ((i * RPI) & 6) * 16)),
+                              ok ? v + i * RPI * hd : a.c.v, ok);
+                    }
                 }
             }
             --fetch;
-            in.next(a, units, C::TILE);
+            if (++in.tile == in.tiles) in.next_unit(a, GT, C::TILE);
         }
         cp_commit();
     };
+    const int bsh = 31 - __clz(a.c.block);
+    // the fragments' places: lane (g, t) reads K chunk 4 c + t of row g, V's
+    // run of channels g of rows 2t, 2t + 1, 2t + 8, 2t + 9
+    const int kfrag = g * HD + (HD == 64 ? t : t ^ ((g & 1) << 2)) * 16;
+    const int vfrag = HD == 64 ? t * 128 + (((g >> 1) ^ (t << 1)) * 16) + (g & 1) * 8 : 2 * t * HD + (g ^ (2 * t)) * 16;
 #pragma unroll
     for (int i = 0; i < C::NST - 1; ++i) issue(i);
 
     int stage = 0;
     while (todo > 0) {
         // one unit, or what of it lies in this share
-        const int b = it.b, u = it.u, h = u / GT, j0 = (u - h * GT) * kGroup, first = it.tile;
+        const int b = it.b, h = it.h, j0 = it.gt * kGroup, first = it.tile;
         const int live = min(G - j0, kGroup), head = h * G + j0 + g;
         const int n_it = min(todo, it.tiles - first);
         const bool whole = first == 0 && n_it == it.tiles;
@@ -393,19 +435,27 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD>::CTAS) kvb_step_kernel(c
             }
         }
 
-        float o[NV][4], m = -INFINITY, l = 0.0f, svm = 0.0f;
+        float o[NV][4], m = -INFINITY, l = 0.0f, svm = 0.0f, rsv = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
 
-        for (int n = 0; n < n_it; ++n) {
-            const int t0 = (first + n) * C::TILE + warp * C::TOK;
-            float sk[KT], sv[KT];
+        const float *ksc = a.c.ks + sc, *vsc = a.c.vs + sc;
+        float sk[KT], sv[KT];                    // a step's 16 tokens lie in one block; loaded a tile ahead
+        auto scales = [&](int t0) {
 #pragma unroll
             for (int k = 0; k < KT; ++k) {
                 const bool in_len = t0 + k * 16 < len;
-                sk[k] = in_len ? a.c.ks[sc + (t0 + k * 16) / a.c.block] : 0.0f;
-                sv[k] = in_len ? a.c.vs[sc + (t0 + k * 16) / a.c.block] : 0.0f;
+                sk[k] = in_len ? ksc[(t0 + k * 16) >> bsh] : 0.0f;
+                sv[k] = in_len ? vsc[(t0 + k * 16) >> bsh] : 0.0f;
             }
+        };
+        scales(first * C::TILE + warp * C::TOK);
+        for (int n = 0; n < n_it; ++n) {
+            const int t0 = (first + n) * C::TILE + warp * C::TOK;
+            float fk[KT], fs[KT];
+#pragma unroll
+            for (int k = 0; k < KT; ++k) fk[k] = sk[k] * qs, fs[k] = sv[k];
+            if (n + 1 < n_it) scales(t0 + C::TILE);
             cp_wait<C::NST - 2>();
             __syncwarp();                        // this stage has landed, the one before it is free
             int fill = stage + C::NST - 1;
@@ -422,23 +472,24 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD>::CTAS) kvb_step_kernel(c
                         int c1[4] = {0, 0, 0, 0}, c2[4] = {0, 0, 0, 0};
 #pragma unroll
                         for (int c = 0; c < HD / 64; ++c) {
-                            // rows of a phase alternate between the line's halves
-                            const int row = k * 16 + j * 8 + g, ch = 4 * c + t;
-                            const int kc = HD == 64 ? ch : ch ^ ((row & 1) << 2);
-                            const uint4 w = *reinterpret_cast<const uint4*>(ks + row * HD + kc * 16);
+                            const uint4 w = *reinterpret_cast<const uint4*>(ks + (k * 16 + j * 8) * HD + (c >> 1) * 128 +
+                                                                             (kfrag ^ ((c & 1) * 64)));
                             mma_s8(c1, qh[c][0][0], qh[c][0][1], qh[c][0][2], qh[c][0][3], w.x, w.y);
                             mma_s8(c1, qh[c][1][0], qh[c][1][1], qh[c][1][2], qh[c][1][3], w.z, w.w);
                             mma_s8(c2, ql[c][0][0], 0u, ql[c][0][1], 0u, w.x, w.y);
                             mma_s8(c2, ql[c][1][0], 0u, ql[c][1][1], 0u, w.z, w.w);
                         }
-                        const float f = sk[k] * qs;
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int tok = t0 + k * 16 + j * 8 + 2 * t + e;
-                            const float s = fmaf((float)c1[e], 65536.0f, (float)(c1[2 + e] * 256 + c2[e]));
-                            z[k][2 * j + e] = tok < len ? s * f : -INFINITY;
-                        }
+                        for (int e = 0; e < 2; ++e)
+                            z[k][2 * j + e] = fmaf((float)c1[e], 65536.0f, (float)(c1[2 + e] * 256 + c2[e])) * fk[k];
                     }
+                if (t0 + C::TOK > len) {
+#pragma unroll
+                    for (int k = 0; k < KT; ++k)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (t0 + k * 16 + (e >> 1) * 8 + 2 * t + (e & 1) >= len) z[k][e] = -INFINITY;
+                }
                 if (scores && g < live) {
                     float* zr = scores + ((int64_t)b * a.heads + head) * a.c.cap + t0 + 2 * t;
 #pragma unroll
@@ -454,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD>::CTAS) kvb_step_kernel(c
                 for (int k = 0; k < KT; ++k) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) mx = fmaxf(mx, z[k][e]);
-                    smx = fmaxf(smx, sv[k]);
+                    smx = fmaxf(smx, fs[k]);
                 }
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
@@ -464,10 +515,11 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD>::CTAS) kvb_step_kernel(c
 #pragma unroll
                     for (int i = 0; i < NV; ++i) o[i][0] *= eo, o[i][1] *= eo, o[i][2] *= eo, o[i][3] *= eo;
                     m = mx, svm = smx;
+                    rsv = svm > 1e-33f ? 32768.0f / svm : 0.0f;   // values below count as 0
                 }
 #pragma unroll
                 for (int k = 0; k < KT; ++k) {
-                    const float fv = svm > 0.0f ? sv[k] / svm * 32768.0f : 0.0f;
+                    const float fv = fs[k] * rsv;
                     uint32_t p[4];               // hi | lo of tokens 2t, 2t + 1, then of 8 + 2t, 8 + 2t + 1
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
@@ -487,14 +539,13 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD>::CTAS) kvb_step_kernel(c
                         uint32_t v[4][RUN / 4];
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
-                            const int row = k * 16 + 2 * t + (q & 1) + (q >> 1) * 8;
                             if constexpr (HD == 64) {
-                                const int line = row >> 1, pc = ((row & 1) * 4 + (g >> 1)) ^ ((line & 3) << 1);
-                                const uint2 w = *reinterpret_cast<const uint2*>(vs + line * 128 + pc * 16 + (g & 1) * 8);
+                                const uint2 w = *reinterpret_cast<const uint2*>(vs + k * 1024 + (q >> 1) * 512 +
+                                                                                (vfrag ^ ((q & 1) * 64)));
                                 v[q][0] = w.x ^ 0x80808080u, v[q][1] = w.y ^ 0x80808080u;
                             } else {
-                                const int pc = (r * 8 + g) ^ (row & 6);
-                                const uint4 w = *reinterpret_cast<const uint4*>(vs + row * HD + pc * 16);
+                                const uint4 w = *reinterpret_cast<const uint4*>(
+                                    vs + (k * 16 + (q & 1) + (q >> 1) * 8) * HD + r * 128 + vfrag);
                                 v[q][0] = w.x ^ 0x80808080u, v[q][1] = w.y ^ 0x80808080u;
                                 v[q][2] = w.z ^ 0x80808080u, v[q][3] = w.w ^ 0x80808080u;
                             }
@@ -560,8 +611,7 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD>::CTAS) kvb_step_kernel(c
             }
         }
         todo -= n_it;
-        it.tile += n_it - 1;
-        it.next(a, units, C::TILE);
+        it.next_unit(a, GT, C::TILE);            // a unit that is cut ends the share
     }
     cp_wait<0>();
 }
