@@ -135,38 +135,43 @@ __global__ void __launch_bounds__(kThreads) kvb_mass_kernel(const KvbAttnArgs a)
 // ---------------------------------------------------------------- one row per slot
 // The cache is streamed once; everything else is small, so DRAM bounds it.
 //
-// Work: a unit is one (slot, KV head, group of 8 query heads); its tokens come
+// Work: a unit is one (slot, KV head, group of GC query heads); its tokens come
 // in tiles of 64 KT. All units' tiles, in order, are dealt out in equal
 // contiguous shares to a fixed grid, so that lengths of any mix load every SM
 // alike and the scratch does not grow with the capacity: a CTA leaves at most
 // two partial units (its first and its last), which kvb_step_finish joins.
 //
 // A warp takes 16 KT tokens of a tile through its own ring of shared-memory
-// stages (cp.async, no block barrier in the loop) and keeps its own running
-// maximum, sum and outputs:
-//   scores   mma m16n8k32 on the int8 codes as they lie. The query row is taken
-//            to 24-bit fixed point of its largest element, its three signed
-//            8-bit digits are rows of the A operand (hi: rows 0-7, mid: 8-15 of
-//            the first product, lo: rows 0-7 of a second): integer sums are exact
-//            and the codes need no conversion.
-//   outputs  mma m16n8k16 in fp16 with fp32 sums: the codes become fp16 exactly
-//            (byte permutes), the weights 2^15 p sv / sv_max enter as hi + lo
-//            halves (22 bits) in rows 0-7 and 8-15; sv_max is the warp's
-//            largest V scale so far, so that weights stay in fp16's range.
+// stages (cp.async, no block barrier in the loop) and keeps its own maxima,
+// sums and outputs. The cache is the 16-row operand of both products, the
+// query heads are their 8 columns:
+//   scores   mma m16n8k32 on the int8 codes as they lie (16 tokens x 32
+//            channels). The query row is taken to 24-bit fixed point of its
+//            largest element; its three signed 8-bit digits make three
+//            products (column n: head n % GC), whose integer sums are exact.
+//   outputs  mma m16n8k16 in fp16 with fp32 sums (16 channels x 16 tokens): the
+//            codes become halves exactly (byte permutes and one subtraction),
+//            the weights enter as hi + lo halves (22 bits), in columns of
+//            their own where GC leaves room.
+// Maxima move lazily: a warp rescales when a score passes its head's reference
+// by 2^6 or a block's V scale its reference by 2^2; the weights
+// exp(z - m) sv / sv_ref 2^7 then stay below 2^15.
 constexpr int kStepWarps = 4;
-constexpr int kGroup = 8;                        // query heads of a unit (rows of the products)
 constexpr int kMaxParts = 2;                     // partial units per CTA
+constexpr float kLazyScore = 6.0f, kLazyScale = 4.0f, kWeightScale = 128.0f;
 
-template <int HD>
+template <int HD, int GC>
 struct StepCfg {
     static constexpr int KT = HD == 64 ? 2 : 1;  // 16-token steps per warp and tile
     static constexpr int TOK = 16 * KT;          // tokens per warp and tile
     static constexpr int TILE = TOK * kStepWarps;
+    static constexpr int CTAS = HD == 256 ? 2 : GC == 8 && HD == 128 ? 3 : 4;
     static constexpr int NST = HD == 256 ? 2 : 3;
     static constexpr int STAGE = 2 * TOK * HD;   // bytes: K rows, V rows
     static constexpr int RING = NST * STAGE;     // per warp
-    static constexpr int CTAS = HD == 256 ? 2 : 3;
-    static constexpr size_t SMEM = (size_t)kStepWarps * RING + kStepWarps * kGroup * (HD + 2) * sizeof(float);
+    static constexpr int NP = GC == 8 ? 2 : 1;   // column tiles of the weights
+    static constexpr size_t PART = (size_t)GC * (HD + 2);   // floats of a partial unit: outputs, maximum, sum
+    static constexpr size_t SMEM = (size_t)kStepWarps * (RING + PART * sizeof(float));
 };
 
 // CTAs with a share: each at least one tile.
@@ -214,11 +219,37 @@ __device__ __forceinline__ void mma_s8(int* c, uint32_t a0, uint32_t a1, uint32_
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// an 8 x 8 matrix of halves transposed across the warp
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+// 16 consecutive elements of a row of type `type`
+__device__ __forceinline__ void load16(const void* base, int type, int64_t at, float* y) {
+    if (type == KVB_F32) {
+        kvb_load8<float>(static_cast<const float*>(base) + at, y);
+        kvb_load8<float>(static_cast<const float*>(base) + at + 8, y + 8);
+    } else if (type == KVB_BF16) {
+        kvb_load8<__nv_bfloat16>(static_cast<const __nv_bfloat16*>(base) + at, y);
+        kvb_load8<__nv_bfloat16>(static_cast<const __nv_bfloat16*>(base) + at + 8, y + 8);
+    } else {
+        kvb_load8<__half>(static_cast<const __half*>(base) + at, y);
+        kvb_load8<__half>(static_cast<const __half*>(base) + at + 8, y + 8);
+    }
+}
+__device__ __forceinline__ void store1(void* base, int type, int64_t at, float y) {
+    if (type == KVB_F32) static_cast<float*>(base)[at] = y;
+    else if (type == KVB_BF16) static_cast<__nv_bfloat16*>(base)[at] = __float2bfloat16_rn(y);
+    else static_cast<__half*>(base)[at] = __float2half_rn(y);
 }
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -259,17 +290,15 @@ struct StepIter {
     }
 };
 
-__host__ __device__ __forceinline__ size_t step_part_floats(int hd_pad) { return (size_t)kGroup * (hd_pad + 2); }
-
-template <int HD, typename T>
-__global__ void __launch_bounds__(kThreads, StepCfg<HD>::CTAS) kvb_step_kernel(const KvbAttnArgs a, float* parts,
-                                                                             float* scores) {
-    using C = StepCfg<HD>;
-    constexpr int KT = C::KT, NV = HD / 8, CH = HD / 16;
+template <int HD, int GC>
+__global__ void __launch_bounds__(kThreads, StepCfg<HD, GC>::CTAS) kvb_step_kernel(const KvbAttnArgs a, float* parts,
+                                                                                 float* scores) {
+    using C = StepCfg<HD, GC>;
+    constexpr int KT = C::KT, CH = HD / 16, MT = HD / 16;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ int s_b, s_off;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32, g = lane >> 2, t = lane & 3;
-    const int hd = a.c.hd, G = a.heads / a.c.heads, GT = (G + kGroup - 1) / kGroup, units = a.c.heads * GT;
+    const int hd = a.c.hd, G = a.heads / a.c.heads, GT = (G + GC - 1) / GC, units = a.c.heads * GT;
     unsigned char* ring = smem + warp * C::RING;
     float* merge = reinterpret_cast<float*>(smem + kStepWarps * C::RING);
     if (hd < HD) {                               // channels past the head stay zero
@@ -373,46 +402,41 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD>::CTAS) kvb_step_kernel(c
     int stage = 0;
     while (todo > 0) {
         // one unit, or what of it lies in this share
-        const int b = it.b, h = it.h, j0 = it.gt * kGroup, first = it.tile;
-        const int live = min(G - j0, kGroup), head = h * G + j0 + g;
+        const int b = it.b, h = it.h, j0 = it.gt * GC, first = it.tile;
+        const int live = min(G - j0, GC), jg = g % GC;         // heads of the unit; the one this lane quantizes
         const int n_it = min(todo, it.tiles - first);
         const bool whole = first == 0 && n_it == it.tiles;
         const int64_t sc = b * a.c.scale_stride + (int64_t)h * (a.c.cap / a.c.block);
         const int len = it.len;
 
-        uint32_t qh[HD / 64][2][4], ql[HD / 64][2][2];
-        float qs;
+        uint32_t qd[3][HD / 64][2][2];           // digit (high first), 64 channels, k step, operand word
+        float qsa, qsb;                          // score factors of this lane's columns' heads
         {
-            const T* qr = static_cast<const T*>(a.q) + b * a.q_stride + (int64_t)head * hd;
+            const int64_t qr = b * a.q_stride + (int64_t)(h * G + j0 + jg) * hd;
             float mx = 0.0f;
             bool nan = false;
 #pragma unroll
             for (int c = 0; c < HD / 64; ++c)
-                if (g < live && c * 64 + t * 16 < hd) {
+                if (jg < live && c * 64 + t * 16 < hd) {
                     float y[16];
-                    kvb_load8<T>(qr + c * 64 + t * 16, y);
-                    kvb_load8<T>(qr + c * 64 + t * 16 + 8, y + 8);
+                    load16(a.q, a.type, qr + c * 64 + t * 16, y);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fabsf(y[i])), nan |= isnan(y[i]);
+                    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fabsf(y[i])), nan |= !(fabsf(y[i]) <= 3.402823466e38f);
                 }
-            if (nan) mx = NAN;
-            const float m1 = __shfl_xor_sync(0xffffffffu, mx, 1);
-            mx = isnan(mx) || isnan(m1) ? NAN : fmaxf(mx, m1);
-            const float m2 = __shfl_xor_sync(0xffffffffu, mx, 2);
-            mx = isnan(mx) || isnan(m2) ? NAN : fmaxf(mx, m2);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const unsigned int bad = __ballot_sync(0xffffffffu, nan);
             const float up = mx > 0.0f ? 8355711.0f / mx : 0.0f;         // 0x7F7F7F: the largest three digits
-            qs = mx * (1.0f / 8355711.0f) * a.scale * kLog2e;            // NaN and infinite rows give NaN
-            if (isinf(mx)) qs = NAN;
+            float qs = mx * (1.0f / 8355711.0f) * a.scale * kLog2e;
+            if (bad >> (lane & ~3) & 15u) qs = NAN;                      // a NaN or infinite row gives NaN
+            qsa = __shfl_sync(0xffffffffu, qs, (2 * t) % GC * 4);
+            qsb = __shfl_sync(0xffffffffu, qs, (2 * t + 1) % GC * 4);
 #pragma unroll
             for (int c = 0; c < HD / 64; ++c) {
                 float y[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) y[i] = 0.0f;
-                if (g < live && c * 64 + t * 16 < hd) {
-                    kvb_load8<T>(qr + c * 64 + t * 16, y);
-                    kvb_load8<T>(qr + c * 64 + t * 16 + 8, y + 8);
-                }
-                uint32_t d[3][4];
+                if (jg < live && c * 64 + t * 16 < hd) load16(a.q, a.type, qr + c * 64 + t * 16, y);
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
                     uint32_t v[4];
@@ -422,22 +446,20 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD>::CTAS) kvb_step_kernel(c
                         v[i] = ((uint32_t)__float2int_rn(x) + 0x808080u) ^ 0x808080u;   // three signed digits
                     }
                     const uint32_t x01 = __byte_perm(v[0], v[1], 0x5140), x23 = __byte_perm(v[2], v[3], 0x5140);
-                    d[2][w] = __byte_perm(x01, x23, 0x5410);             // low digits of the four
-                    d[1][w] = __byte_perm(x01, x23, 0x7632);             // middle ones
-                    d[0][w] = __byte_perm(__byte_perm(v[0], v[1], 0x0062), __byte_perm(v[2], v[3], 0x0062), 0x5410);
-                }
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    qh[c][s][0] = d[0][2 * s], qh[c][s][1] = d[1][2 * s];
-                    qh[c][s][2] = d[0][2 * s + 1], qh[c][s][3] = d[1][2 * s + 1];
-                    ql[c][s][0] = d[2][2 * s], ql[c][s][1] = d[2][2 * s + 1];
+                    qd[2][c][w >> 1][w & 1] = __byte_perm(x01, x23, 0x5410);
+                    qd[1][c][w >> 1][w & 1] = __byte_perm(x01, x23, 0x7632);
+                    qd[0][c][w >> 1][w & 1] =
+                        __byte_perm(__byte_perm(v[0], v[1], 0x0062), __byte_perm(v[2], v[3], 0x0062), 0x5410);
                 }
             }
         }
 
-        float o[NV][4], m = -INFINITY, l = 0.0f, svm = 0.0f, rsv = 0.0f;
+        // outputs: channel tile i, column tile; maxima and sums of the lane's two heads
+        float o[MT][C::NP][4], ma = -INFINITY, mb = -INFINITY, la = 0.0f, lb = 0.0f, svr = 0.0f, rsv = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int x = 0; x < C::NP; ++x) o[i][x][0] = o[i][x][1] = o[i][x][2] = o[i][x][3] = 0.0f;
 
         const float *ksc = a.c.ks + sc, *vsc = a.c.vs + sc;
         float sk[KT], sv[KT];                    // a step's 16 tokens lie in one block; loaded a tile ahead
@@ -454,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD>::CTAS) kvb_step_kernel(c
             const int t0 = (first + n) * C::TILE + warp * C::TOK;
             float fk[KT], fs[KT];
 #pragma unroll
-            for (int k = 0; k < KT; ++k) fk[k] = sk[k] * qs, fs[k] = sv[k];
+            for (int k = 0; k < KT; ++k) fk[k] = sk[k], fs[k] = sv[k];
             if (n + 1 < n_it) scales(t0 + C::TILE);
             cp_wait<C::NST - 2>();
             __syncwarp();                        // this stage has landed, the one before it is free
@@ -464,75 +486,87 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD>::CTAS) kvb_step_kernel(c
             if (t0 < len) {
                 const unsigned char* ks = ring + stage * C::STAGE;
                 const unsigned char* vs = ks + C::TOK * HD;
-                float z[KT][4];                  // [k][2 j + e]: token 16 k + 8 j + 2 t + e of head g
+                float z[KT][4];                  // tokens g, g + 8 of step k: first head, second head
 #pragma unroll
-                for (int k = 0; k < KT; ++k)
+                for (int k = 0; k < KT; ++k) {
+                    int c0[4] = {0, 0, 0, 0}, c1[4] = {0, 0, 0, 0}, c2[4] = {0, 0, 0, 0};
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        int c1[4] = {0, 0, 0, 0}, c2[4] = {0, 0, 0, 0};
-#pragma unroll
-                        for (int c = 0; c < HD / 64; ++c) {
-                            const uint4 w = *reinterpret_cast<const uint4*>(ks + (k * 16 + j * 8) * HD + (c >> 1) * 128 +
-                                                                             (kfrag ^ ((c & 1) * 64)));
-                            mma_s8(c1, qh[c][0][0], qh[c][0][1], qh[c][0][2], qh[c][0][3], w.x, w.y);
-                            mma_s8(c1, qh[c][1][0], qh[c][1][1], qh[c][1][2], qh[c][1][3], w.z, w.w);
-                            mma_s8(c2, ql[c][0][0], 0u, ql[c][0][1], 0u, w.x, w.y);
-                            mma_s8(c2, ql[c][1][0], 0u, ql[c][1][1], 0u, w.z, w.w);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            z[k][2 * j + e] = fmaf((float)c1[e], 65536.0f, (float)(c1[2 + e] * 256 + c2[e])) * fk[k];
+                    for (int c = 0; c < HD / 64; ++c) {
+                        const unsigned char* kr = ks + k * 16 * HD + (c >> 1) * 128 + (kfrag ^ ((c & 1) * 64));
+                        const uint4 u = *reinterpret_cast<const uint4*>(kr);
+                        const uint4 w = *reinterpret_cast<const uint4*>(kr + 8 * HD);
+                        mma_s8(c0, u.x, w.x, u.y, w.y, qd[0][c][0][0], qd[0][c][0][1]);
+                        mma_s8(c1, u.x, w.x, u.y, w.y, qd[1][c][0][0], qd[1][c][0][1]);
+                        mma_s8(c2, u.x, w.x, u.y, w.y, qd[2][c][0][0], qd[2][c][0][1]);
+                        mma_s8(c0, u.z, w.z, u.w, w.w, qd[0][c][1][0], qd[0][c][1][1]);
+                        mma_s8(c1, u.z, w.z, u.w, w.w, qd[1][c][1][0], qd[1][c][1][1]);
+                        mma_s8(c2, u.z, w.z, u.w, w.w, qd[2][c][1][0], qd[2][c][1][1]);
                     }
+                    const float fa = fk[k] * qsa, fb = fk[k] * qsb;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        z[k][e] = fmaf((float)c0[e], 65536.0f, (float)(c1[e] * 256 + c2[e])) * (e & 1 ? fb : fa);
+                }
                 if (t0 + C::TOK > len) {
 #pragma unroll
                     for (int k = 0; k < KT; ++k)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            if (t0 + k * 16 + (e >> 1) * 8 + 2 * t + (e & 1) >= len) z[k][e] = -INFINITY;
+                            if (t0 + k * 16 + (e >> 1) * 8 + g >= len) z[k][e] = -INFINITY;
                 }
-                if (scores && g < live) {
-                    float* zr = scores + ((int64_t)b * a.heads + head) * a.c.cap + t0 + 2 * t;
+                if (scores) {
 #pragma unroll
-                    for (int k = 0; k < KT; ++k)
+                    for (int e = 0; e < 2; ++e)
+                        if (2 * t + e < live) {
+                            float* zr = scores + ((int64_t)b * a.heads + h * G + j0 + 2 * t + e) * a.c.cap + t0 + g;
 #pragma unroll
-                        for (int j = 0; j < 2; ++j)
-                            if (t0 + k * 16 < len)
-                                *reinterpret_cast<float2*>(zr + k * 16 + j * 8) =
-                                    make_float2(z[k][2 * j], z[k][2 * j + 1]);
+                            for (int k = 0; k < KT; ++k)
+                                if (t0 + k * 16 < len) zr[k * 16] = z[k][e], zr[k * 16 + 8] = z[k][2 + e];
+                        }
                 }
-                float mx = m, smx = svm;
-#pragma unroll
-                for (int k = 0; k < KT; ++k) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) mx = fmaxf(mx, z[k][e]);
-                    smx = fmaxf(smx, fs[k]);
+                float xa = fmaxf(z[0][0], z[0][2]), xb = fmaxf(z[0][1], z[0][3]), xs = fs[0];
+                if constexpr (KT == 2) {
+                    xa = fmaxf(xa, fmaxf(z[1][0], z[1][2])), xb = fmaxf(xb, fmaxf(z[1][1], z[1][3]));
+                    xs = fmaxf(xs, fs[1]);
                 }
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                if (__any_sync(0xffffffffu, mx != m || smx != svm)) {
-                    const float el = ex2(m - mx), eo = smx > 0.0f ? el * (svm / smx) : 0.0f;
-                    l *= el;
+                if (__any_sync(0xffffffffu, xa > ma + kLazyScore || xb > mb + kLazyScore || xs > svr * kLazyScale)) {
 #pragma unroll
-                    for (int i = 0; i < NV; ++i) o[i][0] *= eo, o[i][1] *= eo, o[i][2] *= eo, o[i][3] *= eo;
-                    m = mx, svm = smx;
-                    rsv = svm > 1e-33f ? 32768.0f / svm : 0.0f;   // values below count as 0
+                    for (int d = 4; d < 32; d <<= 1) {
+                        xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, d));
+                        xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, d));
+                    }
+                    xa = fmaxf(xa, ma), xb = fmaxf(xb, mb), xs = fmaxf(xs, svr);
+                    const float ea = xa == ma ? 1.0f : ex2(ma - xa), eb = xb == mb ? 1.0f : ex2(mb - xb);
+                    const float es = xs > 0.0f ? svr / xs : 0.0f, oa = ea * es, ob = eb * es;
+                    la *= ea, lb *= eb;
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int x = 0; x < C::NP; ++x)
+                            o[i][x][0] *= oa, o[i][x][1] *= ob, o[i][x][2] *= oa, o[i][x][3] *= ob;
+                    ma = xa, mb = xb, svr = xs;
+                    rsv = svr > 1e-33f ? kWeightScale / svr : 0.0f;      // values below count as 0
                 }
 #pragma unroll
                 for (int k = 0; k < KT; ++k) {
                     const float fv = fs[k] * rsv;
-                    uint32_t p[4];               // hi | lo of tokens 2t, 2t + 1, then of 8 + 2t, 8 + 2t + 1
+                    uint32_t pb[C::NP][2];       // the weights as the products' columns
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const float e0 = ex2(z[k][2 * j] - m), e1 = ex2(z[k][2 * j + 1] - m);
-                        l += e0 + e1;
-                        const float w0 = e0 * fv, w1 = e1 * fv;
-                        const __half2 hi2 = __floats2half2_rn(w0, w1);
-                        const float2 back = __half22float2(hi2);
-                        const __half2 lo2 = __floats2half2_rn(w0 - back.x, w1 - back.y);
-                        p[2 * j] = *reinterpret_cast<const uint32_t*>(&hi2);
-                        p[2 * j + 1] = *reinterpret_cast<const uint32_t*>(&lo2);
+                    for (int j = 0; j < 2; ++j) {                        // tokens g, then g + 8
+                        const float ea = ex2(z[k][2 * j] - ma), eb = ex2(z[k][2 * j + 1] - mb);
+                        la += ea, lb += eb;
+                        const float wa = ea * fv, wb = eb * fv;
+                        const __half2 hi = __floats2half2_rn(wa, wb);
+                        const float2 back = __half22float2(hi);
+                        const __half2 lo = __floats2half2_rn(wa - back.x, wb - back.y);
+                        if constexpr (GC == 8) {
+                            pb[0][j] = transpose8(bits(hi)), pb[1][j] = transpose8(bits(lo));
+                        } else {                 // columns [0, GC): hi, [GC, 2 GC): lo
+                            const uint32_t x = t * 2 < GC ? bits(hi) : t * 2 < 2 * GC ? bits(lo) : 0u;
+                            pb[0][j] = transpose8(x);
+                        }
                     }
-                    // V rows 2t, 2t + 1, 2t + 8, 2t + 9 of this step, NV channels each (HD / 128 runs of 16, or 8)
+                    // V rows 2t, 2t + 1, 2t + 8, 2t + 9 of this step, RUN channels each
                     constexpr int RUN = HD == 64 ? 8 : 16, RUNS = HD == 256 ? 2 : 1;
 #pragma unroll
                     for (int r = 0; r < RUNS; ++r) {
@@ -552,15 +586,20 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD>::CTAS) kvb_step_kernel(c
                         }
 #pragma unroll
                         for (int w = 0; w < RUN / 4; ++w) {
+                            // a product's 16 rows: two channels of every lane group, tokens in pairs
                             const uint32_t a01 = __byte_perm(v[0][w], v[1][w], 0x5140);
                             const uint32_t a23 = __byte_perm(v[0][w], v[1][w], 0x7362);
                             const uint32_t b01 = __byte_perm(v[2][w], v[3][w], 0x5140);
                             const uint32_t b23 = __byte_perm(v[2][w], v[3][w], 0x7362);
-                            float(*oo)[4] = o + r * 16 + w * 4;
-                            mma_f16(oo[0], p, halves_of(a01, 0x4140), halves_of(b01, 0x4140));
-                            mma_f16(oo[1], p, halves_of(a01, 0x4342), halves_of(b01, 0x4342));
-                            mma_f16(oo[2], p, halves_of(a23, 0x4140), halves_of(b23, 0x4140));
-                            mma_f16(oo[3], p, halves_of(a23, 0x4342), halves_of(b23, 0x4342));
+                            const uint32_t x0 = halves_of(a01, 0x4140), x1 = halves_of(a01, 0x4342);
+                            const uint32_t x2 = halves_of(b01, 0x4140), x3 = halves_of(b01, 0x4342);
+                            const uint32_t y0 = halves_of(a23, 0x4140), y1 = halves_of(a23, 0x4342);
+                            const uint32_t y2 = halves_of(b23, 0x4140), y3 = halves_of(b23, 0x4342);
+#pragma unroll
+                            for (int x = 0; x < C::NP; ++x) {
+                                mma_f16(o[r * 8 + 2 * w][x], x0, x1, x2, x3, pb[x][0], pb[x][1]);
+                                mma_f16(o[r * 8 + 2 * w + 1][x], y0, y1, y2, y3, pb[x][0], pb[x][1]);
+                            }
                         }
                     }
                 }
@@ -568,27 +607,40 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD>::CTAS) kvb_step_kernel(c
             if (++stage == C::NST) stage = 0;
         }
 
-        // the warps' states joined: merge[warp][head][HD | m, l]
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        // the warps' states joined: merge[warp][head][HD | maximum, sum]
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+            la += __shfl_xor_sync(0xffffffffu, la, d);
+            lb += __shfl_xor_sync(0xffffffffu, lb, d);
+        }
         __syncthreads();                         // the last unit's readers are done
-        if (g < live) {
-            float* w = merge + (warp * kGroup + g) * (HD + 2);
-            const float f = svm * (1.0f / 32768.0f);
+        {
+            const float f = svr * (1.0f / kWeightScale);
             constexpr int RUN = HD == 64 ? 8 : 16;
+            float* wa = merge + (warp * GC + (2 * t) % GC) * (HD + 2);
+            const bool mine = 2 * t < GC;        // the columns of the lo halves are added to the hi ones'
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
+            for (int i = 0; i < MT; ++i) {
+                float y[4];
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    w[(i / RUN) * 128 + RUN * (2 * t + e) + i % RUN] = (o[i][e] + o[i][2 + e]) * f;
-            if (t == 0) w[HD] = m, w[HD + 1] = l;
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (GC == 8) y[e] = o[i][0][e] + o[i][1][e];
+                    else y[e] = o[i][0][e] + __shfl_down_sync(0xffffffffu, o[i][0][e], GC / 2);
+                }
+                float* w = wa + (i / 8) * 128 + RUN * g + 2 * (i % 8);
+                if (mine) {
+                    *reinterpret_cast<float2*>(w) = make_float2(y[0] * f, y[2] * f);
+                    *reinterpret_cast<float2*>(w + HD + 2) = make_float2(y[1] * f, y[3] * f);
+                }
+            }
+            if (mine && g == 0) wa[HD] = ma, wa[HD + 1] = la, wa[2 * HD + 2] = mb, wa[2 * HD + 3] = lb;
         }
         __syncthreads();
-        float* pt = parts + ((int64_t)blockIdx.x * kMaxParts + (first == 0)) * step_part_floats(HD);
+        float* pt = parts + ((int64_t)blockIdx.x * kMaxParts + (first == 0)) * C::PART;
         for (int i = tid; i < live * HD; i += kThreads) {
             const int j = i / HD, d = i - j * HD;
             const float* w = merge + j * (HD + 2);
-            constexpr int WS = kGroup * (HD + 2);
+            constexpr int WS = GC * (HD + 2);
             float mm = w[HD];
 #pragma unroll
             for (int x = 1; x < kStepWarps; ++x) mm = fmaxf(mm, w[x * WS + HD]);
@@ -598,16 +650,16 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD>::CTAS) kvb_step_kernel(c
                 const float f = w[x * WS + HD] == -INFINITY ? 0.0f : ex2(w[x * WS + HD] - mm);
                 acc = fmaf(w[x * WS + d], f, acc), ll = fmaf(w[x * WS + HD + 1], f, ll);
             }
-            if (whole) {
-                if (d < hd)
-                    static_cast<T*>(a.out)[((int64_t)b * a.heads + h * G + j0 + j) * hd + d] = kvb_t<T>(acc / ll);
-            } else {
+            const int64_t row = (int64_t)b * a.heads + h * G + j0 + j;
+            if (!whole) {
                 pt[j * (HD + 2) + d] = acc;
-            }
-            if (d == 0 && (!whole || scores)) pt[j * (HD + 2) + HD] = mm, pt[j * (HD + 2) + HD + 1] = ll;
-            if (whole && scores && d == 0) {
-                float* ml = scores + (int64_t)a.c.slots * a.heads * a.c.cap + 2 * ((int64_t)b * a.heads + h * G + j0 + j);
-                ml[0] = mm, ml[1] = ll;
+                if (d == 0) pt[j * (HD + 2) + HD] = mm, pt[j * (HD + 2) + HD + 1] = ll;
+            } else {
+                if (d < hd) store1(a.out, a.type, row * hd + d, acc / ll);
+                if (scores && d == 0) {
+                    float* ml = scores + (int64_t)a.c.slots * a.heads * a.c.cap + 2 * row;
+                    ml[0] = mm, ml[1] = ll;
+                }
             }
         }
         todo -= n_it;
@@ -622,20 +674,20 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD>::CTAS) kvb_step_kernel(c
 // chunk's probabilities, from the stored scores.
 constexpr int kMassChunk = 1024;
 
-template <int HD, typename T>
+template <int HD, int GC>
 __global__ void __launch_bounds__(kThreads) kvb_step_finish(const KvbAttnArgs a, const float* parts,
                                                           const float* scores, int grid) {
-    using C = StepCfg<HD>;
+    using C = StepCfg<HD, GC>;
     pdl_wait();
     pdl_trigger();
     const int j = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, hd = a.c.hd;
-    const int G = a.heads / a.c.heads, GT = (G + kGroup - 1) / kGroup, units = a.c.heads * GT;
+    const int G = a.heads / a.c.heads, GT = (G + GC - 1) / GC, units = a.c.heads * GT;
     const int len = step_len(a, b);
     if (blockIdx.z == 0 && j == 0 && tid == 0 && a.r.pos[b] >= a.c.cap) atomicOr(&g_kvb_attn_errors, kKvbErrCapacity);
-    T* out = static_cast<T*>(a.out) + ((int64_t)b * a.heads + j) * hd;
+    const int64_t out = ((int64_t)b * a.heads + j) * hd;
     if (len == 0) {
         if (blockIdx.z == 0)
-            for (int d = tid; d < hd; d += kThreads) out[d] = kvb_t<T>(0.0f);
+            for (int d = tid; d < hd; d += kThreads) store1(a.out, a.type, out + d, 0.0f);
         return;
     }
     const int t0 = blockIdx.z * kMassChunk;
@@ -649,7 +701,7 @@ __global__ void __launch_bounds__(kThreads) kvb_step_finish(const KvbAttnArgs a,
     if (scores && j % G == 0)
         for (int i = tid; i < kMassChunk; i += kThreads) s_mass[i] = 0.0f;
     for (int i = 0; i < heads_here; ++i) {
-        const int jj = j + i, h = jj / G, u = h * GT + (jj - h * G) / kGroup, row = (jj - h * G) % kGroup;
+        const int jj = j + i, h = jj / G, u = h * GT + (jj - h * G) / GC, row = (jj - h * G) % GC;
         const int64_t x0 = before * units + (int64_t)u * tiles, x1 = x0 + tiles;
         const int c0 = (int)(((x0 + 1) * ctas - 1) / total), c1 = (int)((x1 * ctas - 1) / total);
         float m = -INFINITY, l = 0.0f;
@@ -660,7 +712,7 @@ __global__ void __launch_bounds__(kThreads) kvb_step_finish(const KvbAttnArgs a,
         } else {
             // part of CTA c: its last unit (index 1) if the unit begins there, else its first (index 0)
             const float* p0 = parts + row * (HD + 2);
-            auto at = [&](int c) { return p0 + ((int64_t)c * kMaxParts + (c == c0 ? 1 : 0)) * step_part_floats(HD); };
+            auto at = [&](int c) { return p0 + ((int64_t)c * kMaxParts + (c == c0 ? 1 : 0)) * C::PART; };
             float mine = -INFINITY;
             for (int c = c0 + tid; c <= c1; c += kThreads) mine = fmaxf(mine, at(c)[HD]);
             s_m[tid] = mine;
@@ -675,7 +727,7 @@ __global__ void __launch_bounds__(kThreads) kvb_step_finish(const KvbAttnArgs a,
                 for (int d = tid; d < hd; d += kThreads) {
                     float acc = 0.0f;
                     for (int c = c0; c <= c1; ++c) acc = fmaf(at(c)[d], ex2(at(c)[HD] - m), acc);
-                    out[d] = kvb_t<T>(acc / l);
+                    store1(a.out, a.type, out + d, acc / l);
                 }
             __syncthreads();
         }
@@ -694,30 +746,37 @@ __global__ void __launch_bounds__(kThreads) kvb_step_finish(const KvbAttnArgs a,
 constexpr int kSms = 148;
 
 int step_hd(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
+int step_gc(int G) { return G <= 2 ? 2 : G <= 4 ? 4 : 8; }
 
-template <int HD, typename T>
+template <int HD, int GC>
+size_t step_parts() {
+    return (size_t)kSms * StepCfg<HD, GC>::CTAS * kMaxParts * StepCfg<HD, GC>::PART;
+}
+
+template <int HD, int GC>
 cudaError_t step_launch(const KvbAttnArgs& a, cudaStream_t st) {
-    using C = StepCfg<HD>;
+    using C = StepCfg<HD, GC>;
     const int grid = kSms * C::CTAS;
     float* parts = static_cast<float*>(a.scratch);
-    float* scores = a.mass ? parts + (size_t)grid * kMaxParts * step_part_floats(HD) : nullptr;
-    cudaError_t e = cudaFuncSetAttribute(kvb_step_kernel<HD, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
+    float* scores = a.mass ? parts + step_parts<HD, GC>() : nullptr;
+    cudaError_t e = cudaFuncSetAttribute(kvb_step_kernel<HD, GC>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)C::SMEM);
     if (e != cudaSuccess) return e;
-    e = launch_k(kvb_step_kernel<HD, T>, dim3(grid), dim3(kThreads), C::SMEM, st, a, parts, scores);
+    e = launch_k(kvb_step_kernel<HD, GC>, dim3(grid), dim3(kThreads), C::SMEM, st, a, parts, scores);
     if (e != cudaSuccess) return e;
     const int chunks = a.mass ? (a.c.cap + kMassChunk - 1) / kMassChunk : 1;
-    return launch_k(kvb_step_finish<HD, T>, dim3(a.heads, a.c.slots, chunks), dim3(kThreads), 0, st, a,
+    return launch_k(kvb_step_finish<HD, GC>, dim3(a.heads, a.c.slots, chunks), dim3(kThreads), 0, st, a,
                     (const float*)parts, (const float*)scores, grid);
 }
 
-template <typename T>
-cudaError_t step_launch_hd(const KvbAttnArgs& a, cudaStream_t st) {
-    switch (step_hd(a.c.hd)) {
-        case 64: return step_launch<64, T>(a, st);
-        case 128: return step_launch<128, T>(a, st);
-        default: return step_launch<256, T>(a, st);
-    }
-}
+// f<HD, GC>() for a head size and group
+#define KVB_STEP_PICK(f, hd, G, ...)                                                                          \
+    (step_hd(hd) == 64    ? (step_gc(G) == 2 ? f<64, 2>(__VA_ARGS__)                                          \
+                             : step_gc(G) == 4 ? f<64, 4>(__VA_ARGS__) : f<64, 8>(__VA_ARGS__))               \
+     : step_hd(hd) == 128 ? (step_gc(G) == 2 ? f<128, 2>(__VA_ARGS__)                                         \
+                             : step_gc(G) == 4 ? f<128, 4>(__VA_ARGS__) : f<128, 8>(__VA_ARGS__))             \
+                          : (step_gc(G) == 2 ? f<256, 2>(__VA_ARGS__)                                         \
+                             : step_gc(G) == 4 ? f<256, 4>(__VA_ARGS__) : f<256, 8>(__VA_ARGS__)))
 
 template <typename T>
 cudaError_t attn_launch(const KvbAttnArgs& a, cudaStream_t st) {
@@ -730,19 +789,14 @@ cudaError_t attn_launch(const KvbAttnArgs& a, cudaStream_t st) {
 }  // namespace
 
 size_t kvb_attn_scratch(const KvbCache& c, int heads, int rows, bool one_row, bool mass) {
-    if (one_row) {
-        const int hd = step_hd(c.hd), grid = kSms * (hd == 256 ? StepCfg<256>::CTAS : StepCfg<64>::CTAS);
-        const size_t parts = (size_t)grid * kMaxParts * step_part_floats(hd);
-        return (parts + (mass ? (size_t)c.slots * heads * (c.cap + 2) : 0)) * sizeof(float);
-    }
+    if (one_row)
+        return (KVB_STEP_PICK(step_parts, c.hd, heads / c.heads) + (mass ? (size_t)c.slots * heads * (c.cap + 2) : 0)) *
+               sizeof(float);
     return mass ? (size_t)rows * heads * sizeof(float) : 0;
 }
 
 cudaError_t launch_kvb_attn(const KvbAttnArgs& a, cudaStream_t st) {
-    if (!a.r.start)
-        return a.type == KVB_F32    ? step_launch_hd<float>(a, st)
-               : a.type == KVB_BF16 ? step_launch_hd<__nv_bfloat16>(a, st)
-                                    : step_launch_hd<__half>(a, st);
+    if (!a.r.start) return KVB_STEP_PICK(step_launch, a.c.hd, a.heads / a.c.heads, a, st);
     return a.type == KVB_F32    ? attn_launch<float>(a, st)
            : a.type == KVB_BF16 ? attn_launch<__nv_bfloat16>(a, st)
                                 : attn_launch<__half>(a, st);
