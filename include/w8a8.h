@@ -68,7 +68,8 @@ int w8a8_embed(const int32_t* tokens, int rows, const int8_t* emb_q, const float
  * tile; bit 4: a tensor-core GEMM pipeline wait; bit 5: a tensor-parallel
  * exchange wait gave up; bit 6: w8a8_moe_ffn_rows found more pairs of one
  * expert than rows, routing that is not Top-k, and skipped the excess; bit 7:
- * a w8a8_kvb_* row or length past the cache's capacity, skipped).
+ * a w8a8_kvb_* row or length past the cache's capacity, skipped; bit 8: a
+ * pipeline wait of the prompt attention over it gave up).
  * Synchronous with the device.
  * Plays the role of the overlay's sticky list status (llm/sa_funcsim.py:62-66,
  * firmware/rt/rt_fw.c:53-60). */

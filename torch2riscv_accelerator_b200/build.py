@@ -17,7 +17,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libw8a8_b200.so")
 TRACE_LIB = os.path.join(HERE, "libw8a8_b200_trace.so")
 SOURCES = ["capi.cu", "linear.cu", "gemv.cu", "attn.cu", "misc.cu", "moe.cu", "gemm.cu", "kvb.cu",
-           "kvb_attn.cu"]
+           "kvb_attn.cu", "kvb_rows.cu"]
 HEADERS = ["w8a8_math.cuh", "w8a8_internal.h", "sfu_tables.h", "pdl.cuh", "tp.cuh", "linear_common.cuh", "trace.cuh", "tc.cuh",
            "kvb.cuh",
            os.path.join("..", "..", "include", "w8a8.h")]

@@ -91,7 +91,8 @@ int w8a8_error_flags(uint32_t* flags) {
     unsigned int v = 0;
     int st = cuda_status(read_clear_errors(&v));
     *flags = v | gemv_read_clear_errors() | attn_read_clear_errors() | moe_read_clear_errors() |
-             gemm_read_clear_errors() | kvb_read_clear_errors() | kvb_attn_read_clear_errors();
+             gemm_read_clear_errors() | kvb_read_clear_errors() | kvb_attn_read_clear_errors() |
+             kvb_rows_read_clear_errors();
     return st;
 }
 
@@ -768,6 +769,7 @@ int w8a8_kvb_attn(const W8A8KvBlocks* cache, const void* q, int64_t q_stride, in
     if (st) return st;
     const int e = kvb_type_bytes(dtype);
     if (!e || heads <= 0 || heads > 65535 || heads % a.c.heads || !(std::fabs(scale) <= 3.4e38f)) return W8A8_EINVAL;
+    if ((int64_t)rows * heads > INT32_MAX) return W8A8_EINVAL;
     if (rows > 0 && (!q || !out || (rows > 1 && q_stride < (int64_t)heads * a.c.hd))) return W8A8_EINVAL;
     if (!al16(q) || !al16(out) || (q_stride * e) % 16 || !al16(scratch)) return W8A8_EALIGN;
     if (rows == 0) return W8A8_OK;

@@ -1,4 +1,4 @@
-// The block-scaled 8-bit KV cache (kvb.cu, kvb_attn.cu): codes int8
+// The block-scaled 8-bit KV cache (kvb.cu, kvb_attn.cu, kvb_rows.cu): codes int8
 // [slots][kv_heads][cap][hd] for K and V, one fp32 scale per (slot, KV head,
 // block of tokens): the value held is code * scale.
 #pragma once
@@ -106,6 +106,9 @@ cudaError_t launch_kvb_read(const KvbReadArgs& a, cudaStream_t st);
 cudaError_t launch_kvb_evict(const KvbEvictArgs& a, cudaStream_t st);
 size_t kvb_attn_scratch(const KvbCache& c, int heads, int rows, bool one_row, bool mass);
 cudaError_t launch_kvb_attn(const KvbAttnArgs& a, cudaStream_t st);
+size_t kvb_rows_scratch(const KvbCache& c, int heads, int rows, bool mass);
+cudaError_t launch_kvb_rows(const KvbAttnArgs& a, cudaStream_t st);
+unsigned int kvb_rows_read_clear_errors();
 unsigned int kvb_read_clear_errors();
 unsigned int kvb_attn_read_clear_errors();
 
@@ -141,6 +144,37 @@ __device__ __forceinline__ void kvb_load8(const T* p, float* x) {
     }
 }
 
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// two codes (biased by 128, bytes lo and lo + 1 of x) as exact halves
+__device__ __forceinline__ uint32_t halves_of(uint32_t x, uint32_t sel) {
+    const uint32_t h = __byte_perm(x, 0x64646464u, sel);                // 1024 + byte
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), __float2half2_rn(1152.0f));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+__device__ __forceinline__ uint32_t bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+// 16 consecutive elements of a row of type `type`
+__device__ __forceinline__ void load16(const void* base, int type, int64_t at, float* y) {
+    if (type == KVB_F32) {
+        kvb_load8<float>(static_cast<const float*>(base) + at, y);
+        kvb_load8<float>(static_cast<const float*>(base) + at + 8, y + 8);
+    } else if (type == KVB_BF16) {
+        kvb_load8<__nv_bfloat16>(static_cast<const __nv_bfloat16*>(base) + at, y);
+        kvb_load8<__nv_bfloat16>(static_cast<const __nv_bfloat16*>(base) + at + 8, y + 8);
+    } else {
+        kvb_load8<__half>(static_cast<const __half*>(base) + at, y);
+        kvb_load8<__half>(static_cast<const __half*>(base) + at + 8, y + 8);
+    }
+}
+__device__ __forceinline__ void store1(void* base, int type, int64_t at, float y) {
+    if (type == KVB_F32) static_cast<float*>(base)[at] = y;
+    else if (type == KVB_BF16) static_cast<__nv_bfloat16*>(base)[at] = __float2bfloat16_rn(y);
+    else static_cast<__half*>(base)[at] = __float2half_rn(y);
+}
 // rint(num / den) saturated to +-127 as an int8 code, the quotient correctly
 // rounded before the rounding to an integer. The product with rcp ~ 1 / den is
 // within 3 ulp of the quotient (below 1e-4 for |quotient| <= 128), so only
