@@ -538,7 +538,7 @@ int w8a8_kvb_read(const W8A8KvBlocks* cache, int rows, const int32_t* pos, const
  * per slot (decode). scratch: w8a8_kvb_attn_scratch_bytes() bytes (16-byte
  * aligned, contents irrelevant), not shared by calls that can overlap. */
 size_t w8a8_kvb_attn_scratch_bytes(const W8A8KvBlocks* cache, int heads, int rows, int one_row_per_slot,
-                                   int with_mass);
+                                   int with_mass, int dtype);
 int w8a8_kvb_attn(const W8A8KvBlocks* cache, const void* q, int64_t q_stride, int dtype, int heads, int rows,
                   const int32_t* pos, const int32_t* start, float scale, void* out, float* mass, void* scratch,
                   size_t scratch_bytes, void* stream);

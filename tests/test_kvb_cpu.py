@@ -32,7 +32,7 @@ def test_every_call_checks_the_cache(lib, kw, status):
     assert lib.w8a8_kvb_read(c, 2, 16, None, 16, 16, 0, None) == status
     assert lib.w8a8_kvb_attn(c, 16, 256, 0, 4, 2, 16, None, 1.0, 16, None, 16, 1 << 30, None) == status
     assert lib.w8a8_kvb_evict(c, 16, 16, 4, 0, 0, None, None, 16, 32, None) == status
-    assert lib.w8a8_kvb_attn_scratch_bytes(c, 4, 2, 1, 0) == 0
+    assert lib.w8a8_kvb_attn_scratch_bytes(c, 4, 2, 1, 0, 0) == 0
     good = blocks(k=5 << 20, v=6 << 20, k_scale=7 << 20, v_scale=8 << 20)
     assert lib.w8a8_kvb_evict(good, 16, 16, 4, 0, 0, c, 64, 16, 32, None) == status
 
@@ -67,7 +67,7 @@ def test_attention_arguments(lib):
     assert attn(qs=255) == EINVAL and attn(q=20) == EALIGN and attn(out=8) == EALIGN
     assert attn(scale=float("nan")) == EINVAL and attn(scale=float("inf")) == EINVAL
     assert attn(rows=0, start=16, q=None, out=None) == OK
-    need = lib.w8a8_kvb_attn_scratch_bytes(c, 4, 2, 1, 1)
+    need = lib.w8a8_kvb_attn_scratch_bytes(c, 4, 2, 1, 1, 0)
     assert need > 0 and attn(mass=16, size=need - 1) == ESCRATCH and attn(mass=16, scratch=None) == ESCRATCH
 
 

@@ -121,7 +121,7 @@ PROTOTYPES = {
     "w8a8_dequant_resid": (I, [P, P, P, I, I, P, P, P]),
     "w8a8_kvb_append": (I, [C.POINTER(W8A8KvBlocks), P, L, P, L, I, I, P, P, P]),
     "w8a8_kvb_read": (I, [C.POINTER(W8A8KvBlocks), I, P, P, P, P, I, P]),
-    "w8a8_kvb_attn_scratch_bytes": (Z, [C.POINTER(W8A8KvBlocks), I, I, I, I]),
+    "w8a8_kvb_attn_scratch_bytes": (Z, [C.POINTER(W8A8KvBlocks), I, I, I, I, I]),
     "w8a8_kvb_attn": (I, [C.POINTER(W8A8KvBlocks), P, L, I, I, I, P, P, F, P, P, P, Z, P]),
     "w8a8_kvb_evict": (I, [C.POINTER(W8A8KvBlocks), P, P, I, I, I, C.POINTER(W8A8KvBlocks), P, P, P, P]),
 }

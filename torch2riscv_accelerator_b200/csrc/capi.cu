@@ -754,10 +754,10 @@ int w8a8_kvb_read(const W8A8KvBlocks* cache, int rows, const int32_t* pos, const
 }
 
 size_t w8a8_kvb_attn_scratch_bytes(const W8A8KvBlocks* cache, int heads, int rows, int one_row_per_slot,
-                                   int with_mass) {
+                                   int with_mass, int dtype) {
     KvbCache c;
-    if (kvb_cache(cache, &c) || heads <= 0 || heads % c.heads || rows <= 0) return 0;
-    return kvb_attn_scratch(c, heads, rows, one_row_per_slot != 0, with_mass != 0);
+    if (kvb_cache(cache, &c) || !kvb_type_bytes(dtype) || heads <= 0 || heads % c.heads || rows <= 0) return 0;
+    return kvb_attn_scratch(c, heads, rows, one_row_per_slot != 0, with_mass != 0, kvb_type_bytes(dtype));
 }
 
 int w8a8_kvb_attn(const W8A8KvBlocks* cache, const void* q, int64_t q_stride, int dtype, int heads, int rows,
@@ -773,7 +773,7 @@ int w8a8_kvb_attn(const W8A8KvBlocks* cache, const void* q, int64_t q_stride, in
     if (rows > 0 && (!q || !out || (rows > 1 && q_stride < (int64_t)heads * a.c.hd))) return W8A8_EINVAL;
     if (!al16(q) || !al16(out) || (q_stride * e) % 16 || !al16(scratch)) return W8A8_EALIGN;
     if (rows == 0) return W8A8_OK;
-    const size_t need = kvb_attn_scratch(a.c, heads, rows, start == nullptr, mass != nullptr);
+    const size_t need = kvb_attn_scratch(a.c, heads, rows, start == nullptr, mass != nullptr, e);
     if (need && (!scratch || scratch_bytes < need)) return W8A8_ESCRATCH;
     a.q = q, a.q_stride = q_stride, a.out = out, a.heads = heads, a.type = dtype, a.scale = scale, a.mass = mass;
     a.scratch = scratch;

@@ -104,9 +104,9 @@ struct KvbEvictArgs {
 cudaError_t launch_kvb_append(const KvbAppendArgs& a, cudaStream_t st);
 cudaError_t launch_kvb_read(const KvbReadArgs& a, cudaStream_t st);
 cudaError_t launch_kvb_evict(const KvbEvictArgs& a, cudaStream_t st);
-size_t kvb_attn_scratch(const KvbCache& c, int heads, int rows, bool one_row, bool mass);
+size_t kvb_attn_scratch(const KvbCache& c, int heads, int rows, bool one_row, bool mass, int qbytes);
 cudaError_t launch_kvb_attn(const KvbAttnArgs& a, cudaStream_t st);
-size_t kvb_rows_scratch(const KvbCache& c, int heads, int rows, bool mass);
+size_t kvb_rows_scratch(const KvbCache& c, int heads, int rows, bool mass, int qbytes);
 cudaError_t launch_kvb_rows(const KvbAttnArgs& a, cudaStream_t st);
 unsigned int kvb_rows_read_clear_errors();
 unsigned int kvb_read_clear_errors();
@@ -175,6 +175,17 @@ __device__ __forceinline__ void store1(void* base, int type, int64_t at, float y
     else if (type == KVB_BF16) static_cast<__nv_bfloat16*>(base)[at] = __float2bfloat16_rn(y);
     else static_cast<__half*>(base)[at] = __float2half_rn(y);
 }
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// zeros instead of the source where it is not to be read
+__device__ __forceinline__ void cp16z(uint32_t dst, const void* src, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 // rint(num / den) saturated to +-127 as an int8 code, the quotient correctly
 // rounded before the rounding to an integer. The product with rcp ~ 1 / den is
 // within 3 ulp of the quotient (below 1e-4 for |quotient| <= 128), so only

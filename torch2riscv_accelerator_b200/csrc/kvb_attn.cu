@@ -98,17 +98,6 @@ __device__ __forceinline__ int64_t step_scan(const KvbAttnArgs& a, int tile, int
     return x;
 }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-// zeros instead of the source where it is not to be read
-__device__ __forceinline__ void cp16z(uint32_t dst, const void* src, bool in) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 __device__ __forceinline__ void mma_s8(int* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
     asm volatile(
@@ -685,11 +674,11 @@ cudaError_t step_launch(const KvbAttnArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-size_t kvb_attn_scratch(const KvbCache& c, int heads, int rows, bool one_row, bool mass) {
+size_t kvb_attn_scratch(const KvbCache& c, int heads, int rows, bool one_row, bool mass, int qbytes) {
     if (one_row)
         return (KVB_STEP_PICK(step_parts, c.hd, heads / c.heads) + (mass ? (size_t)c.slots * heads * (c.cap + 2) : 0)) *
                sizeof(float);
-    return kvb_rows_scratch(c, heads, rows, mass);
+    return kvb_rows_scratch(c, heads, rows, mass, qbytes);
 }
 
 cudaError_t launch_kvb_attn(const KvbAttnArgs& a, cudaStream_t st) {

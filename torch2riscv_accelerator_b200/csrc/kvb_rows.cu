@@ -13,21 +13,23 @@
 // joins. kvb_rows_plan lists the units, since lengths are device data.
 //
 // Warps of a CTA (one CTA an SM, all 512 TMEM columns):
-//   softmax   4 warps per stream, one row per thread. With two streams the even
-//             tiles go to one and the odd ones to the other, each with its own
-//             maximum, sum and output accumulator: no exchange before the end.
-//   convert   4 warps: int8 codes -> exact halves (byte permutes, one
-//             subtraction) in 128-byte-swizzled tiles, a tile ahead of the
-//             products in registers; the query rows as hi + lo halves (22 bits)
+//   softmax   8 warps: a row's columns are split between two threads, which meet
+//             at one reducing barrier a tile (does any score pass its reference?).
+//   convert   7 warps: int8 codes -> exact halves (byte permutes, one
+//             subtraction) in 128-byte-swizzled tiles, the next tile's codes on
+//             their way in registers; the query rows as hi + lo halves (22 bits)
 //             of the row scaled by a power of two (16-bit queries are exact in
-//             one half).
-//   products  one thread: S = Q K^T (A, B from shared memory), O += P V (P from
-//             TMEM, written over S: hi in columns 0-15, lo in 16-31 of every 32;
+//             one half), in TMEM where it has room (head sizes up to 128), which
+//             halves what the score products read from shared memory.
+//   products  one thread: S = Q K^T for the tile after next, then O += P V (P from
+//             TMEM, written over S: hi in columns 0-7, lo in 8-15 of every 16;
 //             V as it lies, its rows being the contraction).
 // Block scales do not touch the codes: K's multiplies the scores of its 16
-// columns, V's goes into the weights, as exp(z - m) sv / sv_ref 2^7 with the
-// lazily moved references of the one-row kernel (kvb_attn.cu), so that the
+// columns, V's goes into the weights, exp(z - m) sv / sv_ref 2^7 by one
+// exponential, with the lazily moved references of the one-row kernel (kvb_attn.cu), so that the
 // accumulator is rescaled rarely.
+#include <type_traits>
+
 #include "kvb.cuh"
 #include "tc.cuh"
 
@@ -47,7 +49,7 @@ namespace {
 constexpr int kRows = 128;                       // rows of a unit (TMEM lanes)
 constexpr int kSms = 148;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLazyScore = 6.0f, kLazyScale = 4.0f, kWeightScale = 128.0f;
+constexpr float kLazyScore = 6.0f, kLazyLog = 2.0f, kWeightLog = 7.0f;   // log2: see kvb_attn.cu
 constexpr unsigned int kErrWait = 256u;          // error bit 8: a pipeline wait gave up
 constexpr int kPlanThreads = 1024;
 constexpr int kFinishThreads = 256;
@@ -55,21 +57,32 @@ constexpr int kFinishThreads = 256;
 template <int HD>
 struct RowsCfg {
     static constexpr int BN = HD == 256 ? 64 : 128;
-    static constexpr int STREAMS = HD == 256 ? 1 : 2;
     static constexpr int NBUF = HD == 256 ? 1 : 2;
+    static constexpr bool QT = HD <= 128;        // queries in TMEM
     static constexpr int SLABS = HD / 64;        // 64-channel slabs of a tile
     static constexpr int QSLAB = kRows * 128, SLAB = BN * 128, TILE = SLABS * SLAB;   // bytes
-    static constexpr int SOFT = STREAMS * 128;   // softmax threads
-    static constexpr int THREADS = SOFT + 128 + 32;
-    static constexpr size_t smem(bool q2) {
-        return 1024 + (size_t)(q2 ? 2 : 1) * SLABS * QSLAB + (size_t)NBUF * 2 * TILE;
+    static constexpr int SOFT = 256;             // softmax threads
+    static constexpr int CONV = 224;             // converting threads
+    static constexpr int THREADS = 32 + SOFT + CONV;   // 16 warps: 128 registers a thread
+    static constexpr int RAW = BN * HD, NRAW = HD == 256 ? 1 : 4;   // bytes of a tile's codes; tiles on their way
+    // a prepared query row: halves (hi, lo), its score factor in 16 bytes more
+    // (lanes that read one row each then meet no bank conflicts)
+    static constexpr int qrow(int qbytes) { return HD * qbytes + 16; }
+    static constexpr int stage(int qbytes) { return QT && 32 * qrow(qbytes) > RAW ? 32 * qrow(qbytes) : RAW; }
+    static constexpr size_t smem(int qbytes) {
+        return 1024 + (QT ? 0 : (size_t)(qbytes == 4 ? 2 : 1) * SLABS * QSLAB) + (size_t)NBUF * 2 * TILE +
+               (size_t)NRAW * stage(qbytes);
     }
     static constexpr size_t PART = (size_t)kRows * (HD + 2);   // floats of a partial unit
 };
 
+struct __align__(16) RowsUnit {
+    int slot, m, before, tiles;                  // 128-row tile of the slot, tiles of the units before, tiles
+    int p, r0, rows, pad;                        // position of the slot's first row, its row, the slot's n * G live rows
+};
 struct RowsPlan {                                // in scratch: total, units' count, units, slots' first units
     int* head;                                   // [4]: tiles of all units of one KV head, units
-    int4* unit;                                  // slot, 128-row tile, tiles before, tiles
+    RowsUnit* unit;
     int* first;                                  // [slots + 1]
 };
 
@@ -120,21 +133,21 @@ __global__ void __launch_bounds__(kPlanThreads) kvb_rows_plan(const KvbAttnArgs 
     int total = 0;
     for (int u0 = 0; u0 < units; u0 += kPlanThreads) {
         const int u = u0 + tid;
-        int b = 0, m = 0, tiles = 0;
+        RowsUnit v{};
         if (u < units) {
+            int b = 0;
             int hi = S;                          // the last slot with first <= u that has units
             while (hi - b > 1) {
                 const int mid = (b + hi) >> 1;
                 if (plan.first[mid] <= u) b = mid;
                 else hi = mid;
             }
-            m = u - plan.first[b];
             const KvbSpan sp = kvb_span(a.r, b);
-            const int rows = live_rows(sp, a.c.cap) * G;
-            tiles = (sp.p + min(m * kRows + kRows - 1, rows - 1) / G) / bn + 1;
+            v.slot = b, v.m = u - plan.first[b], v.p = sp.p, v.r0 = sp.r0, v.rows = live_rows(sp, a.c.cap) * G;
+            v.tiles = (sp.p + min(v.m * kRows + kRows - 1, v.rows - 1) / G) / bn + 1;
         }
-        const int at = block_scan(tiles, &sum);
-        if (u < units) plan.unit[u] = make_int4(b, m, total + at, tiles);
+        v.before = total + block_scan(v.tiles, &sum);
+        if (u < units) plan.unit[u] = v;
         total += sum;
     }
     if (tid == 0) plan.head[0] = total, plan.head[1] = units;
@@ -145,14 +158,12 @@ struct Seg {
     int64_t x, end;
     int h, u, j, n, tiles;                       // KV head, unit; first tile, tiles here, tiles of the unit
     int slot, m, p, r0, rows;                    // rows: the slot's n * G live ones
-    __device__ __forceinline__ void unit(const KvbAttnArgs& a, const RowsPlan& plan) {
-        const int4 v = plan.unit[u];
-        slot = v.x, m = v.y, tiles = v.w;
-        const KvbSpan s = kvb_span(a.r, slot);
-        p = s.p, r0 = s.r0, rows = live_rows(s, a.c.cap) * (a.heads / a.c.heads);
+    __device__ __forceinline__ void unit(const RowsPlan& plan) {
+        const RowsUnit v = plan.unit[u];
+        slot = v.slot, m = v.m, tiles = v.tiles, p = v.p, r0 = v.r0, rows = v.rows;
         n = (int)min((int64_t)(tiles - j), end - x);
     }
-    __device__ __forceinline__ bool begin(const KvbAttnArgs& a, const RowsPlan& plan, int64_t x0, int64_t x1) {
+    __device__ __forceinline__ bool begin(const RowsPlan& plan, int64_t x0, int64_t x1) {
         x = x0, end = x1;
         if (x >= end) return false;
         const int total = plan.head[0];
@@ -161,19 +172,19 @@ struct Seg {
         int lo = 0, hi = plan.head[1];
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (plan.unit[mid].z <= at) lo = mid;
+            if (plan.unit[mid].before <= at) lo = mid;
             else hi = mid;
         }
-        u = lo, j = at - plan.unit[lo].z;
-        unit(a, plan);
+        u = lo, j = at - plan.unit[lo].before;
+        unit(plan);
         return true;
     }
-    __device__ __forceinline__ bool next(const KvbAttnArgs& a, const RowsPlan& plan) {
+    __device__ __forceinline__ bool next(const RowsPlan& plan) {
         x += n;
         if (x >= end) return false;
         if (++u == plan.head[1]) u = 0, ++h;
         j = 0;
-        unit(a, plan);
+        unit(plan);
         return true;
     }
 };
@@ -184,47 +195,173 @@ __device__ __forceinline__ void rows_share(const RowsPlan& plan, int heads, int 
     if (cta < ctas) *lo = total * cta / ctas, *hi = total * (cta + 1) / ctas;
 }
 
-// 16 codes as 16 halves in two 16-byte chunks of a swizzled row
-__device__ __forceinline__ void put_codes(unsigned char* slab, int row, int ch, int odd, uint4 w) {
+// pairs of floats in one instruction
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t r, float& x, float& y) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+__device__ __forceinline__ uint64_t sub2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+
+// 16 codes as 16 halves in two 16-byte chunks of a swizzled row (`more`: rows
+// that the slab pointer is already past)
+__device__ __forceinline__ void put_codes(unsigned char* slab, int row, int ch, int odd, uint4 w, int more) {
     const uint32_t x[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
     uint4 lo, hi;
     lo = make_uint4(halves_of(x[0], 0x4140), halves_of(x[0], 0x4342), halves_of(x[1], 0x4140), halves_of(x[1], 0x4342));
     hi = make_uint4(halves_of(x[2], 0x4140), halves_of(x[2], 0x4342), halves_of(x[3], 0x4140), halves_of(x[3], 0x4342));
     unsigned char* r = slab + row * 128;
     // lanes of the second slab store their second chunk first: other banks
-    const int c0 = ((2 * ch + odd) ^ (row & 7)) * 16, c1 = ((2 * ch + (odd ^ 1)) ^ (row & 7)) * 16;
+    const int sw = (row + more) & 7, c0 = ((2 * ch + odd) ^ sw) * 16, c1 = ((2 * ch + (odd ^ 1)) ^ sw) * 16;
     *reinterpret_cast<uint4*>(r + c0) = odd ? hi : lo;
     *reinterpret_cast<uint4*>(r + c1) = odd ? lo : hi;
 }
 
-// HD: padded head size; Q2: queries as hi + lo (fp32), P2: weights as hi + lo
-// (fp32 and fp16 outputs; bf16 outputs keep 8 bits, against the half's 11).
-template <int HD, bool Q2, bool P2>
+template <typename T>
+__device__ __forceinline__ void load_row16(const T* p, float* y) {
+    kvb_load8<T>(p, y);
+    kvb_load8<T>(p + 8, y + 8);
+}
+
+// Whether the mbarrier phase with the given parity is over.
+__device__ __forceinline__ bool mbar_done(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
+// Bounded; once one wait has given up nobody waits any more, so that every role
+// runs to its end (the result is then worthless, the error bit is set). Out of
+// line: the roles' loops together have to fit the instruction cache.
+__device__ __noinline__ void wait_long(uint64_t* bar, uint32_t parity, int* dead) {
+    if (*(volatile int*)dead) return;
+    if (!mbar_wait(bar, parity)) {
+        *(volatile int*)dead = 1;
+        atomicOr(&g_kvb_rows_errors, kErrWait);
+    }
+}
+
+// Barrier `id` among n threads, and whether x holds for any of them.
+__device__ __forceinline__ bool barrier_any(int id, int n, bool x) {
+    uint32_t r;
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.u32 p, %3, 0;\n barrier.cta.red.or.pred q, %1, %2, p;\n"
+        " selp.u32 %0, 1, 0, q;\n}\n"
+        : "=r"(r)
+        : "r"(id), "r"(n), "r"((uint32_t)x)
+        : "memory");
+    return r != 0;
+}
+
+// Powers of two that bring a row's largest element (bits of |x|) to [2^13, 2^14),
+// and its score factor; rows with a NaN or an infinity (and bad set) give NaN.
+__device__ __forceinline__ float row_factor(uint32_t top, float scale, float* up, bool* bad) {
+    *bad = top >= 0x7f800000u;
+    const int e = top && !*bad ? min(140 - (int)(top >> 23), 120) : 0;
+    *up = __int_as_float((127 + e) << 23) * (scale < 0.0f ? -1.0f : 1.0f);
+    return *bad ? NAN : fabsf(scale) * kLog2e * __int_as_float((127 - e) << 23);
+}
+
+// The units' query rows as the products take them, 32 rows a CTA, a warp per
+// row: halves in unit order, so that a stage of the main kernel's ring is one
+// run of memory. (Converted there, row by row, they cost each unit 12,000 cycles
+// of cold code and scattered loads between two streams of products.)
+constexpr int kQueryWarps = 8;
+
+template <int HD, typename T>
+__global__ void __launch_bounds__(kQueryWarps * 32) kvb_rows_queries(const KvbAttnArgs a, const RowsPlan plan,
+                                                                   unsigned char* out, int units) {
+    pdl_wait();
+    pdl_trigger();
+    constexpr int V = HD / 32, RS = RowsCfg<HD>::qrow(sizeof(T));
+    const int u = blockIdx.x / 4, part = blockIdx.x % 4, h = blockIdx.y, lane = threadIdx.x & 31, G = a.heads / a.c.heads;
+    if (u >= plan.head[1]) return;
+    const RowsUnit v = plan.unit[u];
+    unsigned char* to = out + (((int64_t)h * units + u) * 4 + part) * 32 * RS;
+    for (int r = threadIdx.x / 32; r < 32; r += kQueryWarps) {
+        const int f = v.m * kRows + part * 32 + r;
+        float x[V];
+        uint32_t top = 0u;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            x[i] = 0.0f;
+            if (f < v.rows && lane * V < a.c.hd)
+                x[i] = kvb_f<T>(static_cast<const T*>(a.q)[(int64_t)(v.r0 + f / G) * a.q_stride +
+                                                           (int64_t)(h * G + f % G) * a.c.hd + lane * V + i]);
+            top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        float up;
+        bool bad;
+        const float factor = row_factor(top, a.scale, &up, &bad);
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            const float y0 = bad ? 0.0f : x[i] * up, y1 = bad ? 0.0f : x[i + 1] * up;
+            const __half2 h2 = __floats2half2_rn(y0, y1);
+            const float2 b2 = __half22float2(h2);
+            unsigned char* p = to + r * RS + (lane * V + i) * 2;
+            *reinterpret_cast<__half2*>(p) = h2;
+            if (sizeof(T) == 4) *reinterpret_cast<__half2*>(p + HD * 2) = __floats2half2_rn(y0 - b2.x, y1 - b2.y);
+        }
+        if (lane == 0) *reinterpret_cast<float*>(to + r * RS + HD * (int)sizeof(T)) = factor;
+    }
+}
+
+// HD: padded head size. Queries enter as hi + lo for fp32 (Q2), the weights
+// always: one half would lose as much as a 16-bit output's rounding, and saves
+// 8 % of the time.
+template <int HD, typename T>
 __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
-    kvb_rows_kernel(const KvbAttnArgs a, const RowsPlan plan, float* parts, float2* stats) {
+    kvb_rows_kernel(const KvbAttnArgs a, const RowsPlan plan, const unsigned char* queries, int units, float* parts,
+                    float2* stats) {
     using C = RowsCfg<HD>;
     constexpr int BN = C::BN, NG = BN / 16;
+    constexpr int RAWS = C::stage(sizeof(T));
+    constexpr bool Q2 = sizeof(T) == 4;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     unsigned char* sq = sm;                                              // [hi, lo][slab][128 rows][128 B]
-    unsigned char* sk = sm + (Q2 ? 2 : 1) * C::SLABS * C::QSLAB;         // [buffer][slab][BN][128 B]
+    unsigned char* sk = sm + (C::QT ? 0 : (Q2 ? 2 : 1) * C::SLABS * C::QSLAB);   // [buffer][slab][BN][128 B]
     unsigned char* sv = sk + C::NBUF * C::TILE;
+    unsigned char* raw = sv + C::NBUF * C::TILE;                         // [NRAW] codes as they lie in the cache, or query rows
     __shared__ __align__(8) uint64_t q_full, q_free, k_full[2], k_free[2], v_full[2], v_free[2], s_full[2], p_full[2],
-        o_full, drained;
+        o_full, drained, raw_full[C::NRAW];
     __shared__ uint32_t tmem_base;
     __shared__ int dead;
-    __shared__ float s_scale[4][2 * NG];         // K, V scales of a tile's 16-token groups
     __shared__ float s_row[2][kRows];            // score factors of the unit's rows
-    __shared__ float s_stat[2][C::STREAMS][3][kRows];
+    __shared__ float s_half[2][kRows];           // a row's half, for its other thread: largest score, at the end the sum
     const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
-    const int hd = a.c.hd, G = a.heads / a.c.heads, B = a.c.block;
+    const int hd = a.c.hd, G = a.heads / a.c.heads;
     if (tid == 0) {
         dead = 0;
         mbar_init(&q_full, 128), mbar_init(&q_free, 1), mbar_init(&o_full, 1), mbar_init(&drained, 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&k_full[i], 128), mbar_init(&k_free[i], 1), mbar_init(&v_full[i], 128), mbar_init(&v_free[i], 1);
-            mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 128);
+            mbar_init(&k_full[i], C::CONV), mbar_init(&k_free[i], 1);
+            mbar_init(&v_full[i], C::CONV), mbar_init(&v_free[i], 1);
+            mbar_init(&s_full[i], 1), mbar_init(&p_full[i], C::SOFT);
         }
+        for (int i = 0; i < C::NRAW; ++i) mbar_init(&raw_full[i], 1);
         mbar_fence_init();
     }
     // every earlier kernel of the stream is complete before this one takes the
@@ -240,225 +377,322 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
     tc_fence_after();
     pdl_trigger();
     const uint32_t tmem = tmem_base;
-    constexpr uint32_t kO = C::STREAMS == 2 ? 2 * BN : 256;              // first output column
-    auto wait = [&](uint64_t* bar, uint32_t parity, bool spin = false) {
-        if (*(volatile int*)&dead) return;
-        if (!(spin ? mbar_wait_spin(bar, parity) : mbar_wait(bar, parity))) {
-            dead = 1;
-            atomicOr(&g_kvb_rows_errors, kErrWait);
-        }
+    constexpr uint32_t kO = 256, kQ = 384;       // columns: two score tiles, outputs, queries (hi, lo)
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (!mbar_done(bar, parity)) wait_long(bar, parity, &dead);
     };
     Seg seg;
     int64_t lo, hi;
     rows_share(plan, a.c.heads, gridDim.x, blockIdx.x, &lo, &hi);
-    const bool any = seg.begin(a, plan, lo, hi);
+    const bool any = seg.begin(plan, lo, hi);
     int J = 0, sn = 0;                           // tiles and units of this CTA so far
 
-    if (warp * 32 >= C::SOFT + 128) {
+    if (warp == 0) {
         // ------------------------------------------------------- products
-        if (lane == 0 && any) {
+        if (any) {                               // the whole warp, one lane issuing
+            const uint32_t lead = lane == 0;
             constexpr uint32_t id_s = idesc_f16(kRows, BN, false), id_o = idesc_f16(kRows, HD, true);
             do {
-                wait(&q_full, sn & 1, true);
+                wait(&q_full, sn & 1);
                 auto scores = [&](int jj) {
-                    const int T = J + jj, kb = T % C::NBUF;
-                    wait(&k_full[kb], (T / C::NBUF) & 1, true);
+                    const int tl = J + jj, kb = tl % C::NBUF;
+                    wait(&k_full[kb], (tl / C::NBUF) & 1);
                     tc_fence_after();
-                    const uint32_t d = tmem + (T & 1) * BN;
+                    const uint32_t d = tmem + (tl & 1) * BN;
 #pragma unroll
                     for (int s = 0; s < C::SLABS; ++s) {
-                        const uint64_t da = smem_desc(sq + s * C::QSLAB), db = smem_desc(sk + kb * C::TILE + s * C::SLAB);
-                        const uint64_t dl = smem_desc(sq + (C::SLABS + s) * C::QSLAB);
+                        const uint64_t db = smem_desc(sk + kb * C::TILE + s * C::SLAB);
+                        const uint32_t at = tmem + kQ + s * 32;
+                        const uint64_t da = smem_desc(sq + s * C::QSLAB), dl = smem_desc(sq + (C::SLABS + s) * C::QSLAB);
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk) {
-                            mma_f16_ss(d, da + 2 * kk, db + 2 * kk, id_s, s > 0 || kk > 0);
-                            if (Q2) mma_f16_ss(d, dl + 2 * kk, db + 2 * kk, id_s, 1u);
+                            if constexpr (C::QT) {
+                                mma_f16_ts(d, at + 8 * kk, db + 2 * kk, id_s, s > 0 || kk > 0, lead);
+                                if (Q2) mma_f16_ts(d, at + 64 + 8 * kk, db + 2 * kk, id_s, 1u, lead);
+                            } else {
+                                mma_f16_ss(d, da + 2 * kk, db + 2 * kk, id_s, s > 0 || kk > 0, lead);
+                                if (Q2) mma_f16_ss(d, dl + 2 * kk, db + 2 * kk, id_s, 1u, lead);
+                            }
                         }
                     }
-                    mma_commit(&k_free[kb]);
-                    mma_commit(&s_full[T & 1]);
-                    if (jj == seg.n - 1) mma_commit(&q_free);
+                    mma_commit(&s_full[tl & 1], lead);
+                    mma_commit(&k_free[kb], lead);
+                    if (jj == seg.n - 1) mma_commit(&q_free, lead);
                 };
                 scores(0);
                 if (seg.n > 1) scores(1);
                 for (int jj = 0; jj < seg.n; ++jj) {
-                    const int T = J + jj, vb = T % C::NBUF;
-                    wait(&v_full[vb], (T / C::NBUF) & 1, true);
-                    wait(&p_full[T & 1], (T >> 1) & 1, true);
+                    const int tl = J + jj, vb = tl % C::NBUF;
+                    wait(&v_full[vb], (tl / C::NBUF) & 1);
+                    wait(&p_full[tl & 1], (tl >> 1) & 1);
                     tc_fence_after();
-                    const uint32_t d = tmem + kO + (C::STREAMS == 2 ? (T & 1) * HD : 0), ap = tmem + (T & 1) * BN;
+                    const uint32_t d = tmem + kO, ap = tmem + (tl & 1) * BN;
                     const uint64_t db = smem_desc_mn(sv + vb * C::TILE, C::SLAB);
-                    const uint32_t more = jj >= C::STREAMS;              // the stream's first tile writes
 #pragma unroll
-                    for (int s = 0; s < BN / 16; ++s) {
-                        const uint32_t at = ap + 32 * (s >> 1) + 8 * (s & 1);
-                        mma_f16_ts(d, at, db + 128 * s, id_o, more || s > 0);
-                        if (P2) mma_f16_ts(d, at + 16, db + 128 * s, id_o, 1u);
+                    for (int s = 0; s < BN / 16; ++s) {                  // 16 tokens: 8 columns hi, 8 lo
+                        const uint32_t at = ap + 16 * s;
+                        mma_f16_ts(d, at, db + 128 * s, id_o, jj > 0 || s > 0, lead);
+                        mma_f16_ts(d, at + 8, db + 128 * s, id_o, 1u, lead);
                     }
-                    mma_commit(&v_free[vb]);
-                    if (jj == seg.n - 1) mma_commit(&o_full);
+                    mma_commit(&v_free[vb], lead);
+                    if (jj == seg.n - 1) mma_commit(&o_full, lead);
                     if (jj + 2 < seg.n) scores(jj + 2);
                 }
                 J += seg.n, ++sn;
-            } while (seg.next(a, plan));
-            mma_commit(&drained);
+            } while (seg.next(plan));
+            mma_commit(&drained, lead);
             mbar_wait(&drained, 0u);             // also after a wait that gave up: nothing in flight below
         }
-    } else if (tid >= C::SOFT) {
+    } else if (tid >= 32 + C::SOFT) {
         // -------------------------------------------------------- convert
-        const int c = tid - C::SOFT;
-        constexpr int CH = HD / 16, PER = BN * CH / 128;                 // 16-code chunks of a row, of a thread
+        const int c = tid - 32 - C::SOFT;
         if (any) {
-            // A tile's K, then its V: the next of them on its way in registers
-            // while this one is converted (one loop body: code that several
-            // roles run at once has to stay within the instruction cache).
-            Seg ld = seg;
-            int lj = 0, lz = 0;                  // what is loaded next: tile of the unit, K or V
-            bool more = true;
-            uint4 cur[PER], nxt[PER];
-            auto load = [&]() {
+            // A tile's K, then its V, in one loop body (see wait_long). A tile's codes
+            // are one run of the cache: one bulk copy each, NRAW of them on their way
+            // (what lies behind the slot's last token is finite and masked). A unit's
+            // prepared query rows come the same way before its first tile, 32 rows a
+            // stage.
+            constexpr int CH = HD / 16, STEP = C::CONV / CH;             // 16-code chunks of a row; rows between a thread's
+            constexpr int PER = (BN + STEP - 1) / STEP;                  // ... chunks of a thread
+            constexpr int NQ = C::QT ? kRows / 32 : 0;                   // stages of query rows
+            constexpr int RS = C::qrow(sizeof(T));
+            Seg ld = seg;                        // first thread: the unit of the next copy, its place in the unit
+            int li = 0, lq = 0;
+            bool more = c == 0;
+            const int row0 = c / CH, ch = c % CH;
+            const bool live_ch = ch * 16 < hd;
+            auto copy = [&]() {
                 if (!more) return;
-                const int t0 = (ld.j + lj) * BN, len = ld.p + ld.rows / G;
-                const int8_t* base = (lz ? a.c.v : a.c.k) + ld.slot * a.c.slot_stride +
-                                     ((int64_t)ld.h * a.c.cap + t0) * hd;
-#pragma unroll
-                for (int i = 0; i < PER; ++i) {
-                    const int idx = i * 128 + c, row = idx / CH, ch = idx % CH;
-                    nxt[i] = make_uint4(0, 0, 0, 0);
-                    if (t0 + row < len && ch * 16 < hd)
-                        nxt[i] = *reinterpret_cast<const uint4*>(base + row * hd + ch * 16);
+                uint64_t* bar = &raw_full[lq % C::NRAW];
+                unsigned char* to = raw + lq % C::NRAW * RAWS;
+                if (li < NQ) {
+                    mbar_expect_tx(bar, 32 * RS);
+                    bulk_g2s(to, queries + (((int64_t)ld.h * units + ld.u) * NQ + li) * 32 * RS, 32 * RS, bar);
+                } else {
+                    const int t0 = (ld.j + (li - NQ) / 2) * BN, n = min(BN, ld.p + ld.rows / G - t0);
+                    const int8_t* at = ((li - NQ) & 1 ? a.c.v : a.c.k) + ld.slot * a.c.slot_stride +
+                                       ((int64_t)ld.h * a.c.cap + t0) * hd;
+                    mbar_expect_tx(bar, n * hd);
+                    bulk_g2s(to, at, n * hd, bar);
                 }
-                if ((lz ^= 1) == 0 && ++lj == ld.n) lj = 0, more = ld.next(a, plan);
+                ++lq;
+                if (++li == NQ + 2 * ld.n) li = 0, more = ld.next(plan);
             };
-            load();
+            int at = 0;                          // stages of the ring used so far
+#pragma unroll 1
+            for (int i = 0; i < C::NRAW; ++i) copy();
             do {
-                // the unit's rows: row c of it
-                if (sn > 0) wait(&q_free, (sn - 1) & 1);
-                {
-                    const int f = seg.m * kRows + c;
-                    const bool live = f < seg.rows;
-                    const int64_t at = (int64_t)(seg.r0 + f / G) * a.q_stride + (int64_t)(seg.h * G + f % G) * hd;
-                    float mx = 0.0f;
-                    bool bad = false;
-                    if (live)
-                        for (int d = 0; d < hd; d += 16) {
+                // the unit's rows, one per thread of four warps
+                if (c < kRows) {
+                    const int qr = (warp & 3) * 32 + lane;
+                    if (sn > 0) wait(&q_free, (sn - 1) & 1);
+                    tc_fence_after();
+                    if constexpr (C::QT) {       // this warp's 32 TMEM lanes are its rows
+                        const int x = at + (warp & 3);
+                        wait(&raw_full[x % C::NRAW], (x / C::NRAW) & 1);
+                        const unsigned char* mine = raw + x % C::NRAW * RAWS + lane * RS;
+                        s_row[sn & 1][qr] = *reinterpret_cast<const float*>(mine + HD * sizeof(T));
+#pragma unroll 1
+                        for (int d = 0; d < HD * (int)sizeof(T); d += 64) {
+                            uint32_t v[16];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                *reinterpret_cast<uint4*>(v + 4 * i) = *reinterpret_cast<const uint4*>(mine + d + 16 * i);
+                            // lo halves begin 64 columns further
+                            tmem_st16(tmem + ((uint32_t)((warp & 3) * 32) << 16) + kQ + (d < HD * 2 ? d / 4 : 64 + (d - HD * 2) / 4), v);
+                        }
+                        tmem_st_wait();
+                    } else {                     // head sizes above 128: straight from the rows
+                        const int f = seg.m * kRows + qr;
+                        const bool live = f < seg.rows;
+                        const T* q = static_cast<const T*>(a.q) + (int64_t)(seg.r0 + f / G) * a.q_stride +
+                                     (int64_t)(seg.h * G + f % G) * hd;
+                        uint32_t top = 0u;
+#pragma unroll 1
+                        for (int d = 0; live && d < hd; d += 16) {
                             float y[16];
-                            load16(a.q, a.type, at + d, y);
+                            load_row16<T>(q + d, y);
 #pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                mx = fmaxf(mx, fabsf(y[i])), bad |= !(fabsf(y[i]) <= 3.402823466e38f);
+                            for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
                         }
-                    // the largest element to [2^13, 2^14)
-                    const int e = mx > 0.0f && !bad ? min(max(13 - ilogbf(mx), -120), 120) : 0;
-                    const float up = a.scale < 0.0f ? -exp2f((float)e) : exp2f((float)e);
-                    s_row[sn & 1][c] = bad ? NAN : fabsf(a.scale) * kLog2e * exp2f((float)-e);
-                    for (int d = 0; d < HD; d += 16) {
-                        float y[16];
+                        float up;
+                        bool bad;
+                        s_row[sn & 1][qr] = row_factor(top, a.scale, &up, &bad);
+#pragma unroll 1
+                        for (int d = 0; d < HD; d += 16) {
+                            float y[16];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) y[i] = 0.0f;
-                        if (live && !bad && d < hd) load16(a.q, a.type, at + d, y);
-                        uint32_t hh[8], ll[8];
+                            for (int i = 0; i < 16; ++i) y[i] = 0.0f;
+                            if (live && !bad && d < hd) load_row16<T>(q + d, y);
+                            uint32_t hh[8], ll[8];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float y0 = y[2 * i] * up, y1 = y[2 * i + 1] * up;
-                            const __half2 h2 = __floats2half2_rn(y0, y1);
-                            const float2 b2 = __half22float2(h2);
-                            hh[i] = bits(h2);
-                            if (Q2) ll[i] = bits(__floats2half2_rn(y0 - b2.x, y1 - b2.y));
+                            for (int i = 0; i < 8; ++i) {
+                                const float y0 = y[2 * i] * up, y1 = y[2 * i + 1] * up;
+                                const __half2 h2 = __floats2half2_rn(y0, y1);
+                                const float2 b2 = __half22float2(h2);
+                                hh[i] = bits(h2), ll[i] = bits(__floats2half2_rn(y0 - b2.x, y1 - b2.y));
+                            }
+                            unsigned char* r = sq + d / 64 * C::QSLAB + qr * 128;
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                const int at16 = ((d % 64 / 8 + x) ^ (qr & 7)) * 16;
+                                *reinterpret_cast<uint4*>(r + at16) =
+                                    make_uint4(hh[4 * x], hh[4 * x + 1], hh[4 * x + 2], hh[4 * x + 3]);
+                                if (Q2)
+                                    *reinterpret_cast<uint4*>(r + C::SLABS * C::QSLAB + at16) =
+                                        make_uint4(ll[4 * x], ll[4 * x + 1], ll[4 * x + 2], ll[4 * x + 3]);
+                            }
                         }
-                        const int slab = d / 64, ch = d % 64 / 8;
-                        unsigned char* r = sq + slab * C::QSLAB + c * 128;
-                        const int c0 = (ch ^ (c & 7)) * 16, c1 = ((ch + 1) ^ (c & 7)) * 16;
-                        *reinterpret_cast<uint4*>(r + c0) = make_uint4(hh[0], hh[1], hh[2], hh[3]);
-                        *reinterpret_cast<uint4*>(r + c1) = make_uint4(hh[4], hh[5], hh[6], hh[7]);
-                        if (Q2) {
-                            r += C::SLABS * C::QSLAB;
-                            *reinterpret_cast<uint4*>(r + c0) = make_uint4(ll[0], ll[1], ll[2], ll[3]);
-                            *reinterpret_cast<uint4*>(r + c1) = make_uint4(ll[4], ll[5], ll[6], ll[7]);
-                        }
+                        fence_async_smem();
                     }
+                    tc_fence_before();
+                    mbar_arrive(&q_full);
                 }
-                fence_async_smem();
-                mbar_arrive(&q_full);
+                if (C::QT) {
+                    at += NQ;
+                    named_barrier_sync(3, C::CONV);
+#pragma unroll 1
+                    for (int i = 0; i < NQ; ++i) copy();
+                }
                 const int n = seg.n;
 #pragma unroll 1
                 for (int jz = 0; jz < 2 * n; ++jz) {
-                    const int z = jz & 1, T = J + (jz >> 1), kb = T % C::NBUF;
-#pragma unroll
-                    for (int i = 0; i < PER; ++i) cur[i] = nxt[i];
-                    load();
-                    if (z == 0 && c < 2 * NG) {
-                        const int t = (seg.j + (jz >> 1)) * BN + c % NG * 16;
-                        const float* s = (c < NG ? a.c.ks : a.c.vs) + seg.slot * a.c.scale_stride +
-                                         (int64_t)seg.h * (a.c.cap / B);
-                        // tile T - 4's readers are done: V of tile T - 1 went in after their weights
-                        s_scale[T & 3][c] = t < seg.p + seg.rows / G ? s[t / B] : 0.0f;
-                    }
-                    if (T >= C::NBUF) wait(z ? &v_free[kb] : &k_free[kb], ((T - C::NBUF) / C::NBUF) & 1);
-                    unsigned char* tile = (z ? sv : sk) + kb * C::TILE;
+                    const int z = jz & 1, tl = J + (jz >> 1), kb = tl % C::NBUF;
+                    wait(&raw_full[at % C::NRAW], (at / C::NRAW) & 1);
+                    const unsigned char* codes = raw + at % C::NRAW * RAWS + row0 * hd + ch * 16;
+                    uint4 x[PER];
 #pragma unroll
                     for (int i = 0; i < PER; ++i) {
-                        const int idx = i * 128 + c, row = idx / CH, ch = idx % CH;
-                        put_codes(tile + (ch / 4) * C::SLAB, row, ch % 4, (ch / 4) & 1, cur[i]);
+                        x[i] = make_uint4(0, 0, 0, 0);
+                        if (live_ch && ((i + 1) * STEP <= BN || row0 + i * STEP < BN))
+                            x[i] = *reinterpret_cast<const uint4*>(codes + i * STEP * hd);
                     }
+                    if (tl >= C::NBUF) wait(z ? &v_free[kb] : &k_free[kb], ((tl - C::NBUF) / C::NBUF) & 1);
+                    unsigned char* tile = (z ? sv : sk) + kb * C::TILE + (ch / 4) * C::SLAB;
+#pragma unroll
+                    for (int i = 0; i < PER; ++i)
+                        if ((i + 1) * STEP <= BN || row0 + i * STEP < BN)
+                            put_codes(tile + i * STEP * 128, row0, ch % 4, (ch / 4) & 1, x[i], STEP % 8 ? i * STEP : 0);
                     fence_async_smem();
                     mbar_arrive(z ? &v_full[kb] : &k_full[kb]);
+                    named_barrier_sync(3, C::CONV);                      // everybody has read the codes
+                    ++at;
+                    copy();
                 }
                 J += n, ++sn;
-            } while (seg.next(a, plan));
+            } while (seg.next(plan));
         }
     } else if (any) {
         // -------------------------------------------------------- softmax
-        const int w = C::STREAMS == 2 ? warp / 4 : 0, row = (warp & 3) * 32 + lane;
+        const int w = (warp - 1) / 4, row = (warp & 3) * 32 + lane;           // this thread's half of the columns, its row
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        constexpr int HC = BN / 2;
+        const int bsh = 31 - __clz(a.c.block);
         do {
             const int f = seg.m * kRows + row;
             const bool live = f < seg.rows;
             const int lim = seg.p + (live ? f : seg.rows - 1) / G;       // the last token that the row sees
             const int all_see = seg.p + seg.m * kRows / G;               // ... that every row sees
-            float m = -INFINITY, l = 0.0f, svr = 0.0f, rsv = 0.0f;
-            bool has = false;                                            // the stream's accumulator is written
+            float m = -INFINITY, l = 0.0f, lr = -200.0f;                 // lr: log2 of the V scale reference
+            // scales of a tile's 16-token groups, loaded a tile ahead: lanes 0-15
+            // K's, lanes 16-31 log2 of V's
+            const float* sc = (lane < 16 ? a.c.ks : a.c.vs) + seg.slot * a.c.scale_stride +
+                              (int64_t)seg.h * (a.c.cap >> bsh);
+            auto scale_of = [&](int t0) {
+                const int t = t0 + lane % 16 * 16;
+                return lane % 16 < NG && t < seg.p + seg.rows / G ? sc[t >> bsh] : 0.0f;
+            };
+            float coming = scale_of(seg.j * BN);
             for (int jj = 0; jj < seg.n; ++jj) {
-                const int T = J + jj;
-                if (C::STREAMS == 2 && (T & 1) != w) continue;
-                const int t0 = (seg.j + jj) * BN;
-                const bool cut = t0 + BN - 1 > all_see;                  // some row does not see the whole tile
-                const uint32_t ts = tmem + lanes + (T & 1) * BN;
-                wait(&s_full[T & 1], (T >> 1) & 1);
+                const int tl = J + jj, t0 = (seg.j + jj) * BN;
+                const uint32_t ts = tmem + lanes + (tl & 1) * BN + w * HC;
+                wait(&s_full[tl & 1], (tl >> 1) & 1);
                 tc_fence_after();
                 const float qs = s_row[sn & 1][row];
-                const float* sc = s_scale[T & 3];
-                float x = -INFINITY, xs = 0.0f;
-#pragma unroll 1
-                for (int c = 0; c < BN / 32; ++c) {
-                    uint32_t v[32];
-                    tmem_ld32(ts + c * 32, v);
-                    tmem_ld_wait();
-                    if (cut) {
+                const float scale = lane < 16 ? coming : __log2f(fmaxf(coming, 1.17549435e-38f));
+                if (jj + 1 < seg.n) coming = scale_of(t0 + BN);
+                float fk[NG / 2], fv[NG / 2];    // this half's groups: score factors, log2 of V's scales
 #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (t0 + c * 32 + i > lim) v[i] = 0xff800000u;
-                    }
+                for (int g = 0; g < NG / 2; ++g) {
+                    fk[g] = __shfl_sync(0xffffffffu, scale, w * (NG / 2) + g) * qs;
+                    fv[g] = __shfl_sync(0xffffffffu, scale, 16 + w * (NG / 2) + g);
+                }
+                const float lv_here = lane >= 16 ? scale : -200.0f;
+                // the scores are read once (a TMEM load waits long while products run)
+                uint32_t v[HC];
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) {
+                for (int c = 0; c < HC / 32; ++c) tmem_ld32(ts + c * 32, v + c * 32);
+                tmem_ld_wait();
+                // seen: how many of this thread's columns the row sees, where some row does not see all
+                auto largest = [&](auto cut, int seen) {
+                    float x = -INFINITY;
+#pragma unroll
+                    for (int g = 0; g < HC / 16; ++g) {
+                        if (cut) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                if (16 * g + i >= seen) v[16 * g + i] = 0xff800000u;
+                        }
                         float y = __uint_as_float(v[16 * g]);
 #pragma unroll
-                        for (int i = 1; i < 16; ++i) y = fmaxf(y, __uint_as_float(v[16 * g + i]));
-                        if (y != -INFINITY) x = fmaxf(x, y * (sc[2 * c + g] * qs));
-                        xs = fmaxf(xs, sc[NG + 2 * c + g]);
+                        for (int i = 1; i < 15; i += 2)
+                            y = fmaxf(fmaxf(y, __uint_as_float(v[16 * g + i])), __uint_as_float(v[16 * g + i + 1]));
+                        y = fmaxf(y, __uint_as_float(v[16 * g + 15]));
+                        if (y != -INFINITY) x = fmaxf(x, y * fk[g]);
                     }
-                }
-                if (__any_sync(0xffffffffu, x > m + kLazyScore || xs > svr * kLazyScale)) {
-                    const float xm = fmaxf(x, m), xv = fmaxf(xs, svr);
-                    const float el = xm == m ? 1.0f : ex2(m - xm), eo = el * (xv > 0.0f ? svr / xv : 0.0f);
-                    if (has) {
-                        if (C::STREAMS == 1 && T > 0) {                  // the products of the tile before
-                            wait(&v_free[(T - 1) % C::NBUF], ((T - 1) / C::NBUF) & 1);
-                            tc_fence_after();
+                    return x;
+                };
+                auto weights = [&](auto cut, int seen) {
+#pragma unroll
+                    for (int g = 0; g < HC / 16; ++g) {
+                        uint32_t p[16];          // hi, lo
+                        // 2^7 sv / sv_ref joins the exponent; the sum of the weights without it
+                        const float lv = fmaxf(fv[g] - lr + kWeightLog, -40.0f), fz = fk[g], off = lv - m;
+                        const uint64_t fz2 = pack2(fz, fz), off2 = pack2(off, off);
+                        uint64_t sum = 0;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int k = 16 * g + 2 * i;
+                            float z0, z1;
+                            unpack2(fma2(pack2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), fz2, off2), z0, z1);
+                            float w0 = ex2(z0), w1 = ex2(z1);
+                            if (cut) {
+                                if (k >= seen) w0 = 0.0f;
+                                if (k + 1 >= seen) w1 = 0.0f;
+                            }
+                            const uint64_t w2 = pack2(w0, w1);
+                            sum = add2(sum, w2);
+                            // hi: 11 bits, lo: the rest, 21 together
+                            const float h0 = __uint_as_float(__float_as_uint(w0) & 0xffffe000u);
+                            const float h1 = __uint_as_float(__float_as_uint(w1) & 0xffffe000u);
+                            float r0, r1;
+                            unpack2(sub2(w2, pack2(h0, h1)), r0, r1);
+                            p[i] = bits(__floats2half2_rn(h0, h1));
+                            p[8 + i] = bits(__floats2half2_rn(r0, r1));
                         }
-                        const uint32_t to = tmem + lanes + kO + (C::STREAMS == 2 ? w * HD : 0);
+                        float a0, a1;
+                        unpack2(sum, a0, a1);
+                        l = fmaf(a0 + a1, ex2(-lv), l);
+                        tmem_st16(ts + g * 16, p);
+                    }
+                };
+                const bool cut = t0 + BN - 1 > all_see;
+                const int seen = lim + 1 - t0 - w * HC;
+                const float x = cut ? largest(std::true_type{}, seen) : largest(std::false_type{}, 0);
+                if (barrier_any(1, C::SOFT, x > m + kLazyScore || lv_here > lr + kLazyLog)) {
+                    s_half[w][row] = x;
+                    named_barrier_sync(2, C::SOFT);
+                    float xs = lv_here;
+#pragma unroll
+                    for (int d = 16; d; d >>= 1) xs = fmaxf(xs, __shfl_xor_sync(0xffffffffu, xs, d));
+                    const float xm = fmaxf(fmaxf(x, s_half[w ^ 1][row]), m), xr = fmaxf(xs, lr);
+                    const float el = xm == m ? 1.0f : ex2(m - xm), eo = el * ex2(lr - xr);
+                    if (jj > 0) {                // the products of the tile before are in
+                        wait(&v_free[(tl - 1) % C::NBUF], ((tl - 1) / C::NBUF) & 1);
+                        tc_fence_after();
+                        const uint32_t to = tmem + lanes + kO + w * (HD / 2);
 #pragma unroll 1
-                        for (int c = 0; c < HD / 16; ++c) {
+                        for (int c = 0; c < HD / 32; ++c) {
                             uint32_t v[16];
                             tmem_ld16(to + c * 16, reinterpret_cast<int*>(v));
 #pragma unroll
@@ -466,114 +700,59 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                             tmem_st16(to + c * 16, v);
                         }
                     }
-                    l *= el, m = xm, svr = xv;
-                    rsv = svr > 1e-33f ? kWeightScale / svr : 0.0f;      // values below count as 0
+                    l *= el, m = xm, lr = xr;
                 }
-                has = true;
-#pragma unroll 1
-                for (int c = 0; c < BN / 32; ++c) {
-                    uint32_t v[32], ph[16], pl[16];
-                    tmem_ld32(ts + c * 32, v);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int g = 0; g < 2; ++g) {
-                        const float fz = sc[2 * c + g] * qs, fv = sc[NG + 2 * c + g] * rsv;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int k = 16 * g + 2 * i;
-                            float e0 = ex2(fmaf(__uint_as_float(v[k]), fz, -m));
-                            float e1 = ex2(fmaf(__uint_as_float(v[k + 1]), fz, -m));
-                            if (cut) {
-                                if (t0 + c * 32 + k > lim) e0 = 0.0f;
-                                if (t0 + c * 32 + k + 1 > lim) e1 = 0.0f;
-                            }
-                            l += e0 + e1;
-                            const float w0 = e0 * fv, w1 = e1 * fv;
-                            const __half2 h2 = __floats2half2_rn(w0, w1);
-                            ph[8 * g + i] = bits(h2);
-                            if (P2) {
-                                const float2 b2 = __half22float2(h2);
-                                pl[8 * g + i] = bits(__floats2half2_rn(w0 - b2.x, w1 - b2.y));
-                            }
-                        }
-                    }
-                    tmem_st16(ts + c * 32, ph);
-                    if (P2) tmem_st16(ts + c * 32 + 16, pl);
-                }
+                if (cut) weights(std::true_type{}, seen);
+                else weights(std::false_type{}, 0);
                 tmem_st_wait();
                 tc_fence_before();
-                mbar_arrive(&p_full[T & 1]);
+                mbar_arrive(&p_full[tl & 1]);
             }
-            // the unit's rows: both streams' accumulators joined
-            float(*st)[3][kRows] = s_stat[sn & 1];
-            st[w][0][row] = m, st[w][1][row] = l, st[w][2][row] = has ? svr * (1.0f / kWeightScale) : 0.0f;
+            // the unit's rows
             wait(&o_full, sn & 1);
             tc_fence_after();
-            named_barrier_sync(1, C::SOFT);
-            float mm = st[0][0][row];
-            if (C::STREAMS == 2) mm = fmaxf(mm, st[C::STREAMS - 1][0][row]);
-            float fo[2] = {0.0f, 0.0f}, ll = 0.0f;
-#pragma unroll
-            for (int s = 0; s < C::STREAMS; ++s) {
-                const float e = st[s][0][row] == -INFINITY ? 0.0f : ex2(st[s][0][row] - mm);
-                ll = fmaf(st[s][1][row], e, ll), fo[s] = st[s][2][row] * e;
-            }
-            // an accumulator that no tile of the unit went into holds what was there before
-            const bool two = C::STREAMS == 2 && seg.n > 1;
-            const int w0 = J & 1;                                        // the first tile's stream
+            barrier_any(1, C::SOFT, false);      // s_half is free
+            s_half[w][row] = l;
+            named_barrier_sync(2, C::SOFT);
+            l += s_half[w ^ 1][row];
             const bool whole = seg.j == 0 && seg.n == seg.tiles;
-            const float inv = whole ? 1.0f / ll : 1.0f;
+            const float fo = ex2(lr - kWeightLog) * (whole ? 1.0f / l : 1.0f);
             const int64_t orow = (int64_t)(seg.r0 + f / G) * a.heads + seg.h * G + f % G;
             float* pt = parts + ((int64_t)blockIdx.x * 2 + (seg.j == 0)) * C::PART;
-            constexpr int COLS = HD / C::STREAMS;
 #pragma unroll 1
-            for (int c = w * COLS; c < (w + 1) * COLS; c += 16) {
-                int o0[16], o1[16];
-                const uint32_t to = tmem + lanes + kO + c;
-                tmem_ld16(to + (C::STREAMS == 2 ? w0 * HD : 0), o0);
-                if (two) tmem_ld16(to + (w0 ^ 1) * HD, o1);
+            for (int c = w * (HD / 2); c < (w + 1) * (HD / 2); c += 16) {
+                int o[16];
+                tmem_ld16(tmem + lanes + kO + c, o);
                 float y[16];
-                const float f0 = fo[C::STREAMS == 2 ? w0 : 0] * inv, f1 = fo[C::STREAMS == 2 ? w0 ^ 1 : 0] * inv;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    y[i] = __int_as_float(o0[i]) * f0;
-                    if (two) y[i] = fmaf(__int_as_float(o1[i]), f1, y[i]);
-                }
+                for (int i = 0; i < 16; ++i) y[i] = __int_as_float(o[i]) * fo;
                 if (!whole) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         *reinterpret_cast<float4*>(pt + row * HD + c + 4 * i) =
                             make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
                 } else if (live && c < hd) {
-                    if (a.type == KVB_F32) {
-                        float4* o = reinterpret_cast<float4*>(static_cast<float*>(a.out) + orow * hd + c);
+                    T* to = static_cast<T*>(a.out) + orow * hd + c;
+                    if constexpr (Q2) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) o[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+                        for (int i = 0; i < 4; ++i)
+                            reinterpret_cast<float4*>(to)[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
                     } else {
-                        uint32_t q[8];
+                        T q[16];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            if (a.type == KVB_BF16) {
-                                const __nv_bfloat162 z = __floats2bfloat162_rn(y[2 * i], y[2 * i + 1]);
-                                q[i] = *reinterpret_cast<const uint32_t*>(&z);
-                            } else {
-                                q[i] = bits(__floats2half2_rn(y[2 * i], y[2 * i + 1]));
-                            }
-                        }
-                        uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + orow * hd + c);
-                        o[0] = make_uint4(q[0], q[1], q[2], q[3]), o[1] = make_uint4(q[4], q[5], q[6], q[7]);
+                        for (int i = 0; i < 16; ++i) q[i] = kvb_t<T>(y[i]);
+                        reinterpret_cast<uint4*>(to)[0] = reinterpret_cast<const uint4*>(q)[0];
+                        reinterpret_cast<uint4*>(to)[1] = reinterpret_cast<const uint4*>(q)[1];
                     }
                 }
             }
             if (w == 0) {
-                if (!whole) pt[kRows * HD + row] = mm, pt[kRows * (HD + 1) + row] = ll;
-                else if (stats && live) stats[orow] = make_float2(mm, 1.0f / ll);
+                if (!whole) pt[kRows * HD + row] = m, pt[kRows * (HD + 1) + row] = l;
+                else if (stats && live) stats[orow] = make_float2(m, 1.0f / l);
             }
-            tc_fence_before();
-            named_barrier_sync(1, C::SOFT);      // the accumulators may be overwritten
-            tc_fence_after();
+            tc_fence_before();                   // the next unit's first weights let the accumulator go
             J += seg.n, ++sn;
-        } while (seg.next(a, plan));
+        } while (seg.next(plan));
     }
     tc_fence_before();
     __syncthreads();
@@ -605,7 +784,7 @@ __global__ void __launch_bounds__(kFinishThreads) kvb_rows_finish(const KvbAttnA
     rows_share(plan, a.c.heads, grid, blockIdx.x - 1, &plo, &phi);
     if (lo >= hi) return;
     Seg s;
-    s.begin(a, plan, lo, hi);
+    s.begin(plan, lo, hi);
     if (s.j == 0 || plo > lo - s.j) return;      // not cut here, or first cut before
     const int64_t end = lo - s.j + s.tiles;
     int last = blockIdx.x;                       // the last share with a part of the unit
@@ -649,43 +828,185 @@ __global__ void __launch_bounds__(kFinishThreads) kvb_rows_finish(const KvbAttnA
 }
 
 // mass[t] += the probabilities of token t over the rows and the query heads of
-// its KV head: one thread per token, in row order.
+// its KV head, from the rows' maxima and sums: the scores once more, tokens as
+// the 16 rows of mma m16n8k16 (the codes as halves in registers for the whole
+// kernel), the prepared queries as its columns (hi and lo into one accumulator).
+// A warp holds 16 TG tokens; with few token tiles the CTA's four warps hold the
+// same ones and share out the rows (SPLIT 4), else they hold four tiles and
+// share the queries they read (SPLIT 1). Sums run in a fixed order: 32 rows at a
+// time, then over the warps. Bound by the tensor products and their exponentials.
 constexpr int kMassThreads = 128;
-__global__ void __launch_bounds__(kMassThreads) kvb_rows_mass(const KvbAttnArgs a, const float2* stats) {
+
+template <int HD, bool Q2>
+struct MassCfg {
+    static constexpr int TG = HD == 256 ? 1 : 2;
+    static constexpr int RS = RowsCfg<HD>::qrow(Q2 ? 4 : 2), CHUNK = 32 * RS;
+};
+
+__device__ __forceinline__ void mma_halves(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <int HD, bool Q2, int SPLIT>
+__global__ void __launch_bounds__(kMassThreads) kvb_rows_mass(const KvbAttnArgs a, const RowsPlan plan,
+                                                            const unsigned char* queries, int units, const float2* stats) {
+    using M = MassCfg<HD, Q2>;
+    constexpr int TG = M::TG, RS = M::RS, KB = HD / 32, TOK = 16 * TG;   // 32-channel blocks; tokens of a warp
+    extern __shared__ __align__(128) unsigned char smem[];               // [2][SPLIT][CHUNK]
+    __shared__ __align__(8) uint64_t full[2];
+    __shared__ float2 s_stat[2][SPLIT][32];
+    __shared__ float s_sum[4][TOK];
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int h = blockIdx.y, b = blockIdx.z, hd = a.c.hd, G = a.heads / a.c.heads;
+    if (tid == 0) {
+        mbar_init(&full[0], 1), mbar_init(&full[1], 1);
+        mbar_fence_init();
+    }
     pdl_wait();
     pdl_trigger();
-    const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, t = blockIdx.x * kMassThreads + tid;
     const KvbSpan sp = kvb_span(a.r, b);
-    const int n = live_rows(sp, a.c.cap), hd = a.c.hd, G = a.heads / a.c.heads, B = a.c.block;
-    if (n <= 0 || blockIdx.x * kMassThreads >= sp.p + n) return;
-    __shared__ __align__(16) float q[kKvbMaxHd];
-    const int64_t head = b * a.c.slot_stride + (int64_t)h * a.c.cap * hd;
-    const float sk = t < sp.p + n ? a.c.ks[b * a.c.scale_stride + (int64_t)h * (a.c.cap / B) + t / B] : 0.0f;
-    float sum = 0.0f;
-    for (int i = 0; i < n; ++i) {
-        for (int g = 0; g < G; ++g) {
-            const int64_t r = sp.r0 + i;
-            __syncthreads();
-            for (int d = tid * 16; d < hd; d += kMassThreads * 16) {
-                load16(a.q, a.type, r * a.q_stride + (int64_t)(h * G + g) * hd + d, q + d);
+    const int n = live_rows(sp, a.c.cap), len = sp.p + n, rows = n * G;
+    const int tile = blockIdx.x * TOK * (4 / SPLIT), t0 = tile + warp / SPLIT * TOK;   // the CTA's, the warp's first token
+    if (n == 0 || tile >= len) return;
+    if (plan.first[b] + (rows + kRows - 1) / kRows > plan.head[1]) return;   // only with offsets out of order
+    __syncthreads();
+
+    // the warp's tokens: channels 32 x + 8 t + 0..7 of rows g and g + 8
+    uint32_t k[TG][KB][2][4];
+    float sk[TG];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) q[d + e] *= a.scale * kLog2e;
-            }
-            __syncthreads();
-            if (t > sp.p + i) continue;
-            const uint4* row = reinterpret_cast<const uint4*>(a.c.k + head + (int64_t)t * hd);
-            float z = 0.0f;
-            for (int c = 0; c < hd / 16; ++c) {
-                const uint4 w = row[c];
-                const int8_t* k = reinterpret_cast<const int8_t*>(&w);
+    for (int j = 0; j < TG; ++j) {
+        sk[j] = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) z = fmaf((float)k[e], q[c * 16 + e], z);
+        for (int x = 0; x < KB; ++x) {
+            uint2 w[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int tok = t0 + 16 * j + 8 * r + g;
+                w[r] = make_uint2(0, 0);
+                if (tok < len && 32 * x + 8 * t < hd)
+                    w[r] = *reinterpret_cast<const uint2*>(a.c.k + b * a.c.slot_stride +
+                                                           ((int64_t)h * a.c.cap + tok) * hd + 32 * x + 8 * t);
+                w[r].x ^= 0x80808080u, w[r].y ^= 0x80808080u;
             }
-            const float2 st = stats[r * a.heads + h * G + g];
-            sum = fmaf(ex2(z * sk - st.x), st.y, sum);
+            k[j][x][0][0] = halves_of(w[0].x, 0x4140), k[j][x][0][1] = halves_of(w[1].x, 0x4140);
+            k[j][x][0][2] = halves_of(w[0].x, 0x4342), k[j][x][0][3] = halves_of(w[1].x, 0x4342);
+            k[j][x][1][0] = halves_of(w[0].y, 0x4140), k[j][x][1][1] = halves_of(w[1].y, 0x4140);
+            k[j][x][1][2] = halves_of(w[0].y, 0x4342), k[j][x][1][3] = halves_of(w[1].y, 0x4342);
         }
+        if (t0 + 16 * j < len)                   // 16 tokens lie in one block
+            sk[j] = a.c.ks[b * a.c.scale_stride + (int64_t)h * (a.c.cap / a.c.block) + (t0 + 16 * j) / a.c.block];
     }
-    if (t < sp.p + n) a.mass[((int64_t)b * a.c.heads + h) * a.c.cap + t] += sum;
+    // chunks of 32 rows (f = query row * G + head), from the first that sees the tile
+    const unsigned char* src = queries + ((int64_t)h * units + plan.first[b]) * 4 * M::CHUNK;
+    const int c0 = max(tile - sp.p, 0) * G / 32, c1 = (rows + 31) / 32;
+    auto fetch = [&](int step) {                 // SPLIT chunks and their rows' maxima and sums
+        const int s = step & 1, c = c0 + step * SPLIT, m = min(SPLIT, c1 - c);
+        if (m <= 0) return;
+        if (tid == 0) {
+            mbar_expect_tx(&full[s], m * M::CHUNK);
+            bulk_g2s(smem + s * SPLIT * M::CHUNK, src + (int64_t)c * M::CHUNK, m * M::CHUNK, &full[s]);
+        }
+        if (tid < 32 * SPLIT) {
+            const int f = c * 32 + tid;          // rows past the last weigh nothing
+            s_stat[s][tid / 32][tid % 32] =
+                f < rows ? stats[(int64_t)(sp.r0 + f / G) * a.heads + h * G + f % G] : make_float2(0.0f, 0.0f);
+        }
+    };
+    fetch(0);
+    fetch(1);
+    float sum[TG][2];
+#pragma unroll
+    for (int j = 0; j < TG; ++j) sum[j][0] = sum[j][1] = 0.0f;
+    const int steps = (c1 - c0 + SPLIT - 1) / SPLIT;
+    for (int step = 0; step < steps; ++step) {
+        const int s = step & 1, c = c0 + step * SPLIT + warp % SPLIT;
+        if (!mbar_wait(&full[s], (step >> 1) & 1) && lane == 0) atomicOr(&g_kvb_rows_errors, kErrWait);
+        __syncthreads();                         // s_stat as well
+        if (c < c1) {
+            const unsigned char* q = smem + (s * SPLIT + warp % SPLIT) * M::CHUNK;
+            const bool cut = sp.p + c * 32 / G < t0 + TOK - 1;           // some row does not see every token
+            float part[TG][2];
+#pragma unroll
+            for (int j = 0; j < TG; ++j) part[j][0] = part[j][1] = 0.0f;
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {        // 8 rows
+                float z[TG][4];
+#pragma unroll
+                for (int j = 0; j < TG; ++j) z[j][0] = z[j][1] = z[j][2] = z[j][3] = 0.0f;
+                const unsigned char* qr = q + (i * 8 + g) * RS + 16 * t;
+#pragma unroll
+                for (int x = 0; x < KB; ++x)
+#pragma unroll
+                    for (int y = 0; y < (Q2 ? 2 : 1); ++y) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(qr + y * HD * 2 + x * 64);
+#pragma unroll
+                        for (int j = 0; j < TG; ++j) {
+                            mma_halves(z[j], k[j][x][0], w.x, w.y);
+                            mma_halves(z[j], k[j][x][1], w.z, w.w);
+                        }
+                    }
+                // columns: rows c * 32 + 8 i + 2 t + e
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int col = i * 8 + 2 * t + e, f = c * 32 + col;
+                    const float fq = *reinterpret_cast<const float*>(q + col * RS + (RS - 16));
+                    const float2 st = s_stat[s][warp % SPLIT][col];
+                    const int lim = f < rows ? sp.p + f / G : -1;
+#pragma unroll
+                    for (int j = 0; j < TG; ++j)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            float w = ex2(fmaf(z[j][2 * r + e], sk[j] * fq, -st.x)) * st.y;
+                            if ((cut || f >= rows) && t0 + 16 * j + 8 * r + g > lim) w = 0.0f;
+                            part[j][r] += w;
+                        }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < TG; ++j) sum[j][0] += part[j][0], sum[j][1] += part[j][1];
+        }
+        __syncthreads();
+        fetch(step + 2);
+    }
+#pragma unroll
+    for (int j = 0; j < TG; ++j)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            sum[j][r] += __shfl_xor_sync(0xffffffffu, sum[j][r], 1);
+            sum[j][r] += __shfl_xor_sync(0xffffffffu, sum[j][r], 2);
+            if (t == 0) s_sum[warp][16 * j + 8 * r + g] = sum[j][r];
+        }
+    __syncthreads();
+    for (int i = tid; i < TOK * (4 / SPLIT); i += kMassThreads) {
+        const int tok = tile + i;
+        if (tok >= len) break;
+        const int w0 = i / TOK * SPLIT;
+        float y = 0.0f;
+#pragma unroll
+        for (int w = 0; w < SPLIT; ++w) y += s_sum[w0 + w][i % TOK];
+        a.mass[((int64_t)b * a.c.heads + h) * a.c.cap + tok] += y;
+    }
+}
+
+template <int HD, bool Q2>
+cudaError_t mass_launch(const KvbAttnArgs& a, const RowsPlan& plan, const unsigned char* queries, int units,
+                        const float2* stats, cudaStream_t st) {
+    using M = MassCfg<HD, Q2>;
+    constexpr int TOK = 16 * M::TG;
+    // four tiles a CTA once that still gives every SM two CTAs (by the capacity:
+    // the lengths are device data)
+    const int64_t tiles = (a.c.cap + TOK - 1) / TOK;
+    const bool share = tiles / 4 * a.c.heads * a.c.slots >= 2 * kSms || HD == 256;
+    const auto kern = share ? kvb_rows_mass<HD, Q2, 1> : kvb_rows_mass<HD, Q2, HD == 256 ? 1 : 4>;
+    const size_t smem = (size_t)2 * (share ? 1 : 4) * M::CHUNK;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    return launch_k(kern, dim3((unsigned)(share ? (tiles + 3) / 4 : tiles), a.c.heads, a.c.slots), dim3(kMassThreads), smem,
+                    st, a, plan, queries, units, stats);
 }
 
 int rows_hd(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
@@ -693,46 +1014,55 @@ int rows_hd(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 size_t up16(size_t x) { return (x + 15) & ~(size_t)15; }
 
 struct RowsLayout {                              // byte offsets in the scratch
-    size_t unit, first, parts, stats, total;
-    RowsLayout(const KvbCache& c, int heads, int rows, bool mass) {
+    size_t unit, first, parts, stats, queries, total;
+    RowsLayout(const KvbCache& c, int heads, int rows, bool mass, int qbytes) {
         const int hd = rows_hd(c.hd);
         unit = 16;
-        first = unit + (size_t)max_units(c, heads, rows) * sizeof(int4);
+        first = unit + (size_t)max_units(c, heads, rows) * sizeof(RowsUnit);
         parts = up16(first + ((size_t)c.slots + 1) * sizeof(int));
         stats = parts + (size_t)kSms * 2 * kRows * (hd + 2) * sizeof(float);
-        total = stats + (mass ? (size_t)rows * heads * sizeof(float2) : 0);
+        queries = up16(stats + (mass ? (size_t)rows * heads * sizeof(float2) : 0));
+        total = queries + (hd <= 128 || mass ? (size_t)max_units(c, heads, rows) * c.heads * kRows * (hd * qbytes + 16) : 0);
     }
 };
 
 template <int HD>
 cudaError_t rows_launch(const KvbAttnArgs& a, cudaStream_t st) {
     using C = RowsCfg<HD>;
-    const RowsLayout L(a.c, a.heads, a.r.rows, a.mass != nullptr);
+    const int qbytes = a.type == KVB_F32 ? 4 : 2, units = (int)max_units(a.c, a.heads, a.r.rows);
+    const RowsLayout L(a.c, a.heads, a.r.rows, a.mass != nullptr, qbytes);
     char* s = static_cast<char*>(a.scratch);
-    const RowsPlan plan{reinterpret_cast<int*>(s), reinterpret_cast<int4*>(s + L.unit), reinterpret_cast<int*>(s + L.first)};
+    const RowsPlan plan{reinterpret_cast<int*>(s), reinterpret_cast<RowsUnit*>(s + L.unit), reinterpret_cast<int*>(s + L.first)};
     float* parts = reinterpret_cast<float*>(s + L.parts);
     float2* stats = a.mass ? reinterpret_cast<float2*>(s + L.stats) : nullptr;
-    cudaError_t e = launch_k(kvb_rows_plan, dim3(1), dim3(kPlanThreads), 0, st, a, plan, C::BN,
-                             (int)max_units(a.c, a.heads, a.r.rows));
+    cudaError_t e = launch_k(kvb_rows_plan, dim3(1), dim3(kPlanThreads), 0, st, a, plan, C::BN, units);
     if (e != cudaSuccess) return e;
-    const bool q2 = a.type == KVB_F32;
-    const auto kern = a.type == KVB_F32    ? kvb_rows_kernel<HD, true, true>
-                      : a.type == KVB_BF16 ? kvb_rows_kernel<HD, false, false>
-                                           : kvb_rows_kernel<HD, false, true>;
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::smem(q2));
+    unsigned char* queries = reinterpret_cast<unsigned char*>(s + L.queries);
+    if (C::QT || a.mass) {
+        const auto prep = a.type == KVB_F32    ? kvb_rows_queries<HD, float>
+                          : a.type == KVB_BF16 ? kvb_rows_queries<HD, __nv_bfloat16>
+                                               : kvb_rows_queries<HD, __half>;
+        e = launch_k(prep, dim3(units * 4, a.c.heads), dim3(kQueryWarps * 32), 0, st, a, plan, queries, units);
+        if (e != cudaSuccess) return e;
+    }
+    const auto kern = a.type == KVB_F32    ? kvb_rows_kernel<HD, float>
+                      : a.type == KVB_BF16 ? kvb_rows_kernel<HD, __nv_bfloat16>
+                                           : kvb_rows_kernel<HD, __half>;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::smem(qbytes));
     if (e != cudaSuccess) return e;
-    e = launch_k(kern, dim3(kSms), dim3(C::THREADS), C::smem(q2), st, a, plan, parts, stats);
+    e = launch_k(kern, dim3(kSms), dim3(C::THREADS), C::smem(qbytes), st, a, plan,
+                 (const unsigned char*)queries, units, parts, stats);
     if (e != cudaSuccess) return e;
     e = launch_k(kvb_rows_finish<HD>, dim3(kSms), dim3(kFinishThreads), 0, st, a, plan, (const float*)parts, stats, kSms);
     if (e != cudaSuccess || !stats) return e;
-    return launch_k(kvb_rows_mass, dim3((a.c.cap + kMassThreads - 1) / kMassThreads, a.c.heads, a.c.slots),
-                    dim3(kMassThreads), 0, st, a, (const float2*)stats);
+    return qbytes == 4 ? mass_launch<HD, true>(a, plan, queries, units, stats, st)
+                       : mass_launch<HD, false>(a, plan, queries, units, stats, st);
 }
 
 }  // namespace
 
-size_t kvb_rows_scratch(const KvbCache& c, int heads, int rows, bool mass) {
-    return RowsLayout(c, heads, rows, mass).total;
+size_t kvb_rows_scratch(const KvbCache& c, int heads, int rows, bool mass, int qbytes) {
+    return RowsLayout(c, heads, rows, mass, qbytes).total;
 }
 
 cudaError_t launch_kvb_rows(const KvbAttnArgs& a, cudaStream_t st) {

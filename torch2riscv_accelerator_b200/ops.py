@@ -520,10 +520,11 @@ def kvb_read(cache, pos, start, rows, dtype=F32, k=None, v=None):
     return k, v
 
 
-def kvb_attn_scratch(cache, heads, rows, start=True, mass=False):
+def kvb_attn_scratch(cache, heads, rows, start=True, mass=False, dtype=F32):
     """Scratch for kvb_attn (start False) or kvb_attn_rows (True) calls of at
     most `rows` rows; one per call that may overlap another."""
-    n = _lib.load().w8a8_kvb_attn_scratch_bytes(ctypes.byref(_kvb(cache)), heads, rows, int(not start), int(mass))
+    n = _lib.load().w8a8_kvb_attn_scratch_bytes(ctypes.byref(_kvb(cache)), heads, rows, int(not start), int(mass),
+                                                _KVB_TYPES[dtype])
     return torch.empty(n, dtype=torch.uint8, device=cache[0].device)
 
 
@@ -543,7 +544,7 @@ def _kvb_attn(q, cache, pos, start, scale, mass, out, scratch):
         raise ValueError(f"out: a contiguous {q.dtype} {tuple(q.shape)} tensor is required")
     if scratch is None:
         n = _lib.load().w8a8_kvb_attn_scratch_bytes(ctypes.byref(c), heads, rows, int(start is None),
-                                                    int(mass is not None))
+                                                    int(mass is not None), dt)
         scratch = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
     elif scratch.device != dev:
         raise ValueError(f"scratch: a tensor on {dev} is required")
