@@ -186,6 +186,11 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// x / y for y > 0; 32-bit where it fits (a 64-bit division is a subroutine)
+__device__ __forceinline__ int64_t div64(int64_t x, int64_t y) {
+    return x >> 32 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
+}
+
 // rint(num / den) saturated to +-127 as an int8 code, the quotient correctly
 // rounded before the rounding to an integer. The product with rcp ~ 1 / den is
 // within 3 ulp of the quotient (below 1e-4 for |quotient| <= 128), so only

@@ -74,11 +74,6 @@ __device__ __forceinline__ int step_len(const KvbAttnArgs& a, int b) {
     return p < 0 || p >= a.c.cap ? 0 : p + 1;
 }
 
-// x / y for y > 0; 32-bit where it fits (a 64-bit division is a subroutine)
-__device__ __forceinline__ int64_t div64(int64_t x, int64_t y) {
-    return x >> 32 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
-}
-
 // Tiles of the slots before slot b (*before, for every thread) and of all slots.
 __device__ __forceinline__ int64_t step_scan(const KvbAttnArgs& a, int tile, int b, int64_t* before) {
     __shared__ int s_sum[2][kThreads / 32];

@@ -51,6 +51,12 @@ constexpr int kSms = 148;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazyScore = 6.0f, kLazyLog = 2.0f, kWeightLog = 7.0f;   // log2: see kvb_attn.cu
 constexpr unsigned int kErrWait = 256u;          // error bit 8: a pipeline wait gave up
+// The tensor cores round each product's running sum towards zero: an accumulator
+// is moved out and begun anew every kFold tiles (fp32: relative error of an output over
+// 8,192 tokens: 6.3e-6 never moved, 1.8e-6 every 8, 1.0e-6 every 4, 4.8e-7 every
+// tile, where the time grows by a quarter).
+template <typename T>
+constexpr int kFold = sizeof(T) == 4 ? 4 : 32;   // (16-bit outputs round by 2e-4 and more)
 constexpr int kPlanThreads = 1024;
 constexpr int kFinishThreads = 256;
 
@@ -73,7 +79,9 @@ struct RowsCfg {
         return 1024 + (QT ? 0 : (size_t)(qbytes == 4 ? 2 : 1) * SLABS * QSLAB) + (size_t)NBUF * 2 * TILE +
                (size_t)NRAW * stage(qbytes);
     }
-    static constexpr size_t PART = (size_t)kRows * (HD + 2);   // floats of a partial unit
+    // floats of a partial unit, and of a CTA's moved-out accumulator: channels in
+    // fours, [HD / 4][row][4], then maxima and sums of the rows
+    static constexpr size_t PART = (size_t)kRows * (HD + 2), ACC = (size_t)kRows * HD;
 };
 
 struct __align__(16) RowsUnit {
@@ -167,7 +175,7 @@ struct Seg {
         x = x0, end = x1;
         if (x >= end) return false;
         const int total = plan.head[0];
-        h = (int)(x / total);
+        h = (int)div64(x, total);
         const int at = (int)(x - (int64_t)h * total);
         int lo = 0, hi = plan.head[1];
         while (hi - lo > 1) {
@@ -192,7 +200,7 @@ struct Seg {
 __device__ __forceinline__ void rows_share(const RowsPlan& plan, int heads, int grid, int cta, int64_t* lo, int64_t* hi) {
     const int64_t total = (int64_t)plan.head[0] * heads, ctas = total < grid ? total : grid;
     *lo = *hi = 0;
-    if (cta < ctas) *lo = total * cta / ctas, *hi = total * (cta + 1) / ctas;
+    if (cta < ctas) *lo = div64(total * cta, ctas), *hi = div64(total * (cta + 1), ctas);
 }
 
 // pairs of floats in one instruction
@@ -283,49 +291,45 @@ __device__ __forceinline__ float row_factor(uint32_t top, float scale, float* up
     return *bad ? NAN : fabsf(scale) * kLog2e * __int_as_float((127 - e) << 23);
 }
 
-// The units' query rows as the products take them, 32 rows a CTA, a warp per
-// row: halves in unit order, so that a stage of the main kernel's ring is one
-// run of memory. (Converted there, row by row, they cost each unit 12,000 cycles
-// of cold code and scattered loads between two streams of products.)
-constexpr int kQueryWarps = 8;
-
+// The units' query rows as the products take them, 32 rows a CTA, a lane per 8
+// channels: halves in unit order, so that a stage of the main kernel's ring is
+// one run of memory. (Converted there, row by row, they cost each unit 12,000
+// cycles of cold code and scattered loads between two streams of products.)
 template <int HD, typename T>
-__global__ void __launch_bounds__(kQueryWarps * 32) kvb_rows_queries(const KvbAttnArgs a, const RowsPlan plan,
-                                                                   unsigned char* out, int units) {
+__global__ void __launch_bounds__(HD / 8 * 32) kvb_rows_queries(const KvbAttnArgs a, const RowsPlan plan,
+                                                              unsigned char* out, int units) {
     pdl_wait();
     pdl_trigger();
-    constexpr int V = HD / 32, RS = RowsCfg<HD>::qrow(sizeof(T));
-    const int u = blockIdx.x / 4, part = blockIdx.x % 4, h = blockIdx.y, lane = threadIdx.x & 31, G = a.heads / a.c.heads;
+    constexpr int RS = RowsCfg<HD>::qrow(sizeof(T)), LPR = HD / 8;       // bytes, lanes of a row
+    const int u = blockIdx.x / 4, part = blockIdx.x % 4, h = blockIdx.y, G = a.heads / a.c.heads;
     if (u >= plan.head[1]) return;
     const RowsUnit v = plan.unit[u];
-    unsigned char* to = out + (((int64_t)h * units + u) * 4 + part) * 32 * RS;
-    for (int r = threadIdx.x / 32; r < 32; r += kQueryWarps) {
-        const int f = v.m * kRows + part * 32 + r;
-        float x[V];
-        uint32_t top = 0u;
+    const int r = threadIdx.x / LPR, d = threadIdx.x % LPR * 8, f = v.m * kRows + part * 32 + r;
+    float x[8];
+    uint32_t top = 0u;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            x[i] = 0.0f;
-            if (f < v.rows && lane * V < a.c.hd)
-                x[i] = kvb_f<T>(static_cast<const T*>(a.q)[(int64_t)(v.r0 + f / G) * a.q_stride +
-                                                           (int64_t)(h * G + f % G) * a.c.hd + lane * V + i]);
-            top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-        }
-        top = __reduce_max_sync(0xffffffffu, top);
-        float up;
-        bool bad;
-        const float factor = row_factor(top, a.scale, &up, &bad);
+    for (int i = 0; i < 8; ++i) x[i] = 0.0f;
+    if (f < v.rows && d < a.c.hd)
+        kvb_load8<T>(static_cast<const T*>(a.q) + (int64_t)(v.r0 + f / G) * a.q_stride + (int64_t)(h * G + f % G) * a.c.hd + d, x);
 #pragma unroll
-        for (int i = 0; i < V; i += 2) {
-            const float y0 = bad ? 0.0f : x[i] * up, y1 = bad ? 0.0f : x[i + 1] * up;
-            const __half2 h2 = __floats2half2_rn(y0, y1);
-            const float2 b2 = __half22float2(h2);
-            unsigned char* p = to + r * RS + (lane * V + i) * 2;
-            *reinterpret_cast<__half2*>(p) = h2;
-            if (sizeof(T) == 4) *reinterpret_cast<__half2*>(p + HD * 2) = __floats2half2_rn(y0 - b2.x, y1 - b2.y);
-        }
-        if (lane == 0) *reinterpret_cast<float*>(to + r * RS + HD * (int)sizeof(T)) = factor;
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+#pragma unroll
+    for (int i = 1; i < LPR; i <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, i));
+    float up;
+    bool bad;
+    const float factor = row_factor(top, a.scale, &up, &bad);
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float y0 = bad ? 0.0f : x[2 * i] * up, y1 = bad ? 0.0f : x[2 * i + 1] * up;
+        const __half2 h2 = __floats2half2_rn(y0, y1);
+        const float2 b2 = __half22float2(h2);
+        hi[i] = bits(h2), lo[i] = bits(__floats2half2_rn(y0 - b2.x, y1 - b2.y));
     }
+    unsigned char* to = out + ((((int64_t)h * units + u) * 4 + part) * 32 + r) * RS;
+    *reinterpret_cast<uint4*>(to + d * 2) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    if (sizeof(T) == 4) *reinterpret_cast<uint4*>(to + HD * 2 + d * 2) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    if (d == 0) *reinterpret_cast<float*>(to + HD * (int)sizeof(T)) = factor;
 }
 
 // HD: padded head size. Queries enter as hi + lo for fp32 (Q2), the weights
@@ -334,7 +338,7 @@ __global__ void __launch_bounds__(kQueryWarps * 32) kvb_rows_queries(const KvbAt
 template <int HD, typename T>
 __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
     kvb_rows_kernel(const KvbAttnArgs a, const RowsPlan plan, const unsigned char* queries, int units, float* parts,
-                    float2* stats) {
+                    float* accs, float2* stats) {
     using C = RowsCfg<HD>;
     constexpr int BN = C::BN, NG = BN / 16;
     constexpr int RAWS = C::stage(sizeof(T));
@@ -399,22 +403,22 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                     wait(&k_full[kb], (tl / C::NBUF) & 1);
                     tc_fence_after();
                     const uint32_t d = tmem + (tl & 1) * BN;
+                    // the lo halves first: every product rounds the running sum towards
+                    // zero, and theirs is small
 #pragma unroll
-                    for (int s = 0; s < C::SLABS; ++s) {
-                        const uint64_t db = smem_desc(sk + kb * C::TILE + s * C::SLAB);
-                        const uint32_t at = tmem + kQ + s * 32;
-                        const uint64_t da = smem_desc(sq + s * C::QSLAB), dl = smem_desc(sq + (C::SLABS + s) * C::QSLAB);
+                    for (int part = Q2 ? 1 : 0; part >= 0; --part)
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk) {
-                            if constexpr (C::QT) {
-                                mma_f16_ts(d, at + 8 * kk, db + 2 * kk, id_s, s > 0 || kk > 0, lead);
-                                if (Q2) mma_f16_ts(d, at + 64 + 8 * kk, db + 2 * kk, id_s, 1u, lead);
-                            } else {
-                                mma_f16_ss(d, da + 2 * kk, db + 2 * kk, id_s, s > 0 || kk > 0, lead);
-                                if (Q2) mma_f16_ss(d, dl + 2 * kk, db + 2 * kk, id_s, 1u, lead);
+                        for (int s = 0; s < C::SLABS; ++s) {
+                            const uint64_t db = smem_desc(sk + kb * C::TILE + s * C::SLAB);
+                            const uint64_t da = smem_desc(sq + (part * C::SLABS + s) * C::QSLAB);
+                            const uint32_t at = tmem + kQ + part * 64 + s * 32;
+#pragma unroll
+                            for (int kk = 0; kk < 4; ++kk) {
+                                const bool more = part != (Q2 ? 1 : 0) || s > 0 || kk > 0;
+                                if constexpr (C::QT) mma_f16_ts(d, at + 8 * kk, db + 2 * kk, id_s, more, lead);
+                                else mma_f16_ss(d, da + 2 * kk, db + 2 * kk, id_s, more, lead);
                             }
                         }
-                    }
                     mma_commit(&s_full[tl & 1], lead);
                     mma_commit(&k_free[kb], lead);
                     if (jj == seg.n - 1) mma_commit(&q_free, lead);
@@ -431,7 +435,7 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
 #pragma unroll
                     for (int s = 0; s < BN / 16; ++s) {                  // 16 tokens: 8 columns hi, 8 lo
                         const uint32_t at = ap + 16 * s;
-                        mma_f16_ts(d, at, db + 128 * s, id_o, jj > 0 || s > 0, lead);
+                        mma_f16_ts(d, at, db + 128 * s, id_o, jj % kFold<T> > 0 || s > 0, lead);
                         mma_f16_ts(d, at + 8, db + 128 * s, id_o, 1u, lead);
                     }
                     mma_commit(&v_free[vb], lead);
@@ -594,6 +598,8 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
             const int lim = seg.p + (live ? f : seg.rows - 1) / G;       // the last token that the row sees
             const int all_see = seg.p + seg.m * kRows / G;               // ... that every row sees
             float m = -INFINITY, l = 0.0f, lr = -200.0f;                 // lr: log2 of the V scale reference
+            float acc_f = 1.0f;                  // rescaling of the moved-out accumulator since it was moved
+            float4* acc = reinterpret_cast<float4*>(accs + (int64_t)blockIdx.x * C::ACC) + w * (HD / 8) * kRows + row;
             // scales of a tile's 16-token groups, loaded a tile ahead: lanes 0-15
             // K's, lanes 16-31 log2 of V's
             const float* sc = (lane < 16 ? a.c.ks : a.c.vs) + seg.slot * a.c.scale_stride +
@@ -700,10 +706,32 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                             tmem_st16(to + c * 16, v);
                         }
                     }
-                    l *= el, m = xm, lr = xr;
+                    l *= el, acc_f *= eo, m = xm, lr = xr;
                 }
                 if (cut) weights(std::true_type{}, seen);
                 else weights(std::false_type{}, 0);
+                if (jj % kFold<T> == 0 && jj > 0) { // the last tiles' outputs move out
+                    wait(&v_free[(tl - 1) % C::NBUF], ((tl - 1) / C::NBUF) & 1);
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < HD / 2; c += 16) {
+                        int o[16];
+                        float4 y[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            y[i] = jj == kFold<T> ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : acc[(c / 4 + i) * kRows];
+                        tmem_ld16(tmem + lanes + kO + w * (HD / 2) + c, o);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            y[i].x = fmaf(y[i].x, acc_f, __int_as_float(o[4 * i]));
+                            y[i].y = fmaf(y[i].y, acc_f, __int_as_float(o[4 * i + 1]));
+                            y[i].z = fmaf(y[i].z, acc_f, __int_as_float(o[4 * i + 2]));
+                            y[i].w = fmaf(y[i].w, acc_f, __int_as_float(o[4 * i + 3]));
+                            acc[(c / 4 + i) * kRows] = y[i];
+                        }
+                    }
+                    acc_f = 1.0f;
+                }
                 tmem_st_wait();
                 tc_fence_before();
                 mbar_arrive(&p_full[tl & 1]);
@@ -725,11 +753,21 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                 tmem_ld16(tmem + lanes + kO + c, o);
                 float y[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) y[i] = __int_as_float(o[i]) * fo;
+                for (int i = 0; i < 16; ++i) y[i] = __int_as_float(o[i]);
+                if (seg.n > kFold<T>) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 x = acc[((c - w * (HD / 2)) / 4 + i) * kRows];
+                        y[4 * i] = fmaf(x.x, acc_f, y[4 * i]), y[4 * i + 1] = fmaf(x.y, acc_f, y[4 * i + 1]);
+                        y[4 * i + 2] = fmaf(x.z, acc_f, y[4 * i + 2]), y[4 * i + 3] = fmaf(x.w, acc_f, y[4 * i + 3]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) y[i] *= fo;
                 if (!whole) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        *reinterpret_cast<float4*>(pt + row * HD + c + 4 * i) =
+                        reinterpret_cast<float4*>(pt)[(c / 4 + i) * kRows + row] =
                             make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
                 } else if (live && c < hd) {
                     T* to = static_cast<T*>(a.out) + orow * hd + c;
@@ -762,8 +800,10 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
     }
 }
 
-// Joins the units that shares cut: CTA c those whose first cut lies at the
-// begin of share c. Also the rows without tokens: zeros.
+// Joins the units that shares cut: CTA (c, y) 16 rows of the unit whose first
+// cut lies at the begin of share c (one CTA a unit took 57 us for 32 units in
+// five parts each). Also the rows without tokens: zeros.
+constexpr int kJoinRows = 16;
 template <int HD>
 __global__ void __launch_bounds__(kFinishThreads) kvb_rows_finish(const KvbAttnArgs a, const RowsPlan plan,
                                                                 const float* parts, float2* stats, int grid) {
@@ -771,7 +811,7 @@ __global__ void __launch_bounds__(kFinishThreads) kvb_rows_finish(const KvbAttnA
     pdl_wait();
     pdl_trigger();
     const int tid = threadIdx.x, hd = a.c.hd, G = a.heads / a.c.heads;
-    for (int b = blockIdx.x; b < a.c.slots; b += gridDim.x) {
+    for (int b = blockIdx.x * gridDim.y + blockIdx.y; b < a.c.slots; b += gridDim.x * gridDim.y) {
         const KvbSpan s = kvb_span(a.r, b);
         const int live = live_rows(s, a.c.cap);
         if (s.p >= 0 && live < s.n && tid == 0) atomicOr(&g_kvb_rows_errors, kKvbErrCapacity);
@@ -794,36 +834,48 @@ __global__ void __launch_bounds__(kFinishThreads) kvb_rows_finish(const KvbAttnA
         e = h2;
     }
     const int c0 = blockIdx.x - 1;
-    __shared__ float s_m[kRows], s_i[kRows];
+    const int r0 = blockIdx.y * kJoinRows;
+    __shared__ float s_m[kJoinRows], s_i[kJoinRows], s_o[kJoinRows][HD + 1];
     auto at = [&](int c) { return parts + ((int64_t)c * 2 + (c == c0)) * C::PART; };
-    if (tid < kRows) {
+    {
+        static_assert(kFinishThreads == 16 * kJoinRows, "16 threads a row");
+        const int row = r0 + tid / 16;           // 16 threads share a row's parts
         float m = -INFINITY, l = 0.0f;
-        for (int c = c0; c <= last; ++c) m = fmaxf(m, at(c)[kRows * HD + tid]);
-        for (int c = c0; c <= last; ++c) {
-            const float mc = at(c)[kRows * HD + tid];
-            if (mc != -INFINITY) l = fmaf(at(c)[kRows * (HD + 1) + tid], ex2(mc - m), l);
+        for (int c = c0 + tid % 16; c <= last; c += 16) m = fmaxf(m, at(c)[kRows * HD + row]);
+#pragma unroll
+        for (int d = 8; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+        for (int c = c0 + tid % 16; c <= last; c += 16) {
+            const float mc = at(c)[kRows * HD + row];
+            if (mc != -INFINITY) l = fmaf(at(c)[kRows * (HD + 1) + row], ex2(mc - m), l);
         }
-        s_m[tid] = m, s_i[tid] = 1.0f / l;
-        const int f = s.m * kRows + tid;
-        if (stats && f < s.rows)
-            stats[(int64_t)(s.r0 + f / G) * a.heads + s.h * G + f % G] = make_float2(m, 1.0f / l);
+#pragma unroll
+        for (int d = 8; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+        if (tid % 16 == 0) {
+            s_m[tid / 16] = m, s_i[tid / 16] = 1.0f / l;
+            const int f = s.m * kRows + row;
+            if (stats && f < s.rows)
+                stats[(int64_t)(s.r0 + f / G) * a.heads + s.h * G + f % G] = make_float2(m, 1.0f / l);
+        }
     }
     __syncthreads();
-    for (int i = tid; i < kRows * HD / 4; i += kFinishThreads) {
-        const int row = i / (HD / 4), d = i % (HD / 4) * 4, f = s.m * kRows + row;
-        if (f >= s.rows || d >= hd) continue;
-        const float m = s_m[row], inv = s_i[row];
+    for (int i = tid; i < kJoinRows * HD / 4; i += kFinishThreads) {
+        const int r = i % kJoinRows, row = r0 + r, d4 = i / kJoinRows;
+        const float m = s_m[r], inv = s_i[r];
         float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
         for (int c = c0; c <= last; ++c) {
-            const float mc = at(c)[kRows * HD + row];
-            if (mc == -INFINITY) continue;
-            const float e = ex2(mc - m);
-            const float4 x = *reinterpret_cast<const float4*>(at(c) + row * HD + d);
+            const float mc = at(c)[kRows * HD + row], e = mc == -INFINITY ? 0.0f : ex2(mc - m);
+            const float4 x = reinterpret_cast<const float4*>(at(c))[d4 * kRows + row];
             y.x = fmaf(x.x, e, y.x), y.y = fmaf(x.y, e, y.y), y.z = fmaf(x.z, e, y.z), y.w = fmaf(x.w, e, y.w);
         }
-        const int64_t o = ((int64_t)(s.r0 + f / G) * a.heads + s.h * G + f % G) * hd + d;
-        store1(a.out, a.type, o, y.x * inv), store1(a.out, a.type, o + 1, y.y * inv);
-        store1(a.out, a.type, o + 2, y.z * inv), store1(a.out, a.type, o + 3, y.w * inv);
+        float* o = &s_o[r][4 * d4];
+        o[0] = y.x * inv, o[1] = y.y * inv, o[2] = y.z * inv, o[3] = y.w * inv;
+    }
+    __syncthreads();
+    for (int i = tid; i < kJoinRows * HD; i += kFinishThreads) {
+        const int r = i / HD, d = i % HD, f = s.m * kRows + r0 + r;
+        if (f < s.rows && d < hd)
+            store1(a.out, a.type, ((int64_t)(s.r0 + f / G) * a.heads + s.h * G + f % G) * hd + d, s_o[r][d]);
     }
 }
 
@@ -1014,13 +1066,14 @@ int rows_hd(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 size_t up16(size_t x) { return (x + 15) & ~(size_t)15; }
 
 struct RowsLayout {                              // byte offsets in the scratch
-    size_t unit, first, parts, stats, queries, total;
+    size_t unit, first, parts, accs, stats, queries, total;
     RowsLayout(const KvbCache& c, int heads, int rows, bool mass, int qbytes) {
         const int hd = rows_hd(c.hd);
         unit = 16;
         first = unit + (size_t)max_units(c, heads, rows) * sizeof(RowsUnit);
         parts = up16(first + ((size_t)c.slots + 1) * sizeof(int));
-        stats = parts + (size_t)kSms * 2 * kRows * (hd + 2) * sizeof(float);
+        accs = parts + (size_t)kSms * 2 * kRows * (hd + 2) * sizeof(float);
+        stats = accs + (size_t)kSms * kRows * hd * sizeof(float);
         queries = up16(stats + (mass ? (size_t)rows * heads * sizeof(float2) : 0));
         total = queries + (hd <= 128 || mass ? (size_t)max_units(c, heads, rows) * c.heads * kRows * (hd * qbytes + 16) : 0);
     }
@@ -1042,7 +1095,7 @@ cudaError_t rows_launch(const KvbAttnArgs& a, cudaStream_t st) {
         const auto prep = a.type == KVB_F32    ? kvb_rows_queries<HD, float>
                           : a.type == KVB_BF16 ? kvb_rows_queries<HD, __nv_bfloat16>
                                                : kvb_rows_queries<HD, __half>;
-        e = launch_k(prep, dim3(units * 4, a.c.heads), dim3(kQueryWarps * 32), 0, st, a, plan, queries, units);
+        e = launch_k(prep, dim3(units * 4, a.c.heads), dim3(HD / 8 * 32), 0, st, a, plan, queries, units);
         if (e != cudaSuccess) return e;
     }
     const auto kern = a.type == KVB_F32    ? kvb_rows_kernel<HD, float>
@@ -1051,9 +1104,10 @@ cudaError_t rows_launch(const KvbAttnArgs& a, cudaStream_t st) {
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::smem(qbytes));
     if (e != cudaSuccess) return e;
     e = launch_k(kern, dim3(kSms), dim3(C::THREADS), C::smem(qbytes), st, a, plan,
-                 (const unsigned char*)queries, units, parts, stats);
+                 (const unsigned char*)queries, units, parts,
+                 reinterpret_cast<float*>(s + L.accs), stats);
     if (e != cudaSuccess) return e;
-    e = launch_k(kvb_rows_finish<HD>, dim3(kSms), dim3(kFinishThreads), 0, st, a, plan, (const float*)parts, stats, kSms);
+    e = launch_k(kvb_rows_finish<HD>, dim3(kSms, kRows / kJoinRows), dim3(kFinishThreads), 0, st, a, plan, (const float*)parts, stats, kSms);
     if (e != cudaSuccess || !stats) return e;
     return qbytes == 4 ? mass_launch<HD, true>(a, plan, queries, units, stats, st)
                        : mass_launch<HD, false>(a, plan, queries, units, stats, st);

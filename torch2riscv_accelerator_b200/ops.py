@@ -7,6 +7,7 @@ runs on the current torch CUDA stream and raises W8A8Error on a nonzero status.
 Tensors are passed as raw device pointers; torch only owns the memory.
 """
 import ctypes
+import functools
 from typing import NamedTuple
 
 import numpy as np
@@ -426,43 +427,48 @@ def kvb_cache(slots, kv_heads, capacity, head_dim, block=64, device="cuda"):
     return KvBlocks(codes(), scales(), codes(), scales())
 
 
+@functools.lru_cache(maxsize=256)
+def _kvb_layout(k, k_st, ks, ks_st, v, v_st, vs, vs_st, name):
+    """What a cache's shapes and strides say: slots, heads, capacity, head_dim,
+    block, slot strides (a refused one raises)."""
+    if len(k) != 4 or v != k or len(ks) != 3 or ks[:2] != k[:2] or vs != ks or ks[2] == 0 or k[2] % ks[2]:
+        raise ValueError(f"{name}: codes {tuple(k)} / {tuple(v)} and scales {tuple(ks)} / {tuple(vs)} do not belong "
+                         "together")
+    S, H, T, D = k
+    NB = ks[2]
+    if k_st[1:] != (T * D, D, 1) or v_st[1:] != k_st[1:] or ks_st[1:] != (NB, 1) or vs_st[1:] != ks_st[1:] or \
+            (S > 1 and (v_st != k_st or vs_st != ks_st)):
+        raise ValueError(f"{name}: each slot's codes and scales must be contiguous, K's and V's alike")
+    return S, H, T, D, T // NB, k_st[0], ks_st[0]
+
+
 def _kvb(cache, name="cache"):
-    """The checked W8A8KvBlocks of a cache."""
+    """The checked W8A8KvBlocks of a cache, and its device."""
     k, ks, v, vs = cache
-    S, H, T, D = k.shape
-    NB = ks.shape[2] if ks.dim() == 3 else 0
-    st, sc = k.stride(), ks.stride()
     if k.dtype != I8 or v.dtype != I8 or ks.dtype != F32 or vs.dtype != F32:
         raise ValueError(f"{name}: int8 codes and fp32 scales are required")
-    if v.shape != k.shape or ks.shape != (S, H, NB) or vs.shape != ks.shape or NB == 0 or T % NB:
-        raise ValueError(f"{name}: codes {tuple(k.shape)} / {tuple(v.shape)} and scales {tuple(ks.shape)} / "
-                         f"{tuple(vs.shape)} do not belong together")
-    if st[1:] != (T * D, D, 1) or sc[1:] != (NB, 1) or (S > 1 and (v.stride() != st or vs.stride() != sc)) or \
-            v.stride()[1:] != st[1:] or vs.stride()[1:] != sc[1:]:
-        raise ValueError(f"{name}: each slot's codes and scales must be contiguous, K's and V's alike")
+    layout = _kvb_layout(k.shape, k.stride(), ks.shape, ks.stride(), v.shape, v.stride(), vs.shape, vs.stride(), name)
     dev = k.device
-    if dev.type != "cuda" or v.device != dev or ks.device != dev or vs.device != dev:
+    if not k.is_cuda or v.device != dev or ks.device != dev or vs.device != dev:
         raise ValueError(f"{name}: CUDA tensors on one device are required")
-    return _lib.W8A8KvBlocks(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), S, H, T, D, T // NB, st[0],
-                             sc[0])
+    return _lib.W8A8KvBlocks(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), *layout), dev
 
 
 def _kvb_index(t, n, dev, name):
-    if t.dtype != I32 or t.dim() != 1 or t.shape[0] != n or t.device != dev or (n > 1 and t.stride(0) != 1):
+    if t.dtype != I32 or t.shape != (n,) or t.device != dev or (n > 1 and t.stride(0) != 1):
         raise ValueError(f"{name}: a contiguous int32 [{n}] tensor on {dev} is required")
 
 
 def _kvb_rows(t, heads, hd, dev, name):
     """(dtype code, elements between rows) of rows [rows, heads, hd] whose rows
     are contiguous (a slice of a wider row is fine)."""
-    code = _KVB_TYPES.get(t.dtype)
-    if code is None or t.dim() != 3 or t.device != dev:
-        raise ValueError(f"{name}: fp32, bf16 or fp16 [rows, {heads}, {hd}] on {dev} is required")
-    st = t.stride()
-    if t.shape[2] != hd or (heads and t.shape[1] != heads) or st[2] != 1 or (t.shape[1] > 1 and st[1] != hd):
-        raise ValueError(f"{name}: [rows, {heads}, {hd}] with contiguous rows is required, got {tuple(t.shape)} "
+    code, sh, st = _KVB_TYPES.get(t.dtype), t.shape, t.stride()
+    if code is None or len(sh) != 3 or t.device != dev:
+        raise ValueError(f"{name}: fp32, bf16 or fp16 [rows, {heads or 'heads'}, {hd}] on {dev} is required")
+    if sh[2] != hd or (heads and sh[1] != heads) or st[2] != 1 or (sh[1] > 1 and st[1] != hd):
+        raise ValueError(f"{name}: [rows, {heads or 'heads'}, {hd}] with contiguous rows is required, got {tuple(sh)} "
                          f"with strides {st}")
-    return code, st[0] if t.shape[0] > 1 else t.shape[1] * hd
+    return code, st[0] if sh[0] > 1 else sh[1] * hd
 
 
 def _kvb_mass(t, k, name="mass"):
@@ -487,8 +493,7 @@ def kvb_append(k, v, cache, pos, start=None):
     start[b] .. start[b + 1] - 1 (start None: row b) at positions pos[b] on
     (negative: an idle slot). A block's scale grows with its largest value; its
     older codes are rescaled with it."""
-    c = _kvb(cache)
-    dev = cache[0].device
+    c, dev = _kvb(cache)
     dt, ks = _kvb_rows(k, c.kv_heads, c.head_dim, dev, "k")
     dv, vs = _kvb_rows(v, c.kv_heads, c.head_dim, dev, "v")
     if dt != dv or k.shape[0] != v.shape[0]:
@@ -503,8 +508,7 @@ def kvb_append(k, v, cache, pos, start=None):
 def kvb_read(cache, pos, start, rows, dtype=F32, k=None, v=None):
     """The values held at the rows' positions: k, v [rows, kv_heads, head_dim]
     (zeros for idle slots; rows behind the last sequence are left alone)."""
-    c = _kvb(cache)
-    dev = cache[0].device
+    c, dev = _kvb(cache)
     _kvb_index(pos, c.slots, dev, "pos")
     if start is not None:
         _kvb_index(start, c.slots + 1, dev, "start")
@@ -520,17 +524,24 @@ def kvb_read(cache, pos, start, rows, dtype=F32, k=None, v=None):
     return k, v
 
 
+@functools.lru_cache(maxsize=256)
+def _kvb_scratch_bytes(layout, heads, rows, one_row, mass, dtype):
+    # sizes alone decide; the pointers are never followed
+    c = _lib.W8A8KvBlocks(256, 256, 256, 256, *layout)
+    return _lib.load().w8a8_kvb_attn_scratch_bytes(ctypes.byref(c), heads, rows, one_row, mass, dtype)
+
+
 def kvb_attn_scratch(cache, heads, rows, start=True, mass=False, dtype=F32):
     """Scratch for kvb_attn (start False) or kvb_attn_rows (True) calls of at
     most `rows` rows; one per call that may overlap another."""
-    n = _lib.load().w8a8_kvb_attn_scratch_bytes(ctypes.byref(_kvb(cache)), heads, rows, int(not start), int(mass),
+    c, dev = _kvb(cache)
+    n = _lib.load().w8a8_kvb_attn_scratch_bytes(ctypes.byref(c), heads, rows, int(not start), int(mass),
                                                 _KVB_TYPES[dtype])
-    return torch.empty(n, dtype=torch.uint8, device=cache[0].device)
+    return torch.empty(n, dtype=torch.uint8, device=dev)
 
 
 def _kvb_attn(q, cache, pos, start, scale, mass, out, scratch):
-    c = _kvb(cache)
-    dev = cache[0].device
+    c, dev = _kvb(cache)
     dt, qs = _kvb_rows(q, 0, c.head_dim, dev, "q")
     rows, heads, hd = q.shape
     _kvb_index(pos, c.slots, dev, "pos")
@@ -539,19 +550,18 @@ def _kvb_attn(q, cache, pos, start, scale, mass, out, scratch):
     if mass is not None:
         _kvb_mass(mass, cache[0])
     if out is None:
-        out = torch.empty((rows, heads, hd), dtype=q.dtype, device=dev)
+        out = q.new_empty(q.shape)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev:
         raise ValueError(f"out: a contiguous {q.dtype} {tuple(q.shape)} tensor is required")
     if scratch is None:
-        n = _lib.load().w8a8_kvb_attn_scratch_bytes(ctypes.byref(c), heads, rows, int(start is None),
-                                                    int(mass is not None), dt)
-        scratch = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        scratch = torch.empty(_kvb_scratch_bytes((c.slots, c.kv_heads, c.capacity, c.head_dim, c.block, c.slot_stride,
+                                                  c.scale_stride), heads, rows, int(start is None),
+                                                 int(mass is not None), dt), dtype=torch.uint8, device=dev)
     elif scratch.device != dev:
         raise ValueError(f"scratch: a tensor on {dev} is required")
     _kvb_call("w8a8_kvb_attn", dev, ctypes.byref(c), q.data_ptr(), qs, dt, heads, rows, pos.data_ptr(),
               None if start is None else start.data_ptr(), hd ** -0.5 if scale is None else scale, out.data_ptr(),
-              None if mass is None else mass.data_ptr(), None if scratch is None else scratch.data_ptr(),
-              0 if scratch is None else scratch.numel())
+              None if mass is None else mass.data_ptr(), scratch.data_ptr(), scratch.numel())
     return out
 
 
@@ -581,17 +591,16 @@ def kvb_evict(cache, mass, count, keep, sink=0, recent=0, dst=None, dst_mass=Non
     those between, moved together in their order; in place, or into dst /
     dst_mass. Returns (kept [slots, kv_heads, keep] int32: each place's former
     position, -1 past the new length; the new lengths [slots] int32)."""
-    c = _kvb(cache)
-    dev = cache[0].device
+    c, dev = _kvb(cache)
     _kvb_mass(mass, cache[0])
     _kvb_index(count, c.slots, dev, "count")
     d = None
     if dst is not None:
-        d = _kvb(dst, "dst")
+        d, ddev = _kvb(dst, "dst")
         if dst_mass is None:
             raise ValueError("dst_mass: required with dst")
         _kvb_mass(dst_mass, dst[0], "dst_mass")
-        if dst[0].device != dev:
+        if ddev != dev:
             raise ValueError(f"dst: a cache on {dev} is required")
     elif dst_mass is not None:
         raise ValueError("dst_mass: only with dst")
