@@ -19,17 +19,17 @@ namespace {
 constexpr float kInv127 = (float)(1.0 / 127.0);
 
 // ------------------------------------------------------------------ append
-// One CTA per (touched block, KV head, K or V). A block's scale is
+// One CTA per (touched block, KV head). A block's scale is
 //   s' = max(s, max|new rows| * F(1/127))   (s = 0 for a block without older tokens)
 // the new codes are rint(x / s') and, where s' grew, the older codes
 // rint((q * s) / s'): each step rounded once, so that the codes do not depend
 // on how the kernel is split. Values are first made finite (NaN 0, infinities
 // the largest finite value), so that one bad element does not void its block.
-constexpr int kAppThreads = 128;
+constexpr int kAppThreads = 256;                 // half of them for K, half for V
 
-__device__ __forceinline__ int touched_blocks(const KvbSpan& s, int cap, int block) {
+__device__ __forceinline__ int touched_blocks(const KvbSpan& s, int cap, int sh) {
     const int n = s.p < 0 ? 0 : min(s.n, cap - s.p);
-    return n > 0 ? (s.p + n - 1) / block - s.p / block + 1 : 0;
+    return n > 0 ? ((s.p + n - 1) >> sh) - (s.p >> sh) + 1 : 0;
 }
 
 __device__ __forceinline__ float finite_of(float x) {
@@ -41,98 +41,100 @@ template <typename T>
 __global__ void __launch_bounds__(kAppThreads) kvb_append_kernel(const KvbAppendArgs a) {
     pdl_wait();
     pdl_trigger();
+    constexpr int H = kAppThreads / 2;
     __shared__ int s_slot, s_index;
     __shared__ unsigned int s_max[kAppThreads / 32];
-    const int tid = threadIdx.x, lane = tid & 31, S = a.c.slots, B = a.c.block;
+    const int tid = threadIdx.x, lane = tid & 31, S = a.c.slots, B = a.c.block, sh = 31 - __clz(B);
     if (tid < 32) {                              // work item blockIdx.x: the slots' touched blocks counted through
-        const int per = (S + 31) / 32, b0 = lane * per, b1 = min(b0 + per, S);
-        int mine = 0;
-        for (int b = b0; b < b1; ++b) mine += touched_blocks(kvb_span(a.r, b), a.c.cap, B);
-        int upto = mine;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int o = __shfl_up_sync(0xffffffffu, upto, d);
-            if (lane >= d) upto += o;
-        }
-        int left = (int)blockIdx.x - (upto - mine);
         if (lane == 0) s_slot = -1;
         __syncwarp();
-        if (left >= 0 && left < mine) {
-            for (int b = b0; b < b1; ++b) {
-                const int n = touched_blocks(kvb_span(a.r, b), a.c.cap, B);
-                if (left < n) {
-                    s_slot = b, s_index = left;
-                    break;
+        int before = 0;
+        bool over = false;
+        for (int b0 = 0; b0 < S; b0 += 128) {    // four slots a lane in flight
+            int n[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int b = b0 + 32 * i + lane;
+                n[i] = 0;
+                if (b < S) {
+                    const KvbSpan s = kvb_span(a.r, b);
+                    n[i] = touched_blocks(s, a.c.cap, sh);
+                    over |= s.p >= 0 && s.n > 0 && s.n > a.c.cap - s.p;
                 }
-                left -= n;
             }
-        }
-        if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0) {
-            bool over = false;
-            for (int b = b0; b < b1; ++b) {
-                const KvbSpan s = kvb_span(a.r, b);
-                over |= s.p >= 0 && s.n > 0 && s.n > a.c.cap - s.p;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                int upto = n[i];
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int o = __shfl_up_sync(0xffffffffu, upto, d);
+                    if (lane >= d) upto += o;
+                }
+                const int at = (int)blockIdx.x - before - (upto - n[i]);
+                if (at >= 0 && at < n[i]) s_slot = b0 + 32 * i + lane, s_index = at;
+                before += __shfl_sync(0xffffffffu, upto, 31);
             }
-            if (over) atomicOr(&g_kvb_errors, kKvbErrCapacity);
+            if (before > (int)blockIdx.x && blockIdx.x + blockIdx.y > 0) break;
         }
+        if (over && blockIdx.x == 0 && blockIdx.y == 0) atomicOr(&g_kvb_errors, kKvbErrCapacity);
     }
     __syncthreads();
     const int b = s_slot;
     if (b < 0) return;
     const KvbSpan sp = kvb_span(a.r, b);
-    const int n = min(sp.n, a.c.cap - sp.p), hd = a.c.hd, h = blockIdx.y;
-    const int blk = sp.p / B + s_index, t0 = max(blk * B, sp.p), t1 = min((blk + 1) * B, sp.p + n);
-    const bool is_v = blockIdx.z != 0;
+    const int n = min(sp.n, a.c.cap - sp.p), hd = a.c.hd, h = blockIdx.y, ht = tid % H;
+    const int blk = (sp.p >> sh) + s_index, t0 = max(blk * B, sp.p), t1 = min((blk + 1) * B, sp.p + n);
+    const bool is_v = tid >= H;
     const int64_t stride = is_v ? a.v_stride : a.k_stride;
     const T* x = static_cast<const T*>(is_v ? a.v : a.k) + (int64_t)(sp.r0 + t0 - sp.p) * stride + h * hd;
     int8_t* codes = (is_v ? a.c.v : a.c.k) + b * a.c.slot_stride + (int64_t)h * a.c.cap * hd;
-    float* scale = (is_v ? a.c.vs : a.c.ks) + b * a.c.scale_stride + (int64_t)h * (a.c.cap / B) + blk;
+    float* scale = (is_v ? a.c.vs : a.c.ks) + b * a.c.scale_stride + (int64_t)h * (a.c.cap >> sh) + blk;
+    const bool older = t0 > blk * B;
+    const float s_old = older ? *scale : 0.0f;
 
-    const int nv = hd / 8, items = (t1 - t0) * nv;
+    // the thread's vectors of 8: number ht, ht + H, ... of the rows' hd / 8 each
+    const int nv = hd / 8, items = (t1 - t0) * nv, step_r = H / nv, step_v = H % nv;
     unsigned int m = 0;                          // max|x| as bits: non-negative floats order as integers
-    for (int i = tid; i < items; i += kAppThreads) {
+    int row = ht / nv, v = ht % nv;
+    for (int i = ht; i < items; i += H) {
         float y[8];
-        kvb_load8<T>(x + (i / nv) * stride + (i % nv) * 8, y);
+        kvb_load8<T>(x + row * stride + v * 8, y);
 #pragma unroll
         for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(fabsf(finite_of(y[j]))));
+        row += step_r, v += step_v;
+        if (v >= nv) v -= nv, ++row;
     }
     m = __reduce_max_sync(0xffffffffu, m);
     if (lane == 0) s_max[tid / 32] = m;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kAppThreads / 32; ++w) m = max(m, s_max[w]);
-    const bool older = t0 > blk * B;
-    const float s_old = older ? *scale : 0.0f;
+    for (int w = 0; w < H / 32; ++w) m = max(m, s_max[(is_v ? H / 32 : 0) + w]);
     const float s_new = fmaxf(s_old, __fmul_rn(__uint_as_float(m), kInv127));
     const float rcp = 1.0f / s_new;
     if (older && s_new != s_old) {
         const int olds = (t0 - blk * B) * (hd / 16);
         uint4* q = reinterpret_cast<uint4*>(codes + (int64_t)blk * B * hd);
-        for (int i = tid; i < olds; i += kAppThreads) {
-            uint4 w = q[i];
-            int8_t* c = reinterpret_cast<int8_t*>(&w);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) c[j] = (int8_t)kvb_code(__fmul_rn((float)c[j], s_old), s_new, rcp);
-            q[i] = w;
-        }
+        for (int i = ht; i < olds; i += H) q[i] = kvb_requant16(q[i], s_old, s_new, rcp);
     }
-    for (int i = tid; i < items; i += kAppThreads) {
-        const int row = i / nv, d = (i % nv) * 8;
+    row = ht / nv, v = ht % nv;
+    for (int i = ht; i < items; i += H) {
         float y[8];
-        kvb_load8<T>(x + row * stride + d, y);
-        uint2 w;
-        int8_t* c = reinterpret_cast<int8_t*>(&w);
+        kvb_load8<T>(x + row * stride + v * 8, y);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) c[j] = s_new > 0.0f ? (int8_t)kvb_code(finite_of(y[j]), s_new, rcp) : (int8_t)0;
-        *reinterpret_cast<uint2*>(codes + (int64_t)(t0 + row) * hd + d) = w;
+        for (int j = 0; j < 8; ++j) y[j] = finite_of(y[j]);
+        uint32_t w[2] = {0u, 0u};
+        if (s_new > 0.0f) kvb_codes<8>(y, s_new, rcp, w);
+        *reinterpret_cast<uint2*>(codes + (int64_t)(t0 + row) * hd + v * 8) = make_uint2(w[0], w[1]);
+        row += step_r, v += step_v;
+        if (v >= nv) v -= nv, ++row;
     }
     __syncthreads();                             // every thread has read the old scale
-    if (tid == 0) *scale = s_new;
+    if (ht == 0) *scale = s_new;
 }
 
 // -------------------------------------------------------------------- read
-// One warp per row: 4 codes per lane, one full 128-byte (16-bit: 64-byte) run
-// of values per store.
+// A warp per row, 4 codes a lane: one full 512-byte (16-bit: 256-byte) run of
+// values per store. Bound by the values' stores.
 constexpr int kReadWarps = 8;
 
 template <typename T>
@@ -144,43 +146,49 @@ __global__ void __launch_bounds__(kReadWarps * 32) kvb_read_kernel(const KvbRead
     const int b = kvb_slot_of(a.r, a.c.slots, r);
     if (b < 0) return;
     const KvbSpan sp = kvb_span(a.r, b);
-    const int hd = a.c.hd, n4 = hd / 4;
-    const bool idle = sp.p < 0, over = !idle && r - sp.r0 >= a.c.cap - sp.p;
-    const int t = idle || over ? 0 : sp.p + (r - sp.r0);
+    const int hd = a.c.hd, n4 = hd / 4, sh = 31 - __clz(a.c.block);
+    const bool idle = sp.p < 0, over = !idle && r - sp.r0 >= a.c.cap - sp.p, none = idle || over;
+    const int t = none ? 0 : sp.p + (r - sp.r0);
     if (over && lane == 0) atomicOr(&g_kvb_errors, kKvbErrCapacity);
-    T* out[2] = {static_cast<T*>(a.k), static_cast<T*>(a.v)};
+    const int64_t head = (int64_t)a.c.cap * hd, first = b * a.c.slot_stride + (int64_t)t * hd;
+    const int64_t shead = a.c.cap >> sh, sfirst = b * a.c.scale_stride + (t >> sh);
+    const int64_t to = (int64_t)r * a.c.heads * hd;
+    int h = lane / n4, d = lane % n4;
+    const int step_h = 32 / n4, step_d = 32 % n4;
+#pragma unroll 4
     for (int i = lane; i < a.c.heads * n4; i += 32) {
-        const int h = i / n4, d = (i % n4) * 4;
+        const int64_t at = first + h * head + d * 4, sat = sfirst + h * shead;
+        char4 q[2] = {make_char4(0, 0, 0, 0), make_char4(0, 0, 0, 0)};
+        float s[2] = {0.0f, 0.0f};
+        if (!none) {
+            q[0] = *reinterpret_cast<const char4*>(a.c.k + at), q[1] = *reinterpret_cast<const char4*>(a.c.v + at);
+            s[0] = a.c.ks[sat], s[1] = a.c.vs[sat];
+        }
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
-            char4 q = make_char4(0, 0, 0, 0);
-            float s = 0.0f;
-            if (!idle && !over) {
-                const int8_t* codes = (z ? a.c.v : a.c.k) + b * a.c.slot_stride;
-                q = *reinterpret_cast<const char4*>(codes + ((int64_t)h * a.c.cap + t) * hd + d);
-                s = (z ? a.c.vs : a.c.ks)[b * a.c.scale_stride + (int64_t)h * (a.c.cap / a.c.block) + t / a.c.block];
-            }
-            T y[4] = {kvb_t<T>(q.x * s), kvb_t<T>(q.y * s), kvb_t<T>(q.z * s), kvb_t<T>(q.w * s)};
-            T* p = out[z] + ((int64_t)r * a.c.heads + h) * hd + d;
+            T y[4] = {kvb_t<T>(q[z].x * s[z]), kvb_t<T>(q[z].y * s[z]), kvb_t<T>(q[z].z * s[z]), kvb_t<T>(q[z].w * s[z])};
+            T* p = static_cast<T*>(z ? a.v : a.k) + to + i * 4;
             if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(y);
             else *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(y);
         }
+        h += step_h, d += step_d;
+        if (d >= n4) d -= n4, ++h;
     }
 }
 
 // ------------------------------------------------------------------- evict
-// One thread-block cluster per (slot, KV head).
-//  1. Selection: the (keep - sink - recent)-th largest weight of the middle
-//     tokens by four 8-bit radix passes over order-preserving keys; the CTAs
-//     count their segments and add the histograms up through distributed
-//     shared memory (integers: the same in every order).
-//  2. The kept indices in order: a token stays if its key is above the
-//     threshold, or equal to it and among the first equal ones.
-//  3. Compaction in rounds of one unit of tokens per CTA. A kept token moves
-//     to a place at or before its own, so in place a round may be stored once
-//     every CTA of the cluster has read its sources: one cluster barrier per
-//     round. A block's new scale is its largest held value * F(1/127).
+// 1. Selection, one CTA per (slot, KV head): the (keep - sink - recent)-th largest
+//    weight of the middle tokens by four 8-bit radix passes over order-preserving
+//    keys (in shared memory up to 32,768 of them), then the kept indices in order:
+//    a token stays if its key is above the threshold, or equal to it and among the
+//    first equal ones.
+// 2. Compaction, 128 tokens a CTA: each block's new scale is its largest held
+//    value * F(1/127). A kept token moves to a place at or before its own, so in
+//    place the CTAs of a (slot, KV head) form one cluster and go in rounds: a round
+//    may be stored once every CTA has read its sources (one cluster barrier).
 namespace cg = cooperative_groups;
+constexpr int kSelThreads = 1024;
+constexpr int kSelKeys = 32768;                  // keys held in shared memory
 constexpr int kEvThreads = 512;
 constexpr int kEvUnit = 128;                     // tokens per CTA and round (a multiple of every block size)
 
@@ -189,150 +197,132 @@ __device__ __forceinline__ unsigned int weight_key(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// ITEMS: 16-code chunks per thread and round, 2 (K, V) * kEvUnit * hd / 16 / kEvThreads
-template <int ITEMS>
-__global__ void __launch_bounds__(kEvThreads) kvb_evict_kernel(const KvbEvictArgs a) {
+__device__ __forceinline__ int evict_count(const KvbEvictArgs& a, int b) { return max(min(a.count[b], a.src.cap), 0); }
+
+__global__ void __launch_bounds__(kSelThreads) kvb_select_kernel(const KvbEvictArgs a, int cached) {
     pdl_wait();
     pdl_trigger();
-    cg::cluster_group cl = cg::this_cluster();
-    const int CN = (int)cl.num_blocks(), rank = (int)cl.block_rank();
-    const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
-    __shared__ unsigned int hist[2][256];
-    __shared__ unsigned int s_prefix, s_left;
-    __shared__ int s_gt, s_eq;                   // this CTA's counts above / at the threshold
-    __shared__ int w_gt[kEvThreads / 32], w_eq[kEvThreads / 32];
-    __shared__ unsigned int s_amax[2][kEvUnit / 16];
-    const int keep = a.keep, cap = a.src.cap;
-    int n = a.count[b];
-    if (n > cap) {
-        if (tid == 0 && rank == 0 && h == 0) atomicOr(&g_kvb_errors, kKvbErrCapacity);
-        n = cap;
+    extern __shared__ unsigned int keys[];
+    __shared__ unsigned int hist[256], s_prefix, s_left;
+    __shared__ int w_gt[kSelThreads / 32], w_eq[kSelThreads / 32];
+    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid / 32, keep = a.keep;
+    const int n = evict_count(a, b), left = min(n, keep);
+    if (h == 0 && tid == 0) {
+        if (a.count[b] > a.src.cap) atomicOr(&g_kvb_errors, kKvbErrCapacity);
+        a.count_out[b] = left;
     }
-    n = max(n, 0);
     const int64_t head = (int64_t)b * a.src.heads + h;
-    const float* mass = a.mass + head * cap;
-    float* dmass = a.dst_mass + head * a.dst.cap;
+    const float* mass = a.mass + head * a.src.cap;
     int32_t* kept = a.kept + head * keep;
     const bool cut = n > keep;
-    const int left = min(n, keep);
-    if (rank == 0 && h == 0 && tid == 0) a.count_out[b] = left;
-    for (int i = rank * kEvThreads + tid; i < keep; i += CN * kEvThreads)
+    for (int i = tid; i < keep; i += kSelThreads)
         if (!cut) kept[i] = i < n ? i : -1;
         else if (i < a.sink) kept[i] = i;
         else if (i >= keep - a.recent) kept[i] = n - keep + i;
-    if (cut) {
-        const int mid = n - a.recent - a.sink, want = keep - a.sink - a.recent;
-        const int seg = (mid + CN - 1) / CN, lo = a.sink + min(rank * seg, mid), hi = a.sink + min((rank + 1) * seg, mid);
-        unsigned int prefix = 0, need = want;
-        if (want > 0) {
-            for (int pass = 0; pass < 4; ++pass) {
-                const int sh = 24 - 8 * pass;
-                unsigned int* hg = hist[pass & 1];
-                if (tid < 256) hg[tid] = 0;
-                __syncthreads();
-                for (int t = lo + tid; t < hi; t += kEvThreads) {
-                    const unsigned int k = weight_key(mass[t]);
-                    if (pass == 0 || (k >> (sh + 8)) == prefix) atomicAdd(&hg[(k >> sh) & 255u], 1u);
-                }
-                cl.sync();
-                if (warp == 0) {                 // digit 255 - 8 lane - j: from the largest down
-                    unsigned int c[8], sum = 0;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) c[j] = 0;
-                    for (int r = 0; r < CN; ++r) {
-                        const unsigned int* o = cl.map_shared_rank(hg, r);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) c[j] += o[255 - 8 * lane - j];
-                    }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) sum += c[j];
-                    unsigned int upto = sum;
-#pragma unroll
-                    for (int d = 1; d < 32; d <<= 1) {
-                        const unsigned int o = __shfl_up_sync(0xffffffffu, upto, d);
-                        if (lane >= d) upto += o;
-                    }
-                    unsigned int above = upto - sum;
-                    if (above < need && need <= upto) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            if (above < need && need <= above + c[j]) {
-                                s_prefix = (prefix << 8) | (255 - 8 * lane - j);
-                                s_left = need - above;
-                            }
-                            above += c[j];
-                        }
-                    }
-                }
-                __syncthreads();
-                prefix = s_prefix, need = s_left;
-                // the buffer of pass + 1 was last read remotely before this pass's barrier
-            }
-        }
-        // counts of this segment, then its place among the cluster's
-        int gt = 0, eq = 0;
-        if (want > 0)
-            for (int t = lo + tid; t < hi; t += kEvThreads) {
-                const unsigned int k = weight_key(mass[t]);
-                gt += k > prefix, eq += k == prefix;
-            }
-        gt = __reduce_add_sync(0xffffffffu, gt), eq = __reduce_add_sync(0xffffffffu, eq);
-        if (lane == 0) w_gt[warp] = gt, w_eq[warp] = eq;
+    const int mid = n - a.recent - a.sink, want = keep - a.sink - a.recent;
+    if (!cut || want == 0) return;
+    mass += a.sink;
+    const bool in_smem = mid <= cached;
+    if (in_smem)
+        for (int t = tid; t < mid; t += kSelThreads) keys[t] = weight_key(mass[t]);
+    auto key = [&](int t) { return in_smem ? keys[t] : weight_key(mass[t]); };
+    const int rounds = (mid + kSelThreads - 1) / kSelThreads;
+    unsigned int prefix = 0, need = want;
+    for (int pass = 0; pass < 4; ++pass) {
+        const int sh = 24 - 8 * pass;
+        if (tid < 256) hist[tid] = 0;
         __syncthreads();
-        if (tid == 0) {
-            int g = 0, e = 0;
-            for (int w = 0; w < kEvThreads / 32; ++w) g += w_gt[w], e += w_eq[w];
-            s_gt = g, s_eq = e;
+        for (int i = 0; i < rounds; ++i) {       // equal digits of a warp count once
+            const int t = i * kSelThreads + tid;
+            const unsigned int k = t < mid ? key(t) : 0u;
+            const bool in = t < mid && (pass == 0 || (k >> (sh + 8)) == prefix);
+            const unsigned int digit = in ? (k >> sh) & 255u : 256u, same = __match_any_sync(0xffffffffu, digit);
+            if (in && lane == __ffs(same) - 1) atomicAdd(&hist[digit], (unsigned int)__popc(same));
         }
-        cl.sync();
-        int gt0 = 0, eq0 = 0;
-        for (int r = 0; r < rank; ++r) gt0 += *cl.map_shared_rank(&s_gt, r), eq0 += *cl.map_shared_rank(&s_eq, r);
-        if (want > 0)
-            for (int c0 = lo; c0 < hi; c0 += kEvThreads) {
-                const int t = c0 + tid;
-                const unsigned int k = t < hi ? weight_key(mass[t]) : 0u;
-                const bool g = t < hi && k > prefix, e = t < hi && k == prefix;
-                const unsigned int bg = __ballot_sync(0xffffffffu, g), be = __ballot_sync(0xffffffffu, e);
-                __syncthreads();
-                if (lane == 0) w_gt[warp] = __popc(bg), w_eq[warp] = __popc(be);
-                __syncthreads();
-                int pg = gt0, pe = eq0;
-                for (int w = 0; w < kEvThreads / 32; ++w) {
-                    if (w < warp) pg += w_gt[w], pe += w_eq[w];
-                    gt0 += w_gt[w], eq0 += w_eq[w];
-                }
-                pg += __popc(bg & ((1u << lane) - 1u)), pe += __popc(be & ((1u << lane) - 1u));
-                if (g || (e && pe < (int)need)) kept[a.sink + pg + min(pe, (int)need)] = t;
+        __syncthreads();
+        if (warp == 0) {                         // digit 255 - 8 lane - j: from the largest down
+            unsigned int c[8], sum = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) c[j] = hist[255 - 8 * lane - j], sum += c[j];
+            unsigned int upto = sum;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const unsigned int o = __shfl_up_sync(0xffffffffu, upto, d);
+                if (lane >= d) upto += o;
             }
+            unsigned int above = upto - sum;
+            if (above < need && need <= upto) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (above < need && need <= above + c[j]) {
+                        s_prefix = (prefix << 8) | (255 - 8 * lane - j);
+                        s_left = need - above;
+                    }
+                    above += c[j];
+                }
+            }
+        }
+        __syncthreads();
+        prefix = s_prefix, need = s_left;
     }
-    cl.sync();                                   // the kept indices are written (and no histogram is read any more)
+    int gt0 = 0, eq0 = 0;                        // above / at the threshold so far
+    for (int i = 0; i < rounds; ++i) {
+        const int t = i * kSelThreads + tid;
+        const unsigned int k = t < mid ? key(t) : 0u;
+        const bool g = t < mid && k > prefix, e = t < mid && k == prefix;
+        const unsigned int bg = __ballot_sync(0xffffffffu, g), be = __ballot_sync(0xffffffffu, e);
+        if (lane == 0) w_gt[warp] = __popc(bg), w_eq[warp] = __popc(be);
+        __syncthreads();
+        int cg_ = w_gt[lane], ce = w_eq[lane], ug = cg_, ue = ce;        // the warps' counts, scanned
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int og = __shfl_up_sync(0xffffffffu, ug, d), oe = __shfl_up_sync(0xffffffffu, ue, d);
+            if (lane >= d) ug += og, ue += oe;
+        }
+        const int pg = gt0 + __shfl_sync(0xffffffffu, ug - cg_, warp) + __popc(bg & ((1u << lane) - 1u));
+        const int pe = eq0 + __shfl_sync(0xffffffffu, ue - ce, warp) + __popc(be & ((1u << lane) - 1u));
+        gt0 += __shfl_sync(0xffffffffu, ug, 31), eq0 += __shfl_sync(0xffffffffu, ue, 31);
+        if (g || (e && pe < (int)need)) kept[a.sink + pg + min(pe, (int)need)] = a.sink + t;
+        __syncthreads();
+    }
+}
 
-    // compaction; nothing to do in place for a slot within its budget
-    if (!cut && a.in_place) return;
-    const int hd = a.src.hd, B = a.src.block, nc = hd / 16, NBs = cap / B, NBd = a.dst.cap / B;
+// ITEMS: 16-code chunks per thread and round, 2 (K, V) * kEvUnit * hd / 16 / kEvThreads
+template <int ITEMS, bool INPLACE>
+__global__ void __launch_bounds__(kEvThreads) kvb_compact_kernel(const KvbEvictArgs a) {
+    pdl_wait();
+    pdl_trigger();
+    const int CN = gridDim.x, rank = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+    __shared__ unsigned int s_amax[2][kEvUnit / 16];
+    const int n = evict_count(a, b), keep = a.keep, left = min(n, keep), cap = a.src.cap;
+    const bool cut = n > keep;
+    if (INPLACE && !cut) return;                 // nothing moves
+    const int64_t head = (int64_t)b * a.src.heads + h;
+    const float* mass = a.mass + head * cap;
+    float* dmass = a.dst_mass + head * a.dst.cap;
+    const int32_t* kept = a.kept + head * keep;
+    const int hd = a.src.hd, B = a.src.block, sh = 31 - __clz(B), nc = hd / 16;
     const int64_t s_head = b * a.src.slot_stride + (int64_t)h * cap * hd;
     const int64_t d_head = b * a.dst.slot_stride + (int64_t)h * a.dst.cap * hd;
-    const int8_t* src[2] = {a.src.k + s_head, a.src.v + s_head};
-    int8_t* dst[2] = {a.dst.k + d_head, a.dst.v + d_head};
-    const int64_t ss = b * a.src.scale_stride + (int64_t)h * NBs, ds = b * a.dst.scale_stride + (int64_t)h * NBd;
-    const float* sscale[2] = {a.src.ks + ss, a.src.vs + ss};
-    float* dscale[2] = {a.dst.ks + ds, a.dst.vs + ds};
-    const int rounds = (left + CN * kEvUnit - 1) / (CN * kEvUnit), per = kEvUnit * nc;
-    for (int round = 0; round < rounds; ++round) {
-        const int base = (round * CN + rank) * kEvUnit, have = min(max(left - base, 0), kEvUnit);
+    const int64_t ss = b * a.src.scale_stride + (int64_t)h * (cap >> sh);
+    const int64_t ds = b * a.dst.scale_stride + (int64_t)h * (a.dst.cap >> sh);
+    const int per = kEvUnit * nc;
+    for (int base = rank * kEvUnit; base < (INPLACE ? (left + CN * kEvUnit - 1) / (CN * kEvUnit) * (CN * kEvUnit) : left);
+         base += CN * kEvUnit) {
+        const int have = min(max(left - base, 0), kEvUnit);
         uint4 q[ITEMS];
         float s_old[ITEMS], w = 0.0f;
         if (tid < 2 * (kEvUnit / 16)) (&s_amax[0][0])[tid] = 0u;
         __syncthreads();
-        if (tid < have) w = mass[__ldcg(kept + base + tid)];
+        if (tid < have) w = mass[kept[base + tid]];
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
             const int item = tid + i * kEvThreads, z = item >= per, at = (item - z * per) / nc, ch = item - z * per - at * nc;
             s_old[i] = 0.0f;
             if (item < 2 * per && at < have) {
-                const int t = __ldcg(kept + base + at);
-                q[i] = *reinterpret_cast<const uint4*>(src[z] + (int64_t)t * hd + ch * 16);
-                s_old[i] = sscale[z][t / B];
+                const int t = kept[base + at];
+                q[i] = *reinterpret_cast<const uint4*>((z ? a.src.v : a.src.k) + s_head + (int64_t)t * hd + ch * 16);
+                s_old[i] = (z ? a.src.vs : a.src.ks)[ss + (t >> sh)];
             }
         }
 #pragma unroll
@@ -344,10 +334,10 @@ __global__ void __launch_bounds__(kEvThreads) kvb_evict_kernel(const KvbEvictArg
                 m4 = __vmaxu4(m4, __vabsdiffs4(q[i].z, 0u));
                 m4 = __vmaxu4(m4, __vabsdiffs4(q[i].w, 0u));
                 const unsigned int m = max(max(m4 & 255u, (m4 >> 8) & 255u), max((m4 >> 16) & 255u, m4 >> 24));
-                atomicMax(&s_amax[z][at / B], __float_as_uint(__fmul_rn((float)m, s_old[i])));
+                atomicMax(&s_amax[z][at >> sh], __float_as_uint(__fmul_rn((float)m, s_old[i])));
             }
         }
-        if (a.in_place) cl.sync();               // the cluster's sources of this round are in registers
+        if (INPLACE) cg::this_cluster().sync();  // the cluster's sources of this round are in registers
         else __syncthreads();
         if (tid < have) dmass[base + tid] = w;
 #pragma unroll
@@ -355,28 +345,29 @@ __global__ void __launch_bounds__(kEvThreads) kvb_evict_kernel(const KvbEvictArg
             const int item = tid + i * kEvThreads, z = item >= per, at = (item - z * per) / nc, ch = item - z * per - at * nc;
             if (item < 2 * per && at < have) {
                 uint4 o = q[i];
+                float s_new = s_old[i];
                 if (cut) {
-                    const float s_new = __fmul_rn(__uint_as_float(s_amax[z][at / B]), kInv127), rcp = 1.0f / s_new;
-                    int8_t* c = reinterpret_cast<int8_t*>(&o);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        c[j] = s_new > 0.0f ? (int8_t)kvb_code(__fmul_rn((float)c[j], s_old[i]), s_new, rcp) : (int8_t)0;
-                    if (ch == 0 && at % B == 0) dscale[z][(base + at) / B] = s_new;
-                } else if (ch == 0 && at % B == 0) {
-                    dscale[z][(base + at) / B] = s_old[i];
+                    s_new = __fmul_rn(__uint_as_float(s_amax[z][at >> sh]), kInv127);
+                    o = s_new > 0.0f ? kvb_requant16(o, s_old[i], s_new, 1.0f / s_new) : make_uint4(0, 0, 0, 0);
                 }
-                *reinterpret_cast<uint4*>(dst[z] + (int64_t)(base + at) * hd + ch * 16) = o;
+                if (ch == 0 && (at & (B - 1)) == 0) (z ? a.dst.vs : a.dst.ks)[ds + ((base + at) >> sh)] = s_new;
+                *reinterpret_cast<uint4*>((z ? a.dst.v : a.dst.k) + d_head + (int64_t)(base + at) * hd + ch * 16) = o;
             }
         }
         __syncthreads();                         // s_amax is free
     }
-    if (a.in_place) cl.sync();                   // every weight has been read
+    if (INPLACE) cg::this_cluster().sync();      // every weight has been read
     const int end = min(n, a.dst.cap);
     for (int i = left + rank * kEvThreads + tid; i < end; i += CN * kEvThreads) dmass[i] = 0.0f;
 }
 
 template <int ITEMS>
-cudaError_t evict_launch(const KvbEvictArgs& a, int cn, cudaStream_t st) {
+cudaError_t compact_launch(const KvbEvictArgs& a, cudaStream_t st) {
+    const int units = (a.keep + kEvUnit - 1) / kEvUnit;
+    if (!a.in_place)
+        return launch_k(kvb_compact_kernel<ITEMS, false>, dim3(units, a.src.heads, a.src.slots), dim3(kEvThreads), 0, st, a);
+    int cn = 8;                                  // the portable cluster size
+    while (cn > 1 && cn / 2 >= units) cn >>= 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(cn, a.src.heads, a.src.slots);
     cfg.blockDim = dim3(kEvThreads);
@@ -390,7 +381,7 @@ cudaError_t evict_launch(const KvbEvictArgs& a, int cn, cudaStream_t st) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = g_use_pdl ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kvb_evict_kernel<ITEMS>, a);
+    return cudaLaunchKernelEx(&cfg, kvb_compact_kernel<ITEMS, true>, a);
 }
 
 }  // namespace
@@ -400,7 +391,7 @@ cudaError_t launch_kvb_append(const KvbAppendArgs& a, cudaStream_t st) {
     // n / block + 2 of them
     const int64_t rows = a.r.rows, some = rows < a.c.slots ? rows : a.c.slots;
     const int64_t by_size = rows / a.c.block + 2 * some;
-    const dim3 grid((unsigned)(rows < by_size ? rows : by_size), a.c.heads, 2);
+    const dim3 grid((unsigned)(rows < by_size ? rows : by_size), a.c.heads);
     auto kern = a.type == KVB_F32    ? kvb_append_kernel<float>
                 : a.type == KVB_BF16 ? kvb_append_kernel<__nv_bfloat16>
                                      : kvb_append_kernel<__half>;
@@ -415,13 +406,16 @@ cudaError_t launch_kvb_read(const KvbReadArgs& a, cudaStream_t st) {
 }
 
 cudaError_t launch_kvb_evict(const KvbEvictArgs& a, cudaStream_t st) {
-    int cn = 8;
-    while (cn > 1 && ((int64_t)a.src.slots * a.src.heads * cn > 296 || cn * kEvUnit > a.src.cap * 2)) cn >>= 1;
+    const int cached = a.src.cap < kSelKeys ? a.src.cap : kSelKeys;
+    cudaError_t e = cudaFuncSetAttribute(kvb_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelKeys * 4);
+    if (e != cudaSuccess) return e;
+    e = launch_k(kvb_select_kernel, dim3(a.src.heads, a.src.slots), dim3(kSelThreads), (size_t)cached * 4, st, a, cached);
+    if (e != cudaSuccess) return e;
     const int items = (2 * kEvUnit * (a.src.hd / 16) + kEvThreads - 1) / kEvThreads;
-    if (items <= 1) return evict_launch<1>(a, cn, st);
-    if (items <= 2) return evict_launch<2>(a, cn, st);
-    if (items <= 4) return evict_launch<4>(a, cn, st);
-    return evict_launch<8>(a, cn, st);
+    if (items <= 1) return compact_launch<1>(a, st);
+    if (items <= 2) return compact_launch<2>(a, st);
+    if (items <= 4) return compact_launch<4>(a, st);
+    return compact_launch<8>(a, st);
 }
 
 }  // namespace w8a8

@@ -191,18 +191,98 @@ __device__ __forceinline__ int64_t div64(int64_t x, int64_t y) {
     return x >> 32 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
 }
 
-// rint(num / den) saturated to +-127 as an int8 code, the quotient correctly
-// rounded before the rounding to an integer. The product with rcp ~ 1 / den is
-// within 3 ulp of the quotient (below 1e-4 for |quotient| <= 128), so only
-// values that close to a half need the division itself.
-__device__ __forceinline__ int kvb_code(float num, float den, float rcp) {
-    float y = __fmul_rn(num, rcp);
-    float q = rintf(y);
-    if (!(fabsf(fabsf(y - q) - 0.5f) > 1e-4f)) {
-        y = __fdiv_rn(num, den);
-        q = rintf(y);
+// pairs of floats in one instruction
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t r, float& x, float& y) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+__device__ __forceinline__ uint64_t sub2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+
+// rint(num / den) saturated to +-127, the quotient correctly rounded before the
+// rounding to an integer.
+__device__ __forceinline__ int kvb_code(float num, float den) {
+    return (int)fminf(fmaxf(rintf(__fdiv_rn(num, den)), -127.0f), 127.0f);
+}
+
+// The codes of N values num (N even): codes = rint(num / den), |num| <= 127 den
+// up to rounding. The product with rcp ~ 1 / den is within 2 ulp of the quotient
+// (3e-5 for |quotient| <= 128), so only where some value lies that close to a
+// half (its distance d to the next integer: |d^2 - 1/4| < 2e-4) is the division
+// itself needed. Adding 1.5 * 2^23 rounds to an integer whose low byte is the
+// code. Scales below 2^-120 (their quotients could leave the range) divide too.
+template <int N>
+__device__ __forceinline__ void kvb_codes(const float* num, float den, float rcp, uint32_t* out) {
+    constexpr float kMagic = 12582912.0f;
+    const uint64_t r2 = pack2(rcp, rcp), m2 = pack2(kMagic, kMagic), q2 = pack2(-0.25f, -0.25f);
+    float near = 1.0f;
+    uint32_t t[N];
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        const uint64_t y = mul2(pack2(num[i], num[i + 1]), r2), s = add2(y, m2), d = sub2(y, sub2(s, m2));
+        float a, b;
+        unpack2(fma2(d, d, q2), a, b);
+        near = fminf(near, fminf(fabsf(a), fabsf(b)));
+        t[i] = (uint32_t)s, t[i + 1] = (uint32_t)(s >> 32);
     }
-    return (int)fminf(fmaxf(q, -127.0f), 127.0f);
+    if (!(near > 2e-4f) || den < 7.5e-37f) {
+#pragma unroll 1
+        for (int w = 0; w < N / 4; ++w) {
+            uint32_t c = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i)          // (registers: no indexing by w)
+                if (i / 4 == w) c |= ((uint32_t)kvb_code(num[i], den) & 255u) << (8 * (i % 4));
+#pragma unroll
+            for (int i = 0; i < N / 4; ++i)
+                if (i == w) out[i] = c;
+        }
+        return;
+    }
+#pragma unroll
+    for (int w = 0; w < N / 4; ++w)
+        out[w] = __byte_perm(__byte_perm(t[4 * w], t[4 * w + 1], 0x0040), __byte_perm(t[4 * w + 2], t[4 * w + 3], 0x0040), 0x5410);
+}
+
+// 16 codes of one scale in another: rint((q * s_old) / s_new)
+__device__ __forceinline__ uint4 kvb_requant16(uint4 w, float s_old, float s_new, float rcp) {
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+    const uint64_t bias2 = pack2(8388736.0f, 8388736.0f), s2 = pack2(s_old, s_old);
+    uint32_t o[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float num[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {            // biased bytes as the low bits of 2^23 + b + 128
+            const uint32_t y = x[2 * h + i / 2] ^ 0x80808080u;
+            const uint64_t f = pack2(__uint_as_float(__byte_perm(y, 0x4b000000u, i % 2 ? 0x7442 : 0x7440)),
+                                     __uint_as_float(__byte_perm(y, 0x4b000000u, i % 2 ? 0x7443 : 0x7441)));
+            unpack2(mul2(sub2(f, bias2), s2), num[2 * i], num[2 * i + 1]);
+        }
+        kvb_codes<8>(num, s_new, rcp, o + 2 * h);
+    }
+    return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 }  // namespace w8a8

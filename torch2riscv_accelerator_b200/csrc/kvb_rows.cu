@@ -203,31 +203,6 @@ __device__ __forceinline__ void rows_share(const RowsPlan& plan, int heads, int 
     if (cta < ctas) *lo = div64(total * cta, ctas), *hi = div64(total * (cta + 1), ctas);
 }
 
-// pairs of floats in one instruction
-__device__ __forceinline__ uint64_t pack2(float x, float y) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-    return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t r, float& x, float& y) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(r));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-    return r;
-}
-__device__ __forceinline__ uint64_t sub2(uint64_t x, uint64_t y) {
-    uint64_t r;
-    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-    return r;
-}
-
 // 16 codes as 16 halves in two 16-byte chunks of a swizzled row (`more`: rows
 // that the slab pointer is already past)
 __device__ __forceinline__ void put_codes(unsigned char* slab, int row, int ch, int odd, uint4 w, int more) {
