@@ -535,8 +535,9 @@ int w8a8_kvb_read(const W8A8KvBlocks* cache, int rows, const int32_t* pos, const
  * idle slots and rows past the capacity. heads a multiple of kv_heads. mass (or
  * NULL): [slots][kv_heads][capacity], each token's probabilities, summed over
  * the rows and the query heads of its KV head, are added. start NULL: one row
- * per slot (decode). scratch: w8a8_kvb_attn_scratch_bytes() bytes (16-byte
- * aligned, contents irrelevant), not shared by calls that can overlap. */
+ * per slot (decode). scratch: w8a8_kvb_attn_scratch_bytes() bytes for at least
+ * this many rows (16-byte aligned, contents irrelevant), not shared by calls
+ * that can overlap. */
 size_t w8a8_kvb_attn_scratch_bytes(const W8A8KvBlocks* cache, int heads, int rows, int one_row_per_slot,
                                    int with_mass, int dtype);
 int w8a8_kvb_attn(const W8A8KvBlocks* cache, const void* q, int64_t q_stride, int dtype, int heads, int rows,

@@ -458,3 +458,25 @@ def test_graph_replay_streams_and_two_calls_at_once():
                 got.append(ops.kvb_attn(q, a, p))
     torch.cuda.synchronize()
     assert all(torch.equal(x, want) for x in got)
+
+
+def test_torch_ops():
+    """torch.ops.w8a8.kvb_* do what the ops calls do."""
+    import torch2riscv_accelerator_b200.torch_ops  # noqa: F401
+    rng = np.random.default_rng(41)
+    arrays = random_cache(rng, 2, 2, 96, 32, 32)
+    a, b = on_gpu(arrays), on_gpu(arrays)
+    k = torch.randn(9, 2, 32, device=DEV)
+    q = torch.randn(9, 4, 32, device=DEV)
+    pos, start = i32([3, 60]), i32([0, 4, 8])
+    m1, m2 = torch.zeros(2, 2, 96, device=DEV), torch.zeros(2, 2, 96, device=DEV)
+    ops.kvb_append(k, -k, a, pos, start)
+    torch.ops.w8a8.kvb_append(k, -k, *b, pos, start)
+    want = ops.kvb_attn_rows(q, a, pos, start, mass=m1, out=torch.zeros_like(q))
+    assert torch.equal(torch.ops.w8a8.kvb_attn_rows(q, *b, pos, start, m2), want) and torch.equal(m1, m2)
+    assert torch.equal(torch.ops.w8a8.kvb_attn(q[:2], *b, pos, None), ops.kvb_attn(q[:2], a, pos))
+    got, want = torch.ops.w8a8.kvb_read(*b, pos, start, 9), ops.kvb_read(a, pos, start, 9)
+    assert all(torch.equal(x[:8], y[:8]) and (x[8] == 0).all() for x, y in zip(got, want))
+    got, want = torch.ops.w8a8.kvb_evict(*b, m2, i32([7, 64]), 6, 1, 2), ops.kvb_evict(a, m1, i32([7, 64]), 6, 1, 2)
+    assert all(torch.equal(x, y) for x, y in zip(got, want)) and all(torch.equal(x, y) for x, y in zip(a, b))
+    assert torch.equal(m1, m2)

@@ -104,3 +104,24 @@ def test_python_calls_check_their_tensors():
         ops.kvb_read(c._replace(k=c.k.transpose(1, 2).contiguous().transpose(1, 2)), pos, None, 2)
     with pytest.raises(ValueError, match="start"):
         ops.kvb_attn_rows(torch.zeros(2, 4, 64), c, pos, None)
+
+
+def test_torch_ops_have_fake_shapes():
+    """torch.ops.w8a8.kvb_*: registered, what they write declared, shapes without a GPU."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    import torch2riscv_accelerator_b200.torch_ops as T
+    assert {"kvb_append", "kvb_read", "kvb_attn", "kvb_attn_rows", "kvb_evict"} <= set(T.OPS)
+    args = {a.name: a for a in torch.ops.w8a8.kvb_evict.default._schema.arguments}
+    assert all(args[n].alias_info.is_write for n in ("k_codes", "k_scale", "v_codes", "v_scale", "mass"))
+    with FakeTensorMode():
+        c = (torch.empty(2, 3, 64, 32, dtype=torch.int8), torch.empty(2, 3, 2)) * 2
+        i = torch.empty(2, dtype=torch.int32)
+        q, mass = torch.empty(5, 6, 32, dtype=torch.bfloat16), torch.empty(2, 3, 64)
+        k = torch.empty(5, 3, 32)
+        s = torch.empty(3, dtype=torch.int32)
+        assert torch.ops.w8a8.kvb_append(k, k, *c, i, s) is None
+        assert torch.ops.w8a8.kvb_attn_rows(q, *c, i, s, mass).shape == q.shape
+        assert torch.ops.w8a8.kvb_attn(q[:2], *c, i, None).dtype == torch.bfloat16
+        assert [t.shape for t in torch.ops.w8a8.kvb_read(*c, i, s, 5)] == [(5, 3, 32)] * 2
+        assert [t.shape for t in torch.ops.w8a8.kvb_evict(*c, mass, i, 7)] == [(2, 3, 7), (2,)]

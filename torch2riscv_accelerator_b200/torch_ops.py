@@ -123,4 +123,79 @@ def _(func, x):
     return torch.empty_like(x)
 
 
-OPS = ("quant_act", "rmsnorm", "linear", "gemm", "linear_fused", "ffn_swiglu", "embed", "classifier", "sfu")
+# ------------------------------------------------- block-scaled 8-bit KV cache
+# (ops.KvBlocks as four tensors: codes int8 [slots, kv_heads, capacity, head_dim],
+# scales fp32 [slots, kv_heads, capacity / block])
+_KV = ("k_codes", "k_scale", "v_codes", "v_scale")
+
+
+@torch.library.custom_op(f"{_LIB}::kvb_append", mutates_args=_KV)
+def kvb_append(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor,
+               v_scale: torch.Tensor, pos: torch.Tensor, start: torch.Tensor | None = None) -> None:
+    """Rows k, v [rows, kv_heads, head_dim] into the cache (ops.kvb_append)."""
+    ops.kvb_append(k, v, (k_codes, k_scale, v_codes, v_scale), pos, start)
+
+
+@kvb_append.register_fake
+def _(k, v, k_codes, k_scale, v_codes, v_scale, pos, start=None):
+    return None
+
+
+@torch.library.custom_op(f"{_LIB}::kvb_read", mutates_args=())
+def kvb_read(k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor, v_scale: torch.Tensor,
+             pos: torch.Tensor, start: torch.Tensor, rows: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """The fp32 values held at the rows' positions (ops.kvb_read); rows behind
+    the last sequence are zero."""
+    k, v = (torch.zeros(rows, k_codes.shape[1], k_codes.shape[3], device=k_codes.device) for _ in range(2))
+    return ops.kvb_read((k_codes, k_scale, v_codes, v_scale), pos, start, rows, k=k, v=v)
+
+
+@kvb_read.register_fake
+def _(k_codes, k_scale, v_codes, v_scale, pos, start, rows):
+    shape = (rows, k_codes.shape[1], k_codes.shape[3])
+    return k_scale.new_empty(shape), k_scale.new_empty(shape)
+
+
+@torch.library.custom_op(f"{_LIB}::kvb_attn", mutates_args=("mass",))
+def kvb_attn(q: torch.Tensor, k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor,
+             v_scale: torch.Tensor, pos: torch.Tensor, mass: torch.Tensor | None,
+             scale: float | None = None) -> torch.Tensor:
+    """Attention of one row per slot (ops.kvb_attn); mass or None."""
+    return ops.kvb_attn(q, (k_codes, k_scale, v_codes, v_scale), pos, scale=scale, mass=mass)
+
+
+@kvb_attn.register_fake
+def _(q, k_codes, k_scale, v_codes, v_scale, pos, mass, scale=None):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op(f"{_LIB}::kvb_attn_rows", mutates_args=("mass",))
+def kvb_attn_rows(q: torch.Tensor, k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor,
+                  v_scale: torch.Tensor, pos: torch.Tensor, start: torch.Tensor, mass: torch.Tensor | None,
+                  scale: float | None = None) -> torch.Tensor:
+    """Attention of prompt rows (ops.kvb_attn_rows), mass or None; rows behind
+    the last sequence are zero."""
+    return ops.kvb_attn_rows(q, (k_codes, k_scale, v_codes, v_scale), pos, start, scale=scale, mass=mass,
+                             out=q.new_zeros(q.shape))
+
+
+@kvb_attn_rows.register_fake
+def _(q, k_codes, k_scale, v_codes, v_scale, pos, start, mass, scale=None):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op(f"{_LIB}::kvb_evict", mutates_args=_KV + ("mass",))
+def kvb_evict(k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor, v_scale: torch.Tensor,
+              mass: torch.Tensor, count: torch.Tensor, keep: int, sink: int = 0,
+              recent: int = 0) -> tuple[torch.Tensor, torch.Tensor]:
+    """Every slot cut in place to its `keep` heaviest tokens (ops.kvb_evict)."""
+    return ops.kvb_evict((k_codes, k_scale, v_codes, v_scale), mass, count, keep, sink=sink, recent=recent)
+
+
+@kvb_evict.register_fake
+def _(k_codes, k_scale, v_codes, v_scale, mass, count, keep, sink=0, recent=0):
+    return count.new_empty((k_codes.shape[0], k_codes.shape[1], keep)), count.new_empty(k_codes.shape[0])
+
+
+OPS = ("quant_act", "rmsnorm", "linear", "gemm", "linear_fused", "ffn_swiglu", "embed", "classifier", "sfu",
+       "kvb_append", "kvb_read", "kvb_attn", "kvb_attn_rows", "kvb_evict")
