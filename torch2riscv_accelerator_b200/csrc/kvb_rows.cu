@@ -54,9 +54,13 @@ constexpr unsigned int kErrWait = 256u;          // error bit 8: a pipeline wait
 // The tensor cores round each product's running sum towards zero: an accumulator
 // is moved out and begun anew every kFold tiles (fp32: relative error of an output over
 // 8,192 tokens: 6.3e-6 never moved, 1.8e-6 every 8, 1.0e-6 every 4, 4.8e-7 every
-// tile, where the time grows by a quarter).
+// tile; 738 us every 4 tiles, 820 every 2).
 template <typename T>
-constexpr int kFold = sizeof(T) == 4 ? 4 : 32;   // (16-bit outputs round by 2e-4 and more)
+constexpr int kFold = sizeof(T) == 4 ? 3 : 32;   // (16-bit outputs round by 2e-4 and more)
+// Shares are equal in tiles plus kUnitCost for each unit begun: a unit's first
+// queries and last outputs cost about as much as two tiles (by tiles alone the
+// CTA with a causal prompt's short units took 20 % longer than the others).
+constexpr int kUnitCost = 2;
 constexpr int kPlanThreads = 1024;
 constexpr int kFinishThreads = 256;
 
@@ -85,11 +89,11 @@ struct RowsCfg {
 };
 
 struct __align__(16) RowsUnit {
-    int slot, m, before, tiles;                  // 128-row tile of the slot, tiles of the units before, tiles
+    int slot, m, before, tiles;                  // 128-row tile of the slot, cost of the units before, tiles
     int p, r0, rows, pad;                        // position of the slot's first row, its row, the slot's n * G live rows
 };
 struct RowsPlan {                                // in scratch: total, units' count, units, slots' first units
-    int* head;                                   // [4]: tiles of all units of one KV head, units
+    int* head;                                   // [4]: cost of all units of one KV head, units
     RowsUnit* unit;
     int* first;                                  // [slots + 1]
 };
@@ -154,22 +158,25 @@ __global__ void __launch_bounds__(kPlanThreads) kvb_rows_plan(const KvbAttnArgs 
             v.slot = b, v.m = u - plan.first[b], v.p = sp.p, v.r0 = sp.r0, v.rows = live_rows(sp, a.c.cap) * G;
             v.tiles = (sp.p + min(v.m * kRows + kRows - 1, v.rows - 1) / G) / bn + 1;
         }
-        v.before = total + block_scan(v.tiles, &sum);
+        v.before = total + block_scan(u < units ? v.tiles + kUnitCost : 0, &sum);
         if (u < units) plan.unit[u] = v;
         total += sum;
     }
     if (tid == 0) plan.head[0] = total, plan.head[1] = units;
 }
 
-// A run of tiles of one unit within a CTA's share [x, end).
+// A run of tiles of one unit within a CTA's share [x, end) of the cost.
 struct Seg {
-    int64_t x, end;
+    int64_t x, end, begin_x;                     // begin_x: where the unit's cost begins
     int h, u, j, n, tiles;                       // KV head, unit; first tile, tiles here, tiles of the unit
     int slot, m, p, r0, rows;                    // rows: the slot's n * G live ones
     __device__ __forceinline__ void unit(const RowsPlan& plan) {
         const RowsUnit v = plan.unit[u];
         slot = v.slot, m = v.m, tiles = v.tiles, p = v.p, r0 = v.r0, rows = v.rows;
-        n = (int)min((int64_t)(tiles - j), end - x);
+        begin_x = (int64_t)h * plan.head[0] + v.before;
+        // a unit's own cost comes before its tiles
+        j = (int)max(x - begin_x - kUnitCost, (int64_t)0);
+        n = (int)(min(max(end - begin_x - kUnitCost, (int64_t)0), (int64_t)tiles) - j);
     }
     __device__ __forceinline__ bool begin(const RowsPlan& plan, int64_t x0, int64_t x1) {
         x = x0, end = x1;
@@ -183,16 +190,17 @@ struct Seg {
             if (plan.unit[mid].before <= at) lo = mid;
             else hi = mid;
         }
-        u = lo, j = at - plan.unit[lo].before;
+        u = lo;
         unit(plan);
-        return true;
+        return n > 0 || next(plan);              // a share may end before the unit's first tile
     }
     __device__ __forceinline__ bool next(const RowsPlan& plan) {
-        x += n;
-        if (x >= end) return false;
-        if (++u == plan.head[1]) u = 0, ++h;
-        j = 0;
-        unit(plan);
+        do {
+            x = begin_x + kUnitCost + tiles;
+            if (x >= end) return false;
+            if (++u == plan.head[1]) u = 0, ++h;
+            unit(plan);
+        } while (n <= 0);
         return true;
     }
 };
@@ -689,20 +697,24 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                     wait(&v_free[(tl - 1) % C::NBUF], ((tl - 1) / C::NBUF) & 1);
                     tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < HD / 2; c += 16) {
-                        int o[16];
-                        float4 y[4];
+                    for (int c = 0; c < HD / 2; c += HD / 4) {           // half of them in flight at a time
+                        float4 y[HD / 16];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
+                        for (int i = 0; i < HD / 16; ++i)
                             y[i] = jj == kFold<T> ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : acc[(c / 4 + i) * kRows];
-                        tmem_ld16(tmem + lanes + kO + w * (HD / 2) + c, o);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            y[i].x = fmaf(y[i].x, acc_f, __int_as_float(o[4 * i]));
-                            y[i].y = fmaf(y[i].y, acc_f, __int_as_float(o[4 * i + 1]));
-                            y[i].z = fmaf(y[i].z, acc_f, __int_as_float(o[4 * i + 2]));
-                            y[i].w = fmaf(y[i].w, acc_f, __int_as_float(o[4 * i + 3]));
-                            acc[(c / 4 + i) * kRows] = y[i];
+                        for (int x = 0; x < HD / 4; x += 16) {
+                            int o[16];
+                            tmem_ld16(tmem + lanes + kO + w * (HD / 2) + c + x, o);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                float4& z = y[x / 4 + i];
+                                z.x = fmaf(z.x, acc_f, __int_as_float(o[4 * i]));
+                                z.y = fmaf(z.y, acc_f, __int_as_float(o[4 * i + 1]));
+                                z.z = fmaf(z.z, acc_f, __int_as_float(o[4 * i + 2]));
+                                z.w = fmaf(z.w, acc_f, __int_as_float(o[4 * i + 3]));
+                                acc[((c + x) / 4 + i) * kRows] = z;
+                            }
                         }
                     }
                     acc_f = 1.0f;
@@ -800,8 +812,8 @@ __global__ void __launch_bounds__(kFinishThreads) kvb_rows_finish(const KvbAttnA
     if (lo >= hi) return;
     Seg s;
     s.begin(plan, lo, hi);
-    if (s.j == 0 || plo > lo - s.j) return;      // not cut here, or first cut before
-    const int64_t end = lo - s.j + s.tiles;
+    if (s.j == 0 || plo > s.begin_x + kUnitCost) return;                 // not cut here, or first cut before
+    const int64_t end = s.begin_x + kUnitCost + s.tiles;
     int last = blockIdx.x;                       // the last share with a part of the unit
     for (int64_t e = hi; e < end;) {
         int64_t l2, h2;
