@@ -5,6 +5,8 @@
 //   z_t = scale * sk[t / B] * (q . k_t),  v_t = sv[t / B] * code
 //
 // for the tokens t <= pos of each row; a row of an idle slot gives zeros.
+#include <cooperative_groups.h>
+
 #include "kvb.cuh"
 
 namespace w8a8 {
@@ -47,7 +49,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Maxima move lazily: a warp rescales when a score passes its head's reference
 // by 2^6 or a block's V scale its reference by 2^2; the weights
 // exp(z - m) sv / sv_ref 2^7 then stay below 2^15.
+namespace cg = cooperative_groups;
 constexpr int kStepWarps = 4;
+constexpr int kClusterMost = 16;                 // CTAs of a cluster
 constexpr int kMaxParts = 2;                     // partial units per CTA
 constexpr float kLazyScore = 6.0f, kLazyScale = 4.0f, kWeightScale = 128.0f;
 
@@ -62,7 +66,7 @@ struct StepCfg {
     static constexpr int RING = NST * STAGE;     // per warp
     static constexpr int NP = GC == 8 ? 2 : 1;   // column tiles of the weights
     static constexpr size_t PART = (size_t)GC * (HD + 2);   // floats of a partial unit: outputs, maximum, sum
-    static constexpr size_t SMEM = (size_t)kStepWarps * (RING + PART * sizeof(float));
+    static constexpr size_t smem(bool cluster) { return (size_t)kStepWarps * RING + (kStepWarps + cluster) * PART * sizeof(float); }
 };
 
 // CTAs with a share: two tiles or more each where there are few (one sequence of
@@ -142,7 +146,11 @@ struct StepIter {
 
 // EXACT: the head fills HD channels (the copies' offsets are then constants:
 // a third of the loop's address arithmetic).
-template <int HD, int GC, bool EXACT>
+// CLUSTER: few units of a small capacity (step_cluster): a unit's tiles go to the
+// CTAs of one cluster in equal runs, whose results meet through distributed shared
+// memory, without a look at the other slots, scratch or a second kernel. One
+// sequence of 2,032 tokens, 8 KV heads: 11.7 -> 8.7 us, and 3 us less of the host.
+template <int HD, int GC, bool EXACT, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, StepCfg<HD, GC>::CTAS) kvb_step_kernel(const KvbAttnArgs a, float* parts,
                                                                                  float* scores) {
     using C = StepCfg<HD, GC>;
@@ -161,46 +169,56 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD, GC>::CTAS) kvb_step_kern
     pdl_wait();
     pdl_trigger();
 
-    // this CTA's share [lo, hi) of the tiles, and the slot it begins in
-    int64_t none;
-    const int64_t total = step_scan(a, C::TILE, 0, &none) * units;
-    const int64_t ctas = step_ctas(total, gridDim.x);
-    if (blockIdx.x >= ctas) return;
-    const int64_t lo = div64(total * blockIdx.x, ctas), hi = div64(total * (blockIdx.x + 1), ctas);
-    if (warp == 0) {
-        const int per = (a.c.slots + 31) / 32, b0 = lane * per, b1 = min(b0 + per, a.c.slots);
-        int64_t mine = 0;
-        for (int b = b0; b < b1; ++b) mine += (step_len(a, b) + C::TILE - 1) / C::TILE;
-        int64_t upto = mine;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int64_t o = __shfl_up_sync(0xffffffffu, upto, d);
-            if (lane >= d) upto += o;
-        }
-        int64_t at = lo - (upto - mine) * units;
-        if (at >= 0 && at < mine * units)
-            for (int b = b0; b < b1; ++b) {
-                const int64_t n = (int64_t)((step_len(a, b) + C::TILE - 1) / C::TILE) * units;
-                if (at < n) {
-                    s_b = b, s_off = (int)at;
-                    break;
-                }
-                at -= n;
-            }
-    }
-    __syncthreads();
     StepIter in, it;                             // the next tile to fetch, the tile at work
-    it.b = s_b;
-    it.h = 0;
-    it.load(a, C::TILE);
-    {
-        const int u = s_off / it.tiles;
-        it.tile = s_off - u * it.tiles;
-        it.h = u / GT, it.gt = u - it.h * GT;
-        it.head += (int64_t)it.h * a.c.cap * hd;
+    int fetch, todo;
+    if constexpr (CLUSTER) {
+        it.b = blockIdx.z, it.h = blockIdx.y / GT, it.gt = blockIdx.y - it.h * GT;
+        it.load(a, C::TILE);
+        if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0 && a.r.pos[it.b] >= a.c.cap)
+            atomicOr(&g_kvb_attn_errors, kKvbErrCapacity);
+        it.tile = it.tiles * (int)blockIdx.x / (int)gridDim.x;
+        fetch = todo = it.tiles * ((int)blockIdx.x + 1) / (int)gridDim.x - it.tile;
+    } else {
+        // this CTA's share [lo, hi) of the tiles, and the slot it begins in
+        int64_t none;
+        const int64_t total = step_scan(a, C::TILE, 0, &none) * units;
+        const int64_t ctas = step_ctas(total, gridDim.x);
+        if (blockIdx.x >= ctas) return;
+        const int64_t lo = div64(total * blockIdx.x, ctas), hi = div64(total * (blockIdx.x + 1), ctas);
+        if (warp == 0) {
+            const int per = (a.c.slots + 31) / 32, b0 = lane * per, b1 = min(b0 + per, a.c.slots);
+            int64_t mine = 0;
+            for (int b = b0; b < b1; ++b) mine += (step_len(a, b) + C::TILE - 1) / C::TILE;
+            int64_t upto = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int64_t o = __shfl_up_sync(0xffffffffu, upto, d);
+                if (lane >= d) upto += o;
+            }
+            int64_t at = lo - (upto - mine) * units;
+            if (at >= 0 && at < mine * units)
+                for (int b = b0; b < b1; ++b) {
+                    const int64_t n = (int64_t)((step_len(a, b) + C::TILE - 1) / C::TILE) * units;
+                    if (at < n) {
+                        s_b = b, s_off = (int)at;
+                        break;
+                    }
+                    at -= n;
+                }
+        }
+        __syncthreads();
+        it.b = s_b;
+        it.h = 0;
+        it.load(a, C::TILE);
+        {
+            const int u = s_off / it.tiles;
+            it.tile = s_off - u * it.tiles;
+            it.h = u / GT, it.gt = u - it.h * GT;
+            it.head += (int64_t)it.h * a.c.cap * hd;
+        }
+        fetch = todo = (int)(hi - lo);
     }
     in = it;
-    int fetch = (int)(hi - lo), todo = fetch;
 
     // Places in a stage without bank conflicts. K (a row's 16-byte chunk ch): the
     // halves of odd rows' 128-byte lines are swapped, so that the two rows that
@@ -252,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD, GC>::CTAS) kvb_step_kern
     for (int i = 0; i < C::NST - 1; ++i) issue(i);
 
     int stage = 0;
-    while (todo > 0) {
+    for (bool once = CLUSTER; todo > 0 || once; once = false) {
         // one unit, or what of it lies in this share
         const int b = it.b, h = it.h, j0 = it.gt * GC, first = it.tile;
         const int live = min(G - j0, GC), jg = g % GC;         // heads of the unit; the one this lane quantizes
@@ -503,7 +521,11 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD, GC>::CTAS) kvb_step_kern
                 acc = fmaf(w[x * WS + d], f, acc), ll = fmaf(w[x * WS + HD + 1], f, ll);
             }
             const int64_t row = (int64_t)b * a.heads + h * G + j0 + j;
-            if (!whole) {
+            if constexpr (CLUSTER) {
+                float* p = merge + kStepWarps * C::PART + j * (HD + 2);
+                p[d] = acc;
+                if (d == 0) p[HD] = mm, p[HD + 1] = ll;
+            } else if (!whole) {
                 pt[j * (HD + 2) + d] = acc;
                 if (d == 0) pt[j * (HD + 2) + HD] = mm, pt[j * (HD + 2) + HD + 1] = ll;
             } else {
@@ -513,6 +535,37 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD, GC>::CTAS) kvb_step_kern
                     ml[0] = mm, ml[1] = ll;
                 }
             }
+        }
+        if constexpr (CLUSTER) {
+            cg::cluster_group cl = cg::this_cluster();
+            cl.sync();
+            const float* own = merge + kStepWarps * C::PART;
+            const int n = cl.num_blocks();
+            for (int i = cl.block_rank() * kThreads + tid; i < live * hd; i += n * kThreads) {
+                const int j = i / hd, d = i - j * hd;
+                float mr[kClusterMost], mm = -INFINITY, acc = 0.0f, ll = 0.0f;
+#pragma unroll
+                for (int r = 0; r < kClusterMost; ++r) {
+                    mr[r] = r < n ? cl.map_shared_rank(own, r)[j * (HD + 2) + HD] : -INFINITY;
+                    mm = fmaxf(mm, mr[r]);
+                }
+#pragma unroll
+                for (int r = 0; r < kClusterMost; ++r)
+                    if (r < n) {
+                        const float* p = cl.map_shared_rank(own, r) + j * (HD + 2);
+                        const float f = mr[r] == -INFINITY ? 0.0f : ex2(mr[r] - mm);
+                        acc = fmaf(p[d], f, acc), ll = fmaf(p[HD + 1], f, ll);
+                    }
+                // a slot without tokens: zeros
+                const int64_t row = (int64_t)b * a.heads + h * G + j0 + j;
+                store1(a.out, a.type, row * hd + d, len > 0 ? acc / ll : 0.0f);
+                if (scores && d == 0) {
+                    float* ml = scores + (int64_t)a.c.slots * a.heads * a.c.cap + 2 * row;
+                    ml[0] = mm, ml[1] = ll;
+                }
+            }
+            cl.sync();                           // the others have read this CTA's results
+            break;
         }
         todo -= n_it;
         it.next_unit(a, GT, C::TILE);            // a unit that is cut ends the share
@@ -636,23 +689,67 @@ size_t step_parts() {
     return (size_t)kSms * StepCfg<HD, GC>::CTAS * kMaxParts * StepCfg<HD, GC>::PART;
 }
 
+// CTAs of a unit's cluster, 0: in shares. By capacity, since the lengths are
+// device data. Clusters win while every unit's fits on the device at once and no
+// CTA gets a long run (a unit has at most 16 CTAs): 32 query heads on 8 KV heads
+// of 128, full slots, shares / clusters of 8 / of 16 in us, caches in L2:
+//   1 x 512 tokens 10.3 / 7.2 / 8.6    1 x 8,192 22 / 15.2 / 13.3   1 x 65,536 49 / 76 / 51
+//   4 x 2,048      19.3 / 11.3 / 20    4 x 8,192 31 / 21.7 / 28     8 x 4,096  31 / 27 / 27
+//   8 x 512        12.8 / 16.0 / 16    (the one range above that clusters lose)
+template <int HD, int GC>
+int step_cluster(const KvbCache& c, int heads) {
+    const int64_t units = (int64_t)c.heads * ((heads / c.heads + GC - 1) / GC) * c.slots;
+    const int64_t room = (int64_t)kSms * StepCfg<HD, GC>::CTAS;
+    if (units * 16 <= room / 2 && c.cap >= 4096 && c.cap <= 16384) return 16;
+    return units * 8 <= room && c.cap <= 8192 ? 8 : 0;
+}
+
+template <int HD, int GC>
+size_t step_scratch(const KvbCache& c, int heads, bool mass) {
+    return ((step_cluster<HD, GC>(c, heads) ? 0 : step_parts<HD, GC>()) + (mass ? (size_t)c.slots * heads * (c.cap + 2) : 0)) * sizeof(float);
+}
+
 template <int HD, int GC>
 cudaError_t step_launch(const KvbAttnArgs& a, cudaStream_t st) {
     using C = StepCfg<HD, GC>;
-    const int grid = kSms * C::CTAS;
+    const int cluster = step_cluster<HD, GC>(a.c, a.heads);
+    const bool exact = a.c.hd == HD;
+    const int GT = (a.heads / a.c.heads + GC - 1) / GC, grid = kSms * C::CTAS;
     float* parts = static_cast<float*>(a.scratch);
-    float* scores = a.mass ? parts + step_parts<HD, GC>() : nullptr;
-    const auto kern = a.c.hd == HD ? kvb_step_kernel<HD, GC, true> : kvb_step_kernel<HD, GC, false>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
+    float* scores = a.mass ? parts + (cluster ? 0 : step_parts<HD, GC>()) : nullptr;
+    const auto kern = cluster ? (exact ? kvb_step_kernel<HD, GC, true, true> : kvb_step_kernel<HD, GC, false, true>)
+                              : (exact ? kvb_step_kernel<HD, GC, true, false> : kvb_step_kernel<HD, GC, false, false>);
+    const size_t smem = C::smem(cluster > 0);
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    e = launch_k(kern, dim3(grid), dim3(kThreads), C::SMEM, st, a, parts, scores);
-    if (e != cudaSuccess) return e;
-    if ((int64_t)a.heads * a.c.slots <= 2 * kSms)
-        e = launch_k(kvb_step_finish<HD, GC, 4>, dim3(a.heads, a.c.slots), dim3(kThreads), 0, st, a, (const float*)parts,
-                     scores, grid);
-    else
-        e = launch_k(kvb_step_finish<HD, GC, 1>, dim3((a.heads + kThreads / 32 - 1) / (kThreads / 32), a.c.slots),
-                     dim3(kThreads), 0, st, a, (const float*)parts, scores, grid);
+    if (cluster) {
+        if (cluster > 8) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(cluster, a.c.heads * GT, a.c.slots);
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = st;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = cluster;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = g_use_pdl ? 2 : 1;
+        e = cudaLaunchKernelEx(&cfg, kern, a, parts, scores);
+    } else {
+        e = launch_k(kern, dim3(grid), dim3(kThreads), smem, st, a, parts, scores);
+        if (e != cudaSuccess) return e;
+        if ((int64_t)a.heads * a.c.slots <= 2 * kSms)
+            e = launch_k(kvb_step_finish<HD, GC, 4>, dim3(a.heads, a.c.slots), dim3(kThreads), 0, st, a,
+                         (const float*)parts, scores, grid);
+        else
+            e = launch_k(kvb_step_finish<HD, GC, 1>, dim3((a.heads + kThreads / 32 - 1) / (kThreads / 32), a.c.slots),
+                         dim3(kThreads), 0, st, a, (const float*)parts, scores, grid);
+    }
     if (e != cudaSuccess || !scores) return e;
     return launch_k(kvb_step_mass, dim3((a.c.cap + kThreads - 1) / kThreads, a.c.heads, a.c.slots), dim3(kThreads), 0, st,
                     a, (const float*)scores);
@@ -670,9 +767,7 @@ cudaError_t step_launch(const KvbAttnArgs& a, cudaStream_t st) {
 }  // namespace
 
 size_t kvb_attn_scratch(const KvbCache& c, int heads, int rows, bool one_row, bool mass, int qbytes) {
-    if (one_row)
-        return (KVB_STEP_PICK(step_parts, c.hd, heads / c.heads) + (mass ? (size_t)c.slots * heads * (c.cap + 2) : 0)) *
-               sizeof(float);
+    if (one_row) return KVB_STEP_PICK(step_scratch, c.hd, heads / c.heads, c, heads, mass);
     return kvb_rows_scratch(c, heads, rows, mass, qbytes);
 }
 

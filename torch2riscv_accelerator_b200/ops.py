@@ -479,7 +479,7 @@ def _kvb_mass(t, k, name="mass"):
 def _kvb_call(fn, dev, *args):
     """One C call on dev's current stream (the device made current for it)."""
     i = dev.index
-    if i == torch.cuda.current_device():
+    if i == torch._C._cuda_getDevice():
         rc = getattr(_lib.load(), fn)(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
         with torch.cuda.device(dev):
@@ -512,13 +512,14 @@ def kvb_read(cache, pos, start, rows, dtype=F32, k=None, v=None):
     _kvb_index(pos, c.slots, dev, "pos")
     if start is not None:
         _kvb_index(start, c.slots + 1, dev, "start")
-    k = torch.empty(rows, c.kv_heads, c.head_dim, dtype=dtype, device=dev) if k is None else k
-    v = torch.empty(rows, c.kv_heads, c.head_dim, dtype=dtype, device=dev) if v is None else v
+    if dtype not in _KVB_TYPES or rows < 0:
+        raise ValueError(f"dtype {dtype}, rows {rows}: fp32, bf16 or fp16 and a row count are required")
+    H, D = c.kv_heads, c.head_dim
     for t, name in ((k, "k"), (v, "v")):
-        if t.shape != (rows, c.kv_heads, c.head_dim) or not t.is_contiguous() or t.device != dev or t.dtype != dtype:
-            raise ValueError(f"{name}: a contiguous {dtype} {(rows, c.kv_heads, c.head_dim)} tensor is required")
-    if dtype not in _KVB_TYPES:
-        raise ValueError(f"dtype {dtype}: fp32, bf16 or fp16")
+        if t is not None and (t.shape != (rows, H, D) or not t.is_contiguous() or t.device != dev or t.dtype != dtype):
+            raise ValueError(f"{name}: a contiguous {dtype} {(rows, H, D)} tensor is required")
+    k = torch.empty_strided((rows, H, D), (H * D, D, 1), dtype=dtype, device=dev) if k is None else k
+    v = torch.empty_strided((rows, H, D), (H * D, D, 1), dtype=dtype, device=dev) if v is None else v
     _kvb_call("w8a8_kvb_read", dev, ctypes.byref(c), rows, pos.data_ptr(),
               None if start is None else start.data_ptr(), k.data_ptr(), v.data_ptr(), _KVB_TYPES[dtype])
     return k, v
@@ -550,18 +551,19 @@ def _kvb_attn(q, cache, pos, start, scale, mass, out, scratch):
     if mass is not None:
         _kvb_mass(mass, cache[0])
     if out is None:
-        out = q.new_empty(q.shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev:
         raise ValueError(f"out: a contiguous {q.dtype} {tuple(q.shape)} tensor is required")
     if scratch is None:
-        scratch = torch.empty(_kvb_scratch_bytes((c.slots, c.kv_heads, c.capacity, c.head_dim, c.block, c.slot_stride,
-                                                  c.scale_stride), heads, rows, int(start is None),
-                                                 int(mass is not None), dt), dtype=torch.uint8, device=dev)
-    elif scratch.device != dev:
-        raise ValueError(f"scratch: a tensor on {dev} is required")
+        n = _kvb_scratch_bytes((c.slots, c.kv_heads, c.capacity, c.head_dim, c.block, c.slot_stride, c.scale_stride),
+                               heads, rows, int(start is None), int(mass is not None), dt)
+        scratch = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    elif scratch.device != dev or scratch.dtype != torch.uint8 or not scratch.is_contiguous():
+        raise ValueError(f"scratch: contiguous bytes on {dev} are required")
     _kvb_call("w8a8_kvb_attn", dev, ctypes.byref(c), q.data_ptr(), qs, dt, heads, rows, pos.data_ptr(),
               None if start is None else start.data_ptr(), hd ** -0.5 if scale is None else scale, out.data_ptr(),
-              None if mass is None else mass.data_ptr(), scratch.data_ptr(), scratch.numel())
+              None if mass is None else mass.data_ptr(), None if scratch is None else scratch.data_ptr(),
+              0 if scratch is None else scratch.numel())
     return out
 
 
@@ -606,8 +608,9 @@ def kvb_evict(cache, mass, count, keep, sink=0, recent=0, dst=None, dst_mass=Non
         raise ValueError("dst_mass: only with dst")
     if not 0 < keep <= c.capacity:
         raise ValueError(f"keep {keep}: 1 .. {c.capacity}")
-    kept = torch.empty(c.slots, c.kv_heads, keep, dtype=I32, device=dev)
-    left = torch.empty(c.slots, dtype=I32, device=dev)
+    H = c.kv_heads
+    kept = torch.empty_strided((c.slots, H, keep), (H * keep, keep, 1), dtype=I32, device=dev)
+    left = torch.empty_like(count)
     _kvb_call("w8a8_kvb_evict", dev, ctypes.byref(c), mass.data_ptr(), count.data_ptr(), keep, sink, recent,
               None if d is None else ctypes.byref(d), None if d is None else dst_mass.data_ptr(), kept.data_ptr(),
               left.data_ptr())
