@@ -870,16 +870,17 @@ __global__ void __launch_bounds__(kFinishThreads) kvb_rows_finish(const KvbAttnA
 // its KV head, from the rows' maxima and sums: the scores once more, tokens as
 // the 16 rows of mma m16n8k16 (the codes as halves in registers for the whole
 // kernel), the prepared queries as its columns (hi and lo into one accumulator).
-// A warp holds 16 TG tokens; with few token tiles the CTA's four warps hold the
-// same ones and share out the rows (SPLIT 4), else they hold four tiles and
-// share the queries they read (SPLIT 1). Sums run in a fixed order: 32 rows at a
-// time, then over the warps. Bound by the tensor products and their exponentials.
+// A warp holds 16 TG tokens; with few token tiles the CTA's warps hold the same
+// ones and share out the rows (kvb_rows_mass_few), else four warps hold four tiles
+// and share the queries they read. Sums run in a fixed order: over a warp's rows,
+// then over the warps. Bound by the tensor products and their exponentials.
 constexpr int kMassThreads = 128;
 
 template <int HD, bool Q2>
 struct MassCfg {
     static constexpr int TG = HD == 256 ? 1 : 2;
-    static constexpr int RS = RowsCfg<HD>::qrow(Q2 ? 4 : 2), CHUNK = 32 * RS;
+    static constexpr int RS = RowsCfg<HD>::qrow(Q2 ? 4 : 2), CHUNK = 32 * RS, GROUP = 8 * RS;
+    static constexpr int STAGES = HD == 256 ? 1 : 3;                     // groups in a warp's ring
 };
 
 __device__ __forceinline__ void mma_halves(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -889,33 +890,12 @@ __device__ __forceinline__ void mma_halves(float* c, const uint32_t* a, uint32_t
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <int HD, bool Q2, int SPLIT>
-__global__ void __launch_bounds__(kMassThreads) kvb_rows_mass(const KvbAttnArgs a, const RowsPlan plan,
-                                                            const unsigned char* queries, int units, const float2* stats) {
-    using M = MassCfg<HD, Q2>;
-    constexpr int TG = M::TG, RS = M::RS, KB = HD / 32, TOK = 16 * TG;   // 32-channel blocks; tokens of a warp
-    extern __shared__ __align__(128) unsigned char smem[];               // [2][SPLIT][CHUNK]
-    __shared__ __align__(8) uint64_t full[2];
-    __shared__ float2 s_stat[2][SPLIT][32];
-    __shared__ float s_sum[4][TOK];
-    const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int h = blockIdx.y, b = blockIdx.z, hd = a.c.hd, G = a.heads / a.c.heads;
-    if (tid == 0) {
-        mbar_init(&full[0], 1), mbar_init(&full[1], 1);
-        mbar_fence_init();
-    }
-    pdl_wait();
-    pdl_trigger();
-    const KvbSpan sp = kvb_span(a.r, b);
-    const int n = live_rows(sp, a.c.cap), len = sp.p + n, rows = n * G;
-    const int tile = blockIdx.x * TOK * (4 / SPLIT), t0 = tile + warp / SPLIT * TOK;   // the CTA's, the warp's first token
-    if (n == 0 || tile >= len) return;
-    if (plan.first[b] + (rows + kRows - 1) / kRows > plan.head[1]) return;   // only with offsets out of order
-    __syncthreads();
-
-    // the warp's tokens: channels 32 x + 8 t + 0..7 of rows g and g + 8
-    uint32_t k[TG][KB][2][4];
-    float sk[TG];
+// A warp's 16 TG tokens from t0 on: channels 32 x + 8 t + 0..7 of rows g and g + 8,
+// and the 16 tokens' scale.
+template <int TG, int KB>
+__device__ __forceinline__ void mass_tokens(const KvbAttnArgs& a, int b, int h, int t0, int len, int g, int t,
+                                            uint32_t (&k)[TG][KB][2][4], float (&sk)[TG]) {
+    const int hd = a.c.hd;
 #pragma unroll
     for (int j = 0; j < TG; ++j) {
         sk[j] = 0.0f;
@@ -939,19 +919,67 @@ __global__ void __launch_bounds__(kMassThreads) kvb_rows_mass(const KvbAttnArgs 
         if (t0 + 16 * j < len)                   // 16 tokens lie in one block
             sk[j] = a.c.ks[b * a.c.scale_stride + (int64_t)h * (a.c.cap / a.c.block) + (t0 + 16 * j) / a.c.block];
     }
+}
+
+// Scores of 8 rows (qr: row g's channels from 8 t on) and the warp's tokens.
+template <int HD, bool Q2>
+__device__ __forceinline__ void mass_scores(const unsigned char* qr, const uint32_t (&k)[MassCfg<HD, Q2>::TG][HD / 32][2][4],
+                                            float (&z)[MassCfg<HD, Q2>::TG][4]) {
+    constexpr int TG = MassCfg<HD, Q2>::TG, KB = HD / 32;
+#pragma unroll
+    for (int j = 0; j < TG; ++j) z[j][0] = z[j][1] = z[j][2] = z[j][3] = 0.0f;
+#pragma unroll
+    for (int x = 0; x < KB; ++x)
+#pragma unroll
+        for (int y = 0; y < (Q2 ? 2 : 1); ++y) {
+            const uint4 w = *reinterpret_cast<const uint4*>(qr + y * HD * 2 + x * 64);
+#pragma unroll
+            for (int j = 0; j < TG; ++j) {
+                mma_halves(z[j], k[j][x][0], w.x, w.y);
+                mma_halves(z[j], k[j][x][1], w.z, w.w);
+            }
+        }
+}
+
+template <int HD, bool Q2>
+__global__ void __launch_bounds__(kMassThreads) kvb_rows_mass(const KvbAttnArgs a, const RowsPlan plan,
+                                                            const unsigned char* queries, int units, const float2* stats) {
+    using M = MassCfg<HD, Q2>;
+    constexpr int TG = M::TG, RS = M::RS, KB = HD / 32, TOK = 16 * TG;   // 32-channel blocks; tokens of a warp
+    extern __shared__ __align__(128) unsigned char smem[];               // [2][CHUNK]
+    __shared__ __align__(8) uint64_t full[2];
+    __shared__ float2 s_stat[2][32];
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int h = blockIdx.y, b = blockIdx.z, G = a.heads / a.c.heads;
+    if (tid == 0) {
+        mbar_init(&full[0], 1), mbar_init(&full[1], 1);
+        mbar_fence_init();
+    }
+    pdl_wait();
+    pdl_trigger();
+    const KvbSpan sp = kvb_span(a.r, b);
+    const int n = live_rows(sp, a.c.cap), len = sp.p + n, rows = n * G;
+    const int tile = blockIdx.x * TOK * 4, t0 = tile + warp * TOK;       // the CTA's, the warp's first token
+    if (n == 0 || tile >= len) return;
+    if (plan.first[b] + (rows + kRows - 1) / kRows > plan.head[1]) return;   // only with offsets out of order
+    __syncthreads();
+
+    uint32_t k[TG][KB][2][4];
+    float sk[TG];
+    mass_tokens<TG, KB>(a, b, h, t0, len, g, t, k, sk);
     // chunks of 32 rows (f = query row * G + head), from the first that sees the tile
     const unsigned char* src = queries + ((int64_t)h * units + plan.first[b]) * 4 * M::CHUNK;
     const int c0 = max(tile - sp.p, 0) * G / 32, c1 = (rows + 31) / 32;
-    auto fetch = [&](int step) {                 // SPLIT chunks and their rows' maxima and sums
-        const int s = step & 1, c = c0 + step * SPLIT, m = min(SPLIT, c1 - c);
-        if (m <= 0) return;
+    auto fetch = [&](int step) {                 // a chunk and its rows' maxima and sums
+        const int s = step & 1, c = c0 + step;
+        if (c >= c1) return;
         if (tid == 0) {
-            mbar_expect_tx(&full[s], m * M::CHUNK);
-            bulk_g2s(smem + s * SPLIT * M::CHUNK, src + (int64_t)c * M::CHUNK, m * M::CHUNK, &full[s]);
+            mbar_expect_tx(&full[s], M::CHUNK);
+            bulk_g2s(smem + s * M::CHUNK, src + (int64_t)c * M::CHUNK, M::CHUNK, &full[s]);
         }
-        if (tid < 32 * SPLIT) {
+        if (tid < 32) {
             const int f = c * 32 + tid;          // rows past the last weigh nothing
-            s_stat[s][tid / 32][tid % 32] =
+            s_stat[s][tid] =
                 f < rows ? stats[(int64_t)(sp.r0 + f / G) * a.heads + h * G + f % G] : make_float2(0.0f, 0.0f);
         }
     };
@@ -960,56 +988,136 @@ __global__ void __launch_bounds__(kMassThreads) kvb_rows_mass(const KvbAttnArgs 
     float sum[TG][2];
 #pragma unroll
     for (int j = 0; j < TG; ++j) sum[j][0] = sum[j][1] = 0.0f;
-    const int steps = (c1 - c0 + SPLIT - 1) / SPLIT;
-    for (int step = 0; step < steps; ++step) {
-        const int s = step & 1, c = c0 + step * SPLIT + warp % SPLIT;
+    for (int c = c0; c < c1; ++c) {
+        const int step = c - c0, s = step & 1;
         if (!mbar_wait(&full[s], (step >> 1) & 1) && lane == 0) atomicOr(&g_kvb_rows_errors, kErrWait);
         __syncthreads();                         // s_stat as well
-        if (c < c1) {
-            const unsigned char* q = smem + (s * SPLIT + warp % SPLIT) * M::CHUNK;
-            const bool cut = sp.p + c * 32 / G < t0 + TOK - 1;           // some row does not see every token
-            float part[TG][2];
+        const unsigned char* q = smem + s * M::CHUNK;
+        const bool cut = sp.p + c * 32 / G < t0 + TOK - 1;               // some row does not see every token
+        float part[TG][2];
 #pragma unroll
-            for (int j = 0; j < TG; ++j) part[j][0] = part[j][1] = 0.0f;
+        for (int j = 0; j < TG; ++j) part[j][0] = part[j][1] = 0.0f;
 #pragma unroll 1
-            for (int i = 0; i < 4; ++i) {        // 8 rows
-                float z[TG][4];
+        for (int i = 0; i < 4; ++i) {            // 8 rows
+            float z[TG][4];
+            mass_scores<HD, Q2>(q + (i * 8 + g) * RS + 16 * t, k, z);
+            // columns: rows c * 32 + 8 i + 2 t + e
 #pragma unroll
-                for (int j = 0; j < TG; ++j) z[j][0] = z[j][1] = z[j][2] = z[j][3] = 0.0f;
-                const unsigned char* qr = q + (i * 8 + g) * RS + 16 * t;
+            for (int e = 0; e < 2; ++e) {
+                const int col = i * 8 + 2 * t + e, f = c * 32 + col;
+                const float fq = *reinterpret_cast<const float*>(q + col * RS + (RS - 16));
+                const float2 st = s_stat[s][col];
+                const int lim = f < rows ? sp.p + f / G : -1;
 #pragma unroll
-                for (int x = 0; x < KB; ++x)
+                for (int j = 0; j < TG; ++j)
 #pragma unroll
-                    for (int y = 0; y < (Q2 ? 2 : 1); ++y) {
-                        const uint4 w = *reinterpret_cast<const uint4*>(qr + y * HD * 2 + x * 64);
-#pragma unroll
-                        for (int j = 0; j < TG; ++j) {
-                            mma_halves(z[j], k[j][x][0], w.x, w.y);
-                            mma_halves(z[j], k[j][x][1], w.z, w.w);
-                        }
+                    for (int r = 0; r < 2; ++r) {
+                        float w = ex2(fmaf(z[j][2 * r + e], sk[j] * fq, -st.x)) * st.y;
+                        if ((cut || f >= rows) && t0 + 16 * j + 8 * r + g > lim) w = 0.0f;
+                        part[j][r] += w;
                     }
-                // columns: rows c * 32 + 8 i + 2 t + e
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int col = i * 8 + 2 * t + e, f = c * 32 + col;
-                    const float fq = *reinterpret_cast<const float*>(q + col * RS + (RS - 16));
-                    const float2 st = s_stat[s][warp % SPLIT][col];
-                    const int lim = f < rows ? sp.p + f / G : -1;
-#pragma unroll
-                    for (int j = 0; j < TG; ++j)
-#pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            float w = ex2(fmaf(z[j][2 * r + e], sk[j] * fq, -st.x)) * st.y;
-                            if ((cut || f >= rows) && t0 + 16 * j + 8 * r + g > lim) w = 0.0f;
-                            part[j][r] += w;
-                        }
-                }
             }
-#pragma unroll
-            for (int j = 0; j < TG; ++j) sum[j][0] += part[j][0], sum[j][1] += part[j][1];
         }
+#pragma unroll
+        for (int j = 0; j < TG; ++j) sum[j][0] += part[j][0], sum[j][1] += part[j][1];
         __syncthreads();
         fetch(step + 2);
+    }
+#pragma unroll
+    for (int j = 0; j < TG; ++j)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            sum[j][r] += __shfl_xor_sync(0xffffffffu, sum[j][r], 1);
+            sum[j][r] += __shfl_xor_sync(0xffffffffu, sum[j][r], 2);
+            const int tok = t0 + 16 * j + 8 * r + g;
+            if (t == 0 && tok < len) a.mass[((int64_t)b * a.c.heads + h) * a.c.cap + tok] += sum[j][r];
+        }
+}
+
+// Few token tiles: sixteen warps on the same 16 TG tokens, each taking every
+// sixteenth group of 8 rows through a ring of its own, so that no barrier stands
+// in the loop and four warps a scheduler cover the products' latency. 1,500 rows
+// of 9 heads on 3 KV heads of 64, two sequences: FEW_US us against 100 with four warps
+// that met at each 32 rows.
+constexpr int kFewWarps = 16;
+
+template <int HD, bool Q2>
+__global__ void __launch_bounds__(kFewWarps * 32) kvb_rows_mass_few(const KvbAttnArgs a, const RowsPlan plan,
+                                                                  const unsigned char* queries, int units,
+                                                                  const float2* stats) {
+    using M = MassCfg<HD, Q2>;
+    constexpr int TG = M::TG, RS = M::RS, KB = HD / 32, TOK = 16 * TG;
+    constexpr int GROUP = M::GROUP, STAGES = M::STAGES;
+    extern __shared__ __align__(128) unsigned char smem[];               // [kFewWarps][STAGES][GROUP]
+    __shared__ __align__(8) uint64_t full[kFewWarps][STAGES];
+    __shared__ float s_sum[kFewWarps][TOK];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int h = blockIdx.y, b = blockIdx.z, G = a.heads / a.c.heads;
+    if (lane == 0) {
+        for (int i = 0; i < STAGES; ++i) mbar_init(&full[warp][i], 1);
+        mbar_fence_init();
+    }
+    __syncwarp();
+    pdl_wait();
+    pdl_trigger();
+    const KvbSpan sp = kvb_span(a.r, b);
+    const int n = live_rows(sp, a.c.cap), len = sp.p + n, rows = n * G, t0 = blockIdx.x * TOK;
+    if (n == 0 || t0 >= len) return;
+    if (plan.first[b] + (rows + kRows - 1) / kRows > plan.head[1]) return;   // only with offsets out of order
+
+    // groups of 8 rows (f = query row * G + head), from the first that sees the tile
+    const unsigned char* src = queries + ((int64_t)h * units + plan.first[b]) * 4 * M::CHUNK;
+    const int c0 = max(t0 - sp.p, 0) * G / 8 + warp, c1 = (rows + 7) / 8;
+    unsigned char* ring = smem + warp * STAGES * GROUP;
+    auto fetch = [&](int c, int s) {
+        if (lane == 0 && c < c1) {
+            mbar_expect_tx(&full[warp][s], GROUP);
+            bulk_g2s(ring + s * GROUP, src + (int64_t)c * GROUP, GROUP, &full[warp][s]);
+        }
+    };
+    // lane 8 x + i: row i of the group, its maximum, 1 / sum and last visible token
+    auto load_stat = [&](int c, int* lim) {
+        const int f = c * 8 + (lane & 7), i = f / G;
+        *lim = f < rows ? sp.p + i : -1;
+        return f < rows ? stats[(int64_t)(sp.r0 + i) * a.heads + h * G + (f - i * G)] : make_float2(0.0f, 0.0f);
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) fetch(c0 + i * kFewWarps, i);
+    uint32_t k[TG][KB][2][4];
+    float sk[TG], sum[TG][2];
+    mass_tokens<TG, KB>(a, b, h, t0, len, g, t, k, sk);
+#pragma unroll
+    for (int j = 0; j < TG; ++j) sum[j][0] = sum[j][1] = 0.0f;
+    int s = 0, phase = 0, lim_next;
+    float2 st_next = load_stat(c0, &lim_next);
+    for (int c = c0; c < c1; c += kFewWarps) {
+        const float2 st = st_next;
+        const int lim = lim_next;
+        st_next = load_stat(c + kFewWarps, &lim_next);
+        if (!mbar_wait(&full[warp][s], phase) && lane == 0) atomicOr(&g_kvb_rows_errors, kErrWait);
+        const unsigned char* q = ring + s * GROUP;
+        float z[TG][4], fq[2];
+        mass_scores<HD, Q2>(q + g * RS + 16 * t, k, z);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) fq[e] = *reinterpret_cast<const float*>(q + (2 * t + e) * RS + (RS - 16));
+        __syncwarp();                            // the stage is read
+        fetch(c + STAGES * kFewWarps, s);
+        if (++s == STAGES) s = 0, phase ^= 1;
+        // columns: rows 8 c + 2 t + e
+        const bool cut = sp.p + c * 8 / G < t0 + TOK - 1 || c * 8 + 7 >= rows;       // some row does not see every token
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float mx = __shfl_sync(0xffffffffu, st.x, 2 * t + e), inv = __shfl_sync(0xffffffffu, st.y, 2 * t + e);
+            const int last = __shfl_sync(0xffffffffu, lim, 2 * t + e);
+#pragma unroll
+            for (int j = 0; j < TG; ++j)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    float w = ex2(fmaf(z[j][2 * r + e], sk[j] * fq[e], -mx)) * inv;
+                    if (cut && t0 + 16 * j + 8 * r + g > last) w = 0.0f;
+                    sum[j][r] += w;
+                }
+        }
     }
 #pragma unroll
     for (int j = 0; j < TG; ++j)
@@ -1020,14 +1128,11 @@ __global__ void __launch_bounds__(kMassThreads) kvb_rows_mass(const KvbAttnArgs 
             if (t == 0) s_sum[warp][16 * j + 8 * r + g] = sum[j][r];
         }
     __syncthreads();
-    for (int i = tid; i < TOK * (4 / SPLIT); i += kMassThreads) {
-        const int tok = tile + i;
-        if (tok >= len) break;
-        const int w0 = i / TOK * SPLIT;
+    if (threadIdx.x < TOK && t0 + threadIdx.x < len) {
         float y = 0.0f;
 #pragma unroll
-        for (int w = 0; w < SPLIT; ++w) y += s_sum[w0 + w][i % TOK];
-        a.mass[((int64_t)b * a.c.heads + h) * a.c.cap + tok] += y;
+        for (int w = 0; w < kFewWarps; ++w) y += s_sum[w][threadIdx.x];
+        a.mass[((int64_t)b * a.c.heads + h) * a.c.cap + t0 + threadIdx.x] += y;
     }
 }
 
@@ -1036,16 +1141,16 @@ cudaError_t mass_launch(const KvbAttnArgs& a, const RowsPlan& plan, const unsign
                         const float2* stats, cudaStream_t st) {
     using M = MassCfg<HD, Q2>;
     constexpr int TOK = 16 * M::TG;
-    // four tiles a CTA once that still gives every SM two CTAs (by the capacity:
-    // the lengths are device data)
     const int64_t tiles = (a.c.cap + TOK - 1) / TOK;
-    const bool share = tiles / 4 * a.c.heads * a.c.slots >= 2 * kSms || HD == 256;
-    const auto kern = share ? kvb_rows_mass<HD, Q2, 1> : kvb_rows_mass<HD, Q2, HD == 256 ? 1 : 4>;
-    const size_t smem = (size_t)2 * (share ? 1 : 4) * M::CHUNK;
+    // four tiles a CTA, which reads a quarter of the queries, once that still gives
+    // every SM two CTAs (by the capacity: the lengths are device data)
+    const bool share = tiles / 4 * a.c.heads * a.c.slots >= 2 * kSms;
+    const auto kern = share ? kvb_rows_mass<HD, Q2> : kvb_rows_mass_few<HD, Q2>;
+    const size_t smem = share ? (size_t)2 * M::CHUNK : (size_t)kFewWarps * M::STAGES * M::GROUP;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    return launch_k(kern, dim3((unsigned)(share ? (tiles + 3) / 4 : tiles), a.c.heads, a.c.slots), dim3(kMassThreads), smem,
-                    st, a, plan, queries, units, stats);
+    return launch_k(kern, dim3((unsigned)(share ? (tiles + 3) / 4 : tiles), a.c.heads, a.c.slots),
+                    dim3(share ? kMassThreads : kFewWarps * 32), smem, st, a, plan, queries, units, stats);
 }
 
 int rows_hd(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
