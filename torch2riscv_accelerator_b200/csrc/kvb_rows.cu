@@ -52,9 +52,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLazyScore = 6.0f, kLazyLog = 2.0f, kWeightLog = 7.0f;   // log2: see kvb_attn.cu
 constexpr unsigned int kErrWait = 256u;          // error bit 8: a pipeline wait gave up
 // The tensor cores round each product's running sum towards zero: an accumulator
-// is moved out and begun anew every kFold tiles (fp32: relative error of an output over
-// 8,192 tokens: 6.3e-6 never moved, 1.8e-6 every 8, 1.0e-6 every 4, 4.8e-7 every
-// tile; 738 us every 4 tiles, 820 every 2).
+// is moved out and begun anew every kFold tiles (fp32, relative error of an output over
+// 8,192 tokens: 6.3e-6 never moved, 1.8e-6 every 8, 1.0e-6 every 4, 8e-7 every 3,
+// 6.4e-7 every 2; moving out every 2 tiles instead of 4 costs 11 % of the time).
 template <typename T>
 constexpr int kFold = sizeof(T) == 4 ? 3 : 32;   // (16-bit outputs round by 2e-4 and more)
 // Shares are equal in tiles plus kUnitCost for each unit begun: a unit's first
@@ -92,10 +92,15 @@ struct __align__(16) RowsUnit {
     int slot, m, before, tiles;                  // 128-row tile of the slot, cost of the units before, tiles
     int p, r0, rows, pad;                        // position of the slot's first row, its row, the slot's n * G live rows
 };
-struct RowsPlan {                                // in scratch: total, units' count, units, slots' first units
+struct __align__(16) RowsShare {                 // a CTA's share [lo, hi) of the cost
+    int64_t lo, hi;
+    int h, u, join, pad;                         // KV head and unit where it begins; if that unit is cut there for the
+};                                               // first time, the last share with a part of it, else -1
+struct RowsPlan {                                // in scratch
     int* head;                                   // [4]: cost of all units of one KV head, units
     RowsUnit* unit;
-    int* first;                                  // [slots + 1]
+    int* first;                                  // [slots + 1]: the slots' first units
+    RowsShare* share;                            // [kSms]
 };
 
 __host__ __device__ inline int64_t max_units(const KvbCache& c, int heads, int rows) {
@@ -131,6 +136,7 @@ __global__ void __launch_bounds__(kPlanThreads) kvb_rows_plan(const KvbAttnArgs 
     pdl_wait();
     pdl_trigger();
     const int tid = threadIdx.x, S = a.c.slots, G = a.heads / a.c.heads;
+    __shared__ int s_before[kPlanThreads];       // the first units' costs before them
     int units = 0, sum;
     for (int b0 = 0; b0 < S; b0 += kPlanThreads) {
         const int b = b0 + tid;
@@ -160,9 +166,35 @@ __global__ void __launch_bounds__(kPlanThreads) kvb_rows_plan(const KvbAttnArgs 
         }
         v.before = total + block_scan(u < units ? v.tiles + kUnitCost : 0, &sum);
         if (u < units) plan.unit[u] = v;
+        if (u0 == 0) s_before[tid] = v.before;
         total += sum;
     }
     if (tid == 0) plan.head[0] = total, plan.head[1] = units;
+    __syncthreads();
+    // the shares, and where they begin (searched here once: a search through
+    // global memory in every CTA of two kernels took 1.5 us in each)
+    if (tid < kSms) {
+        RowsShare w{};
+        w.join = -1;
+        const int64_t all = (int64_t)total * a.c.heads, ctas = min(all, (int64_t)kSms);
+        if (tid < ctas) {
+            w.lo = div64(all * tid, ctas), w.hi = div64(all * (tid + 1), ctas);
+            w.h = (int)div64(w.lo, total);
+            const int at = (int)(w.lo - (int64_t)w.h * total);
+            int u = 0, hi = units;               // the last unit that begins at or before `at`
+            while (hi - u > 1) {
+                const int mid = (u + hi) >> 1;
+                if ((mid < kPlanThreads ? s_before[mid] : plan.unit[mid].before) <= at) u = mid;
+                else hi = mid;
+            }
+            w.u = u;
+            const int64_t begin = (int64_t)w.h * total + (u < kPlanThreads ? s_before[u] : plan.unit[u].before);
+            const int64_t end = begin + kUnitCost + plan.unit[u].tiles;
+            if (w.lo > begin + kUnitCost && div64(all * (tid - 1), ctas) <= begin + kUnitCost)
+                w.join = (int)div64(end * ctas - 1, all);
+        }
+        plan.share[tid] = w;
+    }
 }
 
 // A run of tiles of one unit within a CTA's share [x, end) of the cost.
@@ -178,19 +210,11 @@ struct Seg {
         j = (int)max(x - begin_x - kUnitCost, (int64_t)0);
         n = (int)(min(max(end - begin_x - kUnitCost, (int64_t)0), (int64_t)tiles) - j);
     }
-    __device__ __forceinline__ bool begin(const RowsPlan& plan, int64_t x0, int64_t x1) {
-        x = x0, end = x1;
+    __device__ __forceinline__ bool begin(const RowsPlan& plan, int cta) {
+        const RowsShare w = plan.share[cta];
+        x = w.lo, end = w.hi;
         if (x >= end) return false;
-        const int total = plan.head[0];
-        h = (int)div64(x, total);
-        const int at = (int)(x - (int64_t)h * total);
-        int lo = 0, hi = plan.head[1];
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (plan.unit[mid].before <= at) lo = mid;
-            else hi = mid;
-        }
-        u = lo;
+        h = w.h, u = w.u;
         unit(plan);
         return n > 0 || next(plan);              // a share may end before the unit's first tile
     }
@@ -204,12 +228,6 @@ struct Seg {
         return true;
     }
 };
-
-__device__ __forceinline__ void rows_share(const RowsPlan& plan, int heads, int grid, int cta, int64_t* lo, int64_t* hi) {
-    const int64_t total = (int64_t)plan.head[0] * heads, ctas = total < grid ? total : grid;
-    *lo = *hi = 0;
-    if (cta < ctas) *lo = div64(total * cta, ctas), *hi = div64(total * (cta + 1), ctas);
-}
 
 // 16 codes as 16 halves in two 16-byte chunks of a swizzled row (`more`: rows
 // that the slab pointer is already past)
@@ -369,9 +387,7 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
         if (!mbar_done(bar, parity)) wait_long(bar, parity, &dead);
     };
     Seg seg;
-    int64_t lo, hi;
-    rows_share(plan, a.c.heads, gridDim.x, blockIdx.x, &lo, &hi);
-    const bool any = seg.begin(plan, lo, hi);
+    const bool any = seg.begin(plan, blockIdx.x);
     int J = 0, sn = 0;                           // tiles and units of this CTA so far
 
     if (warp == 0) {
@@ -793,7 +809,7 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
 constexpr int kJoinRows = 16;
 template <int HD>
 __global__ void __launch_bounds__(kFinishThreads) kvb_rows_finish(const KvbAttnArgs a, const RowsPlan plan,
-                                                                const float* parts, float2* stats, int grid) {
+                                                                const float* parts, float2* stats) {
     using C = RowsCfg<HD>;
     pdl_wait();
     pdl_trigger();
@@ -805,21 +821,10 @@ __global__ void __launch_bounds__(kFinishThreads) kvb_rows_finish(const KvbAttnA
         const int64_t e0 = (int64_t)(s.r0 + live) * a.heads * hd, e1 = (int64_t)(s.r0 + s.n) * a.heads * hd;
         for (int64_t i = e0 + tid; i < e1; i += kFinishThreads) store1(a.out, a.type, i, 0.0f);
     }
-    int64_t lo, hi, plo, phi;
-    if (blockIdx.x == 0) return;
-    rows_share(plan, a.c.heads, grid, blockIdx.x, &lo, &hi);
-    rows_share(plan, a.c.heads, grid, blockIdx.x - 1, &plo, &phi);
-    if (lo >= hi) return;
-    Seg s;
-    s.begin(plan, lo, hi);
-    if (s.j == 0 || plo > s.begin_x + kUnitCost) return;                 // not cut here, or first cut before
-    const int64_t end = s.begin_x + kUnitCost + s.tiles;
-    int last = blockIdx.x;                       // the last share with a part of the unit
-    for (int64_t e = hi; e < end;) {
-        int64_t l2, h2;
-        rows_share(plan, a.c.heads, grid, ++last, &l2, &h2);
-        e = h2;
-    }
+    const RowsShare w = plan.share[blockIdx.x];
+    const int last = w.join;
+    if (last < 0) return;                        // no unit's first cut
+    const RowsUnit s = plan.unit[w.u];
     const int c0 = blockIdx.x - 1;
     const int r0 = blockIdx.y * kJoinRows;
     __shared__ float s_m[kJoinRows], s_i[kJoinRows], s_o[kJoinRows][HD + 1];
@@ -828,20 +833,23 @@ __global__ void __launch_bounds__(kFinishThreads) kvb_rows_finish(const KvbAttnA
         static_assert(kFinishThreads == 16 * kJoinRows, "16 threads a row");
         const int row = r0 + tid / 16;           // 16 threads share a row's parts
         float m = -INFINITY, l = 0.0f;
-        for (int c = c0 + tid % 16; c <= last; c += 16) m = fmaxf(m, at(c)[kRows * HD + row]);
-#pragma unroll
-        for (int d = 8; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
         for (int c = c0 + tid % 16; c <= last; c += 16) {
-            const float mc = at(c)[kRows * HD + row];
-            if (mc != -INFINITY) l = fmaf(at(c)[kRows * (HD + 1) + row], ex2(mc - m), l);
+            const float mc = at(c)[kRows * HD + row], lc = at(c)[kRows * (HD + 1) + row], top = fmaxf(m, mc);
+            l = (m == -INFINITY ? l : l * ex2(m - top)) + (mc == -INFINITY ? lc : lc * ex2(mc - top));
+            m = top;
         }
+        float top = m;
+#pragma unroll
+        for (int d = 8; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        if (m != -INFINITY) l *= ex2(m - top);
+        m = top;
 #pragma unroll
         for (int d = 8; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
         if (tid % 16 == 0) {
             s_m[tid / 16] = m, s_i[tid / 16] = 1.0f / l;
             const int f = s.m * kRows + row;
             if (stats && f < s.rows)
-                stats[(int64_t)(s.r0 + f / G) * a.heads + s.h * G + f % G] = make_float2(m, 1.0f / l);
+                stats[(int64_t)(s.r0 + f / G) * a.heads + w.h * G + f % G] = make_float2(m, 1.0f / l);
         }
     }
     __syncthreads();
@@ -862,7 +870,7 @@ __global__ void __launch_bounds__(kFinishThreads) kvb_rows_finish(const KvbAttnA
     for (int i = tid; i < kJoinRows * HD; i += kFinishThreads) {
         const int r = i / HD, d = i % HD, f = s.m * kRows + r0 + r;
         if (f < s.rows && d < hd)
-            store1(a.out, a.type, ((int64_t)(s.r0 + f / G) * a.heads + s.h * G + f % G) * hd + d, s_o[r][d]);
+            store1(a.out, a.type, ((int64_t)(s.r0 + f / G) * a.heads + w.h * G + f % G) * hd + d, s_o[r][d]);
     }
 }
 
@@ -1037,7 +1045,7 @@ __global__ void __launch_bounds__(kMassThreads) kvb_rows_mass(const KvbAttnArgs 
 // Few token tiles: sixteen warps on the same 16 TG tokens, each taking every
 // sixteenth group of 8 rows through a ring of its own, so that no barrier stands
 // in the loop and four warps a scheduler cover the products' latency. 1,500 rows
-// of 9 heads on 3 KV heads of 64, two sequences: FEW_US us against 100 with four warps
+// of 9 heads on 3 KV heads of 64, two sequences: 27 us against 90 with four warps
 // that met at each 32 rows.
 constexpr int kFewWarps = 16;
 
@@ -1052,7 +1060,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) kvb_rows_mass_few(const KvbAtt
     __shared__ __align__(8) uint64_t full[kFewWarps][STAGES];
     __shared__ float s_sum[kFewWarps][TOK];
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int h = blockIdx.y, b = blockIdx.z, G = a.heads / a.c.heads;
+    const int h = blockIdx.x, b = blockIdx.y, G = a.heads / a.c.heads;
     if (lane == 0) {
         for (int i = 0; i < STAGES; ++i) mbar_init(&full[warp][i], 1);
         mbar_fence_init();
@@ -1061,7 +1069,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) kvb_rows_mass_few(const KvbAtt
     pdl_wait();
     pdl_trigger();
     const KvbSpan sp = kvb_span(a.r, b);
-    const int n = live_rows(sp, a.c.cap), len = sp.p + n, rows = n * G, t0 = blockIdx.x * TOK;
+    const int n = live_rows(sp, a.c.cap), len = sp.p + n, rows = n * G, t0 = blockIdx.z * TOK;   // the longest first
     if (n == 0 || t0 >= len) return;
     if (plan.first[b] + (rows + kRows - 1) / kRows > plan.head[1]) return;   // only with offsets out of order
 
@@ -1149,7 +1157,8 @@ cudaError_t mass_launch(const KvbAttnArgs& a, const RowsPlan& plan, const unsign
     const size_t smem = share ? (size_t)2 * M::CHUNK : (size_t)kFewWarps * M::STAGES * M::GROUP;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
-    return launch_k(kern, dim3((unsigned)(share ? (tiles + 3) / 4 : tiles), a.c.heads, a.c.slots),
+    const unsigned n = (unsigned)(share ? (tiles + 3) / 4 : tiles);
+    return launch_k(kern, share ? dim3(n, a.c.heads, a.c.slots) : dim3(a.c.heads, a.c.slots, n),
                     dim3(share ? kMassThreads : kFewWarps * 32), smem, st, a, plan, queries, units, stats);
 }
 
@@ -1158,10 +1167,11 @@ int rows_hd(int hd) { return hd <= 64 ? 64 : hd <= 128 ? 128 : 256; }
 size_t up16(size_t x) { return (x + 15) & ~(size_t)15; }
 
 struct RowsLayout {                              // byte offsets in the scratch
-    size_t unit, first, parts, accs, stats, queries, total;
+    size_t share, unit, first, parts, accs, stats, queries, total;
     RowsLayout(const KvbCache& c, int heads, int rows, bool mass, int qbytes) {
         const int hd = rows_hd(c.hd);
-        unit = 16;
+        share = 16;
+        unit = share + kSms * sizeof(RowsShare);
         first = unit + (size_t)max_units(c, heads, rows) * sizeof(RowsUnit);
         parts = up16(first + ((size_t)c.slots + 1) * sizeof(int));
         accs = parts + (size_t)kSms * 2 * kRows * (hd + 2) * sizeof(float);
@@ -1177,7 +1187,8 @@ cudaError_t rows_launch(const KvbAttnArgs& a, cudaStream_t st) {
     const int qbytes = a.type == KVB_F32 ? 4 : 2, units = (int)max_units(a.c, a.heads, a.r.rows);
     const RowsLayout L(a.c, a.heads, a.r.rows, a.mass != nullptr, qbytes);
     char* s = static_cast<char*>(a.scratch);
-    const RowsPlan plan{reinterpret_cast<int*>(s), reinterpret_cast<RowsUnit*>(s + L.unit), reinterpret_cast<int*>(s + L.first)};
+    const RowsPlan plan{reinterpret_cast<int*>(s), reinterpret_cast<RowsUnit*>(s + L.unit), reinterpret_cast<int*>(s + L.first),
+                        reinterpret_cast<RowsShare*>(s + L.share)};
     float* parts = reinterpret_cast<float*>(s + L.parts);
     float2* stats = a.mass ? reinterpret_cast<float2*>(s + L.stats) : nullptr;
     cudaError_t e = launch_k(kvb_rows_plan, dim3(1), dim3(kPlanThreads), 0, st, a, plan, C::BN, units);
@@ -1199,7 +1210,7 @@ cudaError_t rows_launch(const KvbAttnArgs& a, cudaStream_t st) {
                  (const unsigned char*)queries, units, parts,
                  reinterpret_cast<float*>(s + L.accs), stats);
     if (e != cudaSuccess) return e;
-    e = launch_k(kvb_rows_finish<HD>, dim3(kSms, kRows / kJoinRows), dim3(kFinishThreads), 0, st, a, plan, (const float*)parts, stats, kSms);
+    e = launch_k(kvb_rows_finish<HD>, dim3(kSms, kRows / kJoinRows), dim3(kFinishThreads), 0, st, a, plan, (const float*)parts, stats);
     if (e != cudaSuccess || !stats) return e;
     return qbytes == 4 ? mass_launch<HD, true>(a, plan, queries, units, stats, st)
                        : mass_launch<HD, false>(a, plan, queries, units, stats, st);
