@@ -1045,8 +1045,8 @@ __global__ void __launch_bounds__(kMassThreads) kvb_rows_mass(const KvbAttnArgs 
 // Few token tiles: sixteen warps on the same 16 TG tokens, each taking every
 // sixteenth group of 8 rows through a ring of its own, so that no barrier stands
 // in the loop and four warps a scheduler cover the products' latency. 1,500 rows
-// of 9 heads on 3 KV heads of 64, two sequences: 27 us against 90 with four warps
-// that met at each 32 rows.
+// of 9 heads on 3 KV heads of 64, two sequences: 38 us against 100 with four warps
+// that met at each 32 rows (57 with eight; bound by its instructions, not the rings).
 constexpr int kFewWarps = 16;
 
 template <int HD, bool Q2>

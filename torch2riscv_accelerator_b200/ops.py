@@ -428,14 +428,17 @@ def kvb_cache(slots, kv_heads, capacity, head_dim, block=64, device="cuda"):
 
 
 @functools.lru_cache(maxsize=256)
-def _kvb_layout(k, k_st, ks, ks_st, v, v_st, vs, vs_st, name):
-    """What a cache's shapes and strides say: slots, heads, capacity, head_dim,
-    block, slot strides (a refused one raises)."""
+def _kvb_layout(k, ks, v, vs, strides, name):
+    """What a cache's shapes and strides (None: all contiguous) say: slots,
+    heads, capacity, head_dim, block, slot strides (a refused one raises)."""
     if len(k) != 4 or v != k or len(ks) != 3 or ks[:2] != k[:2] or vs != ks or ks[2] == 0 or k[2] % ks[2]:
         raise ValueError(f"{name}: codes {tuple(k)} / {tuple(v)} and scales {tuple(ks)} / {tuple(vs)} do not belong "
                          "together")
     S, H, T, D = k
     NB = ks[2]
+    if strides is None:
+        return S, H, T, D, T // NB, H * T * D, H * NB
+    k_st, ks_st, v_st, vs_st = strides
     if k_st[1:] != (T * D, D, 1) or v_st[1:] != k_st[1:] or ks_st[1:] != (NB, 1) or vs_st[1:] != ks_st[1:] or \
             (S > 1 and (v_st != k_st or vs_st != ks_st)):
         raise ValueError(f"{name}: each slot's codes and scales must be contiguous, K's and V's alike")
@@ -443,28 +446,30 @@ def _kvb_layout(k, k_st, ks, ks_st, v, v_st, vs, vs_st, name):
 
 
 def _kvb(cache, name="cache"):
-    """The checked W8A8KvBlocks of a cache, and its device."""
+    """The checked W8A8KvBlocks of a cache, and its device's index."""
     k, ks, v, vs = cache
     if k.dtype != I8 or v.dtype != I8 or ks.dtype != F32 or vs.dtype != F32:
         raise ValueError(f"{name}: int8 codes and fp32 scales are required")
-    layout = _kvb_layout(k.shape, k.stride(), ks.shape, ks.stride(), v.shape, v.stride(), vs.shape, vs.stride(), name)
-    dev = k.device
-    if not k.is_cuda or v.device != dev or ks.device != dev or vs.device != dev:
+    dense = k.is_contiguous() and ks.is_contiguous() and v.is_contiguous() and vs.is_contiguous()
+    layout = _kvb_layout(k.shape, ks.shape, v.shape, vs.shape,
+                         None if dense else (k.stride(), ks.stride(), v.stride(), vs.stride()), name)
+    dev = k.get_device()
+    if not k.is_cuda or ks.get_device() != dev or v.get_device() != dev or vs.get_device() != dev:
         raise ValueError(f"{name}: CUDA tensors on one device are required")
     return _lib.W8A8KvBlocks(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), *layout), dev
 
 
 def _kvb_index(t, n, dev, name):
-    if t.dtype != I32 or t.shape != (n,) or t.device != dev or (n > 1 and t.stride(0) != 1):
-        raise ValueError(f"{name}: a contiguous int32 [{n}] tensor on {dev} is required")
+    if t.dtype != I32 or t.shape != (n,) or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous int32 [{n}] tensor on cuda:{dev} is required")
 
 
 def _kvb_rows(t, heads, hd, dev, name):
     """(dtype code, elements between rows) of rows [rows, heads, hd] whose rows
     are contiguous (a slice of a wider row is fine)."""
     code, sh, st = _KVB_TYPES.get(t.dtype), t.shape, t.stride()
-    if code is None or len(sh) != 3 or t.device != dev:
-        raise ValueError(f"{name}: fp32, bf16 or fp16 [rows, {heads or 'heads'}, {hd}] on {dev} is required")
+    if code is None or len(sh) != 3 or t.get_device() != dev:
+        raise ValueError(f"{name}: fp32, bf16 or fp16 [rows, {heads or 'heads'}, {hd}] on cuda:{dev} is required")
     if sh[2] != hd or (heads and sh[1] != heads) or st[2] != 1 or (sh[1] > 1 and st[1] != hd):
         raise ValueError(f"{name}: [rows, {heads or 'heads'}, {hd}] with contiguous rows is required, got {tuple(sh)} "
                          f"with strides {st}")
@@ -472,18 +477,17 @@ def _kvb_rows(t, heads, hd, dev, name):
 
 
 def _kvb_mass(t, k, name="mass"):
-    if t.dtype != F32 or t.shape != k.shape[:3] or not t.is_contiguous() or t.device != k.device:
+    if t.dtype != F32 or t.shape != k.shape[:3] or not t.is_contiguous() or t.get_device() != k.get_device():
         raise ValueError(f"{name}: a contiguous fp32 {tuple(k.shape[:3])} tensor on {k.device} is required")
 
 
 def _kvb_call(fn, dev, *args):
-    """One C call on dev's current stream (the device made current for it)."""
-    i = dev.index
-    if i == torch._C._cuda_getDevice():
-        rc = getattr(_lib.load(), fn)(*args, torch._C._cuda_getCurrentRawStream(i))
+    """One C call on the current stream of device dev (made current for it)."""
+    if dev == torch._C._cuda_getDevice():
+        rc = getattr(_lib.load(), fn)(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = getattr(_lib.load(), fn)(*args, torch._C._cuda_getCurrentRawStream(i))
+            rc = getattr(_lib.load(), fn)(*args, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         _lib.check(fn, rc)
 
@@ -516,7 +520,8 @@ def kvb_read(cache, pos, start, rows, dtype=F32, k=None, v=None):
         raise ValueError(f"dtype {dtype}, rows {rows}: fp32, bf16 or fp16 and a row count are required")
     H, D = c.kv_heads, c.head_dim
     for t, name in ((k, "k"), (v, "v")):
-        if t is not None and (t.shape != (rows, H, D) or not t.is_contiguous() or t.device != dev or t.dtype != dtype):
+        if t is not None and (t.shape != (rows, H, D) or not t.is_contiguous() or t.get_device() != dev or
+                              t.dtype != dtype):
             raise ValueError(f"{name}: a contiguous {dtype} {(rows, H, D)} tensor is required")
     k = torch.empty_strided((rows, H, D), (H * D, D, 1), dtype=dtype, device=dev) if k is None else k
     v = torch.empty_strided((rows, H, D), (H * D, D, 1), dtype=dtype, device=dev) if v is None else v
@@ -552,14 +557,14 @@ def _kvb_attn(q, cache, pos, start, scale, mass, out, scratch):
         _kvb_mass(mass, cache[0])
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.device != dev:
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.get_device() != dev:
         raise ValueError(f"out: a contiguous {q.dtype} {tuple(q.shape)} tensor is required")
     if scratch is None:
         n = _kvb_scratch_bytes((c.slots, c.kv_heads, c.capacity, c.head_dim, c.block, c.slot_stride, c.scale_stride),
                                heads, rows, int(start is None), int(mass is not None), dt)
         scratch = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    elif scratch.device != dev or scratch.dtype != torch.uint8 or not scratch.is_contiguous():
-        raise ValueError(f"scratch: contiguous bytes on {dev} are required")
+    elif scratch.get_device() != dev or scratch.dtype != torch.uint8 or not scratch.is_contiguous():
+        raise ValueError(f"scratch: contiguous bytes on cuda:{dev} are required")
     _kvb_call("w8a8_kvb_attn", dev, ctypes.byref(c), q.data_ptr(), qs, dt, heads, rows, pos.data_ptr(),
               None if start is None else start.data_ptr(), hd ** -0.5 if scale is None else scale, out.data_ptr(),
               None if mass is None else mass.data_ptr(), None if scratch is None else scratch.data_ptr(),
@@ -603,7 +608,7 @@ def kvb_evict(cache, mass, count, keep, sink=0, recent=0, dst=None, dst_mass=Non
             raise ValueError("dst_mass: required with dst")
         _kvb_mass(dst_mass, dst[0], "dst_mass")
         if ddev != dev:
-            raise ValueError(f"dst: a cache on {dev} is required")
+            raise ValueError(f"dst: a cache on cuda:{dev} is required")
     elif dst_mass is not None:
         raise ValueError("dst_mass: only with dst")
     if not 0 < keep <= c.capacity:
