@@ -480,3 +480,167 @@ def test_torch_ops():
     got, want = torch.ops.w8a8.kvb_evict(*b, m2, i32([7, 64]), 6, 1, 2), ops.kvb_evict(a, m1, i32([7, 64]), 6, 1, 2)
     assert all(torch.equal(x, y) for x, y in zip(got, want)) and all(torch.equal(x, y) for x, y in zip(a, b))
     assert torch.equal(m1, m2)
+
+
+# ------------------------------------------------------- the forms for many units
+@pytest.mark.parametrize("heads,kv_heads,hd,block,dt,S,cap,mass", [
+    (6, 3, 64, 32, "fp32", 120, 192, True),
+    (8, 2, 64, 64, "bf16", 150, 128, False),
+    (12, 4, 128, 64, "fp32", 60, 320, True),
+    (16, 2, 128, 16, "fp16", 70, 208, True),
+    (9, 9, 112, 16, "fp32", 40, 160, False),
+    (4, 2, 256, 64, "fp32", 40, 256, True),
+    (12, 1, 208, 16, "bf16", 90, 96, True),
+    (4, 2, 64, 128, "fp32", 1, 20096, True),
+    (2, 1, 128, 128, "fp16", 2, 16512, False),
+    (4, 2, 128, 64, "fp32", 2, 4160, True)])
+def test_step_attention_of_many_slots_and_long_ones(heads, kv_heads, hd, block, dt, S, cap, mass):
+    """Sequences of every length up to the capacity, idle ones between them."""
+    rng = np.random.default_rng(heads * hd + S)
+    cache = random_cache(rng, S, kv_heads, cap, hd, block)
+    pos = rng.integers(0, cap, S)
+    pos[-1], pos[:S // 5] = cap - 1, -1
+    dev = on_gpu(cache)
+    q, q64 = rounded(rng, (S, heads, hd), TYPES[dt], 1.5)
+    m, want = torch.zeros(S, kv_heads, cap, device=DEV), np.zeros((S, kv_heads, cap))
+    out = ops.kvb_attn(q, dev, i32(pos), mass=m if mass else None)
+    ref = R.attend(q64, *cache, pos, mass=want)
+    check_attn(out, ref, TYPES[dt], cap, hd)
+    assert (host(out.float())[pos < 0] == 0).all()
+    if mass:
+        check_mass(m, want, np.zeros_like(want), ref[1].max(), cap, hd)
+    assert torch.equal(ops.kvb_attn(q, dev, i32(pos)), out)
+    scratch = ops.kvb_attn_scratch(dev, heads, S, start=False, mass=True, dtype=TYPES[dt])
+    scratch.fill_(255)                                                    # its contents do not matter
+    again = torch.zeros_like(m)
+    assert torch.equal(ops.kvb_attn(q, dev, i32(pos), mass=again, scratch=scratch), out)
+    assert not mass or torch.equal(again, m)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,block,dt,S,cap", [
+    (4, 2, 64, 64, "fp32", 160, 128), (6, 2, 128, 32, "bf16", 150, 160), (3, 3, 80, 16, "fp32", 110, 144),
+    (2, 1, 256, 64, "fp16", 80, 256)])
+def test_prompt_attention_of_many_slots(heads, kv_heads, hd, block, dt, S, cap):
+    """Prompts of a few rows each, idle and empty ones between them."""
+    rng = np.random.default_rng(heads * hd + S)
+    cache = random_cache(rng, S, kv_heads, cap, hd, block)
+    counts = rng.integers(0, 9, S)
+    pos = rng.integers(0, cap - 8, S)
+    pos[::7], counts[::5] = -1, 0
+    start = np.concatenate([[0], np.cumsum(counts)])
+    dev = on_gpu(cache)
+    q, q64 = rounded(rng, (start[-1] + 2, heads, hd), TYPES[dt], 1.5)
+    m, want = torch.zeros(S, kv_heads, cap, device=DEV), np.zeros((S, kv_heads, cap))
+    scratch = ops.kvb_attn_scratch(dev, heads, q.shape[0], mass=True, dtype=TYPES[dt])
+    scratch.fill_(255)
+    out = torch.full_like(q, 7.0)
+    ops.kvb_attn_rows(q, dev, i32(pos), i32(start), mass=m, out=out, scratch=scratch)
+    ref = R.attend(q64[:start[-1]], *cache, pos, start, mass=want)
+    check_attn(out[:start[-1]], ref, TYPES[dt], cap, hd)
+    assert (host(out.float())[start[-1]:] == 7).all()
+    check_mass(m, want, np.zeros_like(want), ref[1].max(), cap, hd)
+
+
+@pytest.mark.parametrize("rows", [False, True])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_a_bad_query_row_stays_alone(rows, hd):
+    """A row with a NaN or an infinity gives NaN, its neighbours what they gave without it; a negative scale."""
+    rng = np.random.default_rng(hd)
+    cache = random_cache(rng, 3, 2, 128, hd, 64)
+    dev = on_gpu(cache)
+    counts = [5, 20, 1] if rows else [1, 1, 1]
+    start = np.concatenate([[0], np.cumsum(counts)])
+    pos = [3, 100, 60]
+    q, q64 = rounded(rng, (start[-1], 4, hd), torch.float32)
+    call = lambda x: (ops.kvb_attn_rows(x, dev, i32(pos), i32(start), scale=-0.1) if rows else
+                      ops.kvb_attn(x, dev, i32(pos), scale=-0.1))
+    want = call(q)
+    check_attn(want, R.attend(q64, *cache, pos, start, scale=-0.1), torch.float32, 128, hd)
+    bad = q.clone()
+    bad[1, 0, 3], bad[1, 3, 0] = float("nan"), float("-inf")
+    got = call(bad)
+    assert got[1, 0].isnan().all() and got[1, 3].isnan().all()
+    keep = torch.ones(q.shape[:2], dtype=torch.bool, device=DEV)
+    keep[1, 0] = keep[1, 3] = False
+    assert torch.equal(got[keep], want[keep])
+
+
+@pytest.mark.parametrize("rows", [False, True])
+def test_nothing_to_attend(rows):
+    """Only idle slots, or no rows at all: zeros, and nothing else is touched."""
+    rng = np.random.default_rng(3)
+    dev = on_gpu(random_cache(rng, 3, 2, 64, 64, 64))
+    m = torch.ones(3, 2, 64, device=DEV)
+    if rows:
+        q = torch.randn(6, 4, 64, device=DEV)
+        out = torch.full_like(q, 7.0)
+        ops.kvb_attn_rows(q, dev, i32([-1, -5, -1]), i32([0, 2, 2, 4]), mass=m, out=out)
+        assert (out[:4] == 0).all() and (out[4:] == 7).all()
+        out.fill_(7.0)
+        ops.kvb_attn_rows(q, dev, i32([0, 3, 63]), i32([0, 0, 0, 0]), mass=m, out=out)
+        assert (out == 7).all()
+        assert ops.kvb_attn_rows(q[:0], dev, i32([0, 3, 63]), i32([0, 0, 0, 0])).shape == (0, 4, 64)
+    else:
+        assert (ops.kvb_attn(torch.randn(3, 4, 64, device=DEV), dev, i32([-1, -7, -1]), mass=m) == 0).all()
+    assert (m == 1).all()
+
+
+def test_prompts_and_eviction_captured_and_on_two_streams():
+    """A captured prompt (append, attention with weights, cut in place, read-back)
+    replayed with other lengths; prompt attention and many-slot steps on two
+    streams at once."""
+    rng = np.random.default_rng(37)
+    S, heads, H, hd, block, cap, R0, keep = 3, 6, 2, 64, 32, 256, 160, 48
+    arrays = random_cache(rng, S, H, cap, hd, block)
+    a, b = on_gpu(arrays), on_gpu(arrays)
+    qkv = torch.zeros(R0, heads + 2 * H, hd, device=DEV)
+    pos, start, count = i32([0] * S), i32([0] * (S + 1)), i32([0] * S)
+    mass, out, zero = torch.zeros(S, H, cap, device=DEV), torch.zeros(R0, heads, hd, device=DEV), i32([0] * S)
+
+    def step(c, x, p, st, n, m, o):
+        ops.kvb_append(x[:, heads:heads + H], x[:, heads + H:], c, p, st)
+        ops.kvb_attn_rows(x[:, :heads], c, p, st, mass=m, out=o)
+        kept, left = ops.kvb_evict(c, m, n, keep, sink=1, recent=9)
+        return kept, left, *ops.kvb_read(c, zero, None, S)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(a, qkv, pos, start, count, mass, out)
+    torch.cuda.current_stream().wait_stream(side)
+    for t, w in zip(a, arrays):
+        t.copy_(cu(w))
+    mass.zero_()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        held = step(a, qkv, pos, start, count, mass, out)
+    m2 = torch.zeros_like(mass)
+    p = [0, 0, 0]
+    for counts in ([150, 3, 0], [1, 60, 99], [40, 40, 40]):
+        x = torch.randn(R0, heads + 2 * H, hd, device=DEV)
+        st = np.concatenate([[0], np.cumsum(counts)])
+        n = [u + v for u, v in zip(p, counts)]
+        for t, w in ((qkv, x), (pos, i32(p)), (start, i32(st)), (count, i32(n))):
+            t.copy_(w)
+        out.zero_()
+        g.replay()
+        o2 = torch.zeros_like(out)
+        got = step(b, x, i32(p), i32(st), i32(n), m2, o2)
+        assert torch.equal(out, o2) and torch.equal(mass, m2)
+        assert all(torch.equal(u, v) for u, v in zip(held, got))
+        assert all(torch.equal(u, v) for u, v in zip(a, b))
+        p = host(got[1]).tolist()
+        assert p == [min(v, keep) for v in n]
+    many = on_gpu(random_cache(rng, 100, 4, 128, 64, 64))
+    q1, p1 = torch.randn(100, 8, 64, device=DEV), i32(rng.integers(0, 128, 100))
+    q2, p2, s2 = torch.randn(300, heads, hd, device=DEV), i32([5, 100, 0]), i32([0, 130, 200, 300])
+    calls = [lambda: ops.kvb_attn(q1, many, p1), lambda: ops.kvb_attn_rows(q2[:, :, :], a, p2, s2),
+             lambda: ops.kvb_attn(q2[:S], a, p2)]
+    want = [f() for f in calls]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(3)], []
+    for i in range(24):
+        with torch.cuda.stream(streams[i % 3]):
+            got.append((i // 3 % 3, calls[i // 3 % 3]()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i, x in got)
