@@ -26,8 +26,15 @@
 //             V as it lies, its rows being the contraction).
 // Block scales do not touch the codes: K's multiplies the scores of its 16
 // columns, V's goes into the weights, exp(z - m) sv / sv_ref 2^7 by one
-// exponential, with the lazily moved references of the one-row kernel (kvb_attn.cu), so that the
-// accumulator is rescaled rarely.
+// exponential, with the lazily moved references of the one-row kernel
+// (kvb_attn.cu), so that the accumulator is rescaled rarely.
+//
+// Bound by two chains of about 3,700 cycles a tile of 128 rows x 128 tokens that run
+// beside each other: the products' thread (2,048 cycles of products for fp32, the
+// rest hand-overs) and the softmax warps (wait, read 64 scores, exponentials, write
+// the weights). 8,192 causal rows, 16 heads on 8 KV heads of 128, fp32: 610 us, 0.45
+// PFLOP/s of the formula's operations and 0.9 of those done (hi and lo); the tensor
+// pipe is active 41 % of the time, 3 % of the DRAM's rate is used.
 #include <type_traits>
 
 #include "kvb.cuh"
