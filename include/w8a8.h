@@ -533,8 +533,8 @@ int w8a8_kvb_read(const W8A8KvBlocks* cache, int rows, const int32_t* pos, const
  * over their slot's tokens up to and with their own position (appended
  * before): out [rows][heads][head_dim] = softmax(scale * q . k) v, zero for
  * idle slots and rows past the capacity. heads a multiple of kv_heads. mass (or
- * NULL): [slots][kv_heads][capacity], each token's probabilities, summed over
- * the rows and the query heads of its KV head, are added. start NULL: one row
+ * NULL; 16-byte aligned): [slots][kv_heads][capacity], each token's probabilities,
+ * summed over the rows and the query heads of its KV head, are added. start NULL: one row
  * per slot (decode). scratch: w8a8_kvb_attn_scratch_bytes() bytes for at least
  * this many rows (16-byte aligned, contents irrelevant), not shared by calls
  * that can overlap. */

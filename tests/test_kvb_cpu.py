@@ -65,6 +65,7 @@ def test_attention_arguments(lib):
     assert attn(t=-1) == EINVAL and attn(q=None) == EINVAL and attn(out=None) == EINVAL
     assert attn(rows=1) == EINVAL and attn(pos=None) == EINVAL
     assert attn(qs=255) == EINVAL and attn(q=20) == EALIGN and attn(out=8) == EALIGN
+    assert attn(mass=4) == EALIGN and attn(scratch=8, mass=16) == EALIGN
     assert attn(scale=float("nan")) == EINVAL and attn(scale=float("inf")) == EINVAL
     assert attn(rows=0, start=16, q=None, out=None) == OK
     need = lib.w8a8_kvb_attn_scratch_bytes(c, 4, 2, 1, 1, 0)

@@ -771,7 +771,7 @@ int w8a8_kvb_attn(const W8A8KvBlocks* cache, const void* q, int64_t q_stride, in
     if (!e || heads <= 0 || heads > 65535 || heads % a.c.heads || !(std::fabs(scale) <= 3.4e38f)) return W8A8_EINVAL;
     if ((int64_t)rows * heads > INT32_MAX) return W8A8_EINVAL;
     if (rows > 0 && (!q || !out || (rows > 1 && q_stride < (int64_t)heads * a.c.hd))) return W8A8_EINVAL;
-    if (!al16(q) || !al16(out) || (q_stride * e) % 16 || !al16(scratch)) return W8A8_EALIGN;
+    if (!al16(q) || !al16(out) || (q_stride * e) % 16 || !al16(mass) || !al16(scratch)) return W8A8_EALIGN;
     if (rows == 0) return W8A8_OK;
     const size_t need = kvb_attn_scratch(a.c, heads, rows, start == nullptr, mass != nullptr, e);
     if (need && (!scratch || scratch_bytes < need)) return W8A8_ESCRATCH;
