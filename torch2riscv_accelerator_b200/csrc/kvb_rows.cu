@@ -68,7 +68,7 @@ constexpr int kFold = sizeof(T) == 4 ? 3 : 32;   // (16-bit outputs round by 2e-
 // queries and last outputs cost about as much as two tiles (by tiles alone the
 // CTA with a causal prompt's short units took 20 % longer than the others).
 constexpr int kUnitCost = 2;
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 256;                 // (1,024: 1.8 us longer, in the scans)
 constexpr int kFinishThreads = 256;
 
 template <int HD>
@@ -118,7 +118,7 @@ __device__ __forceinline__ int live_rows(const KvbSpan& s, int cap) { return s.p
 
 // exclusive scan over the CTA's kPlanThreads threads; *sum the total
 __device__ __forceinline__ int block_scan(int x, int* sum) {
-    __shared__ int w[32];
+    __shared__ int w[kPlanThreads / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     int upto = x;
 #pragma unroll
@@ -130,7 +130,7 @@ __device__ __forceinline__ int block_scan(int x, int* sum) {
     __syncthreads();
     int before = 0, all = 0;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i < kPlanThreads / 32; ++i) {
         if (i < warp) before += w[i];
         all += w[i];
     }
@@ -894,8 +894,10 @@ constexpr int kMassThreads = 128;
 template <int HD, bool Q2>
 struct MassCfg {
     static constexpr int TG = HD == 256 ? 1 : 2;
-    static constexpr int RS = RowsCfg<HD>::qrow(Q2 ? 4 : 2), CHUNK = 32 * RS, GROUP = 8 * RS;
-    static constexpr int STAGES = HD == 256 ? 1 : 3;                     // groups in a warp's ring
+    static constexpr int RS = RowsCfg<HD>::qrow(Q2 ? 4 : 2), CHUNK = 32 * RS;
+    // kvb_rows_mass_few: rows of a step, groups of them in a warp's ring (208 KB in 16)
+    static constexpr int STEP = HD == 64 ? 16 : 8, GROUP = STEP * RS;
+    static constexpr int STAGES = HD == 256 ? 1 : 3;
 };
 
 __device__ __forceinline__ void mma_halves(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -1050,10 +1052,11 @@ __global__ void __launch_bounds__(kMassThreads) kvb_rows_mass(const KvbAttnArgs 
 }
 
 // Few token tiles: sixteen warps on the same 16 TG tokens, each taking every
-// sixteenth group of 8 rows through a ring of its own, so that no barrier stands
+// sixteenth group of STEP rows through a ring of its own, so that no barrier stands
 // in the loop and four warps a scheduler cover the products' latency. 1,500 rows
-// of 9 heads on 3 KV heads of 64, two sequences: 38 us against 100 with four warps
-// that met at each 32 rows (57 with eight; bound by its instructions, not the rings).
+// of 9 heads on 3 KV heads of 64, two sequences: 31 us (38 with 8 rows a step, 57 with
+// half the warps) against 100 with four warps that met at each 32 rows. Bound by
+// its instructions, not by the rings.
 constexpr int kFewWarps = 16;
 
 template <int HD, bool Q2>
@@ -1062,7 +1065,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) kvb_rows_mass_few(const KvbAtt
                                                                   const float2* stats) {
     using M = MassCfg<HD, Q2>;
     constexpr int TG = M::TG, RS = M::RS, KB = HD / 32, TOK = 16 * TG;
-    constexpr int GROUP = M::GROUP, STAGES = M::STAGES;
+    constexpr int STEP = M::STEP, GROUP = M::GROUP, STAGES = M::STAGES;
     extern __shared__ __align__(128) unsigned char smem[];               // [kFewWarps][STAGES][GROUP]
     __shared__ __align__(8) uint64_t full[kFewWarps][STAGES];
     __shared__ float s_sum[kFewWarps][TOK];
@@ -1080,9 +1083,9 @@ __global__ void __launch_bounds__(kFewWarps * 32) kvb_rows_mass_few(const KvbAtt
     if (n == 0 || t0 >= len) return;
     if (plan.first[b] + (rows + kRows - 1) / kRows > plan.head[1]) return;   // only with offsets out of order
 
-    // groups of 8 rows (f = query row * G + head), from the first that sees the tile
+    // groups of STEP rows (f = query row * G + head), from the first that sees the tile
     const unsigned char* src = queries + ((int64_t)h * units + plan.first[b]) * 4 * M::CHUNK;
-    const int c0 = max(t0 - sp.p, 0) * G / 8 + warp, c1 = (rows + 7) / 8;
+    const int c0 = max(t0 - sp.p, 0) * G / STEP + warp, c1 = (rows + STEP - 1) / STEP;
     unsigned char* ring = smem + warp * STAGES * GROUP;
     auto fetch = [&](int c, int s) {
         if (lane == 0 && c < c1) {
@@ -1090,9 +1093,9 @@ __global__ void __launch_bounds__(kFewWarps * 32) kvb_rows_mass_few(const KvbAtt
             bulk_g2s(ring + s * GROUP, src + (int64_t)c * GROUP, GROUP, &full[warp][s]);
         }
     };
-    // lane 8 x + i: row i of the group, its maximum, 1 / sum and last visible token
+    // lane STEP x + i: row i of the group, its maximum, 1 / sum and last visible token
     auto load_stat = [&](int c, int* lim) {
-        const int f = c * 8 + (lane & 7), i = f / G;
+        const int f = c * STEP + (lane & (STEP - 1)), i = f / G;
         *lim = f < rows ? sp.p + i : -1;
         return f < rows ? stats[(int64_t)(sp.r0 + i) * a.heads + h * G + (f - i * G)] : make_float2(0.0f, 0.0f);
     };
@@ -1111,28 +1114,33 @@ __global__ void __launch_bounds__(kFewWarps * 32) kvb_rows_mass_few(const KvbAtt
         st_next = load_stat(c + kFewWarps, &lim_next);
         if (!mbar_wait(&full[warp][s], phase) && lane == 0) atomicOr(&g_kvb_rows_errors, kErrWait);
         const unsigned char* q = ring + s * GROUP;
-        float z[TG][4], fq[2];
-        mass_scores<HD, Q2>(q + g * RS + 16 * t, k, z);
+        float z[STEP / 8][TG][4], fq[STEP / 8][2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) fq[e] = *reinterpret_cast<const float*>(q + (2 * t + e) * RS + (RS - 16));
+        for (int i = 0; i < STEP / 8; ++i) {
+            mass_scores<HD, Q2>(q + (8 * i + g) * RS + 16 * t, k, z[i]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) fq[i][e] = *reinterpret_cast<const float*>(q + (8 * i + 2 * t + e) * RS + (RS - 16));
+        }
         __syncwarp();                            // the stage is read
         fetch(c + STAGES * kFewWarps, s);
         if (++s == STAGES) s = 0, phase ^= 1;
-        // columns: rows 8 c + 2 t + e
-        const bool cut = sp.p + c * 8 / G < t0 + TOK - 1 || c * 8 + 7 >= rows;       // some row does not see every token
+        const bool cut = sp.p + c * STEP / G < t0 + TOK - 1 || (c + 1) * STEP > rows;    // some row does not see every token
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const float mx = __shfl_sync(0xffffffffu, st.x, 2 * t + e), inv = __shfl_sync(0xffffffffu, st.y, 2 * t + e);
-            const int last = __shfl_sync(0xffffffffu, lim, 2 * t + e);
+        for (int i = 0; i < STEP / 8; ++i)
 #pragma unroll
-            for (int j = 0; j < TG; ++j)
+            for (int e = 0; e < 2; ++e) {        // column 2 t + e: row STEP c + 8 i + 2 t + e
+                const int from = 8 * i + 2 * t + e;
+                const float mx = __shfl_sync(0xffffffffu, st.x, from), inv = __shfl_sync(0xffffffffu, st.y, from);
+                const int last = cut ? __shfl_sync(0xffffffffu, lim, from) : 0;
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    float w = ex2(fmaf(z[j][2 * r + e], sk[j] * fq[e], -mx)) * inv;
-                    if (cut && t0 + 16 * j + 8 * r + g > last) w = 0.0f;
-                    sum[j][r] += w;
-                }
-        }
+                for (int j = 0; j < TG; ++j)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        float w = ex2(fmaf(z[i][j][2 * r + e], sk[j] * fq[i][e], -mx)) * inv;
+                        if (cut && t0 + 16 * j + 8 * r + g > last) w = 0.0f;
+                        sum[j][r] += w;
+                    }
+            }
     }
 #pragma unroll
     for (int j = 0; j < TG; ++j)
