@@ -520,7 +520,8 @@ typedef struct {
  * s' = max(s, max|new| * F(1/127)) (s = 0 without older tokens in it), new
  * codes = rint(x / s'), older codes = rint((q * s) / s') when s' grew; a block
  * that holds only zeros has scale 0. NaN is written as 0, an infinity as the
- * largest finite value. */
+ * largest finite value. The slot then ends with its last row: what it held behind
+ * it is not rescaled and does not count any more. */
 int w8a8_kvb_append(const W8A8KvBlocks* cache, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                     int dtype, int rows, const int32_t* pos, const int32_t* start, void* stream);
 

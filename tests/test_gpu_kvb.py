@@ -493,7 +493,8 @@ def test_torch_ops():
     (12, 1, 208, 16, "bf16", 90, 96, True),
     (4, 2, 64, 128, "fp32", 1, 20096, True),
     (2, 1, 128, 128, "fp16", 2, 16512, False),
-    (4, 2, 128, 64, "fp32", 2, 4160, True)])
+    (4, 2, 128, 64, "fp32", 2, 4160, True),
+    (2, 1, 32, 16, "fp32", 700, 48, True)])
 def test_step_attention_of_many_slots_and_long_ones(heads, kv_heads, hd, block, dt, S, cap, mass):
     """Sequences of every length up to the capacity, idle ones between them."""
     rng = np.random.default_rng(heads * hd + S)
@@ -519,7 +520,7 @@ def test_step_attention_of_many_slots_and_long_ones(heads, kv_heads, hd, block, 
 
 @pytest.mark.parametrize("heads,kv_heads,hd,block,dt,S,cap", [
     (4, 2, 64, 64, "fp32", 160, 128), (6, 2, 128, 32, "bf16", 150, 160), (3, 3, 80, 16, "fp32", 110, 144),
-    (2, 1, 256, 64, "fp16", 80, 256)])
+    (2, 1, 256, 64, "fp16", 80, 256), (2, 1, 32, 16, "fp32", 700, 48)])
 def test_prompt_attention_of_many_slots(heads, kv_heads, hd, block, dt, S, cap):
     """Prompts of a few rows each, idle and empty ones between them."""
     rng = np.random.default_rng(heads * hd + S)

@@ -496,7 +496,8 @@ def kvb_append(k, v, cache, pos, start=None):
     """Rows k, v [rows, kv_heads, head_dim] into the cache: slot b's rows
     start[b] .. start[b + 1] - 1 (start None: row b) at positions pos[b] on
     (negative: an idle slot). A block's scale grows with its largest value; its
-    older codes are rescaled with it."""
+    older codes are rescaled with it. The slot ends with its last row: tokens it
+    held behind it are lost."""
     c, dev = _kvb(cache)
     dt, ks = _kvb_rows(k, c.kv_heads, c.head_dim, dev, "k")
     dv, vs = _kvb_rows(v, c.kv_heads, c.head_dim, dev, "v")
@@ -575,8 +576,8 @@ def _kvb_attn(q, cache, pos, start, scale, mass, out, scratch):
 def kvb_attn(q, cache, pos, scale=None, mass=None, out=None, scratch=None):
     """Decode attention over the cache: row b of q [slots, heads, head_dim]
     attends slot b's tokens 0 .. pos[b] (its own appended before); a negative
-    pos gives a zero row. scale: 1 / sqrt(head_dim) by default. mass (fp32
-    [slots, kv_heads, capacity]): each token's probabilities, summed over the
+    pos gives a zero row, a NaN or an infinity in a head's query NaN. scale:
+    1 / sqrt(head_dim) by default. mass (fp32 [slots, kv_heads, capacity]): each token's probabilities, summed over the
     query heads of its KV head, are added to it. scratch: kvb_attn_scratch()
     bytes of this call's own, or None to take them from torch's allocator."""
     return _kvb_attn(q, cache, pos, None, scale, mass, out, scratch)
