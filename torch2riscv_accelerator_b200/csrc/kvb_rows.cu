@@ -29,12 +29,14 @@
 // exponential, with the lazily moved references of the one-row kernel
 // (kvb_attn.cu), so that the accumulator is rescaled rarely.
 //
-// Bound by two chains of about 3,700 cycles a tile of 128 rows x 128 tokens that run
-// beside each other: the products' thread (2,048 cycles of products for fp32, the
-// rest hand-overs) and the softmax warps (wait, read 64 scores, exponentials, write
-// the weights). 8,192 causal rows, 16 heads on 8 KV heads of 128, fp32: 610 us, 0.45
+// Bound by two chains that run beside each other: the softmax warps (wait, read 64
+// scores, exponentials, write the weights; two warps a scheduler, half of all issue
+// slots) and the products' thread (for fp32 2,048 cycles of products a tile, the rest
+// hand-overs). 8,192 causal rows, 16 heads on 8 KV heads of 128, fp32: 610 us, 0.45
 // PFLOP/s of the formula's operations and 0.9 of those done (hi and lo); the tensor
-// pipe is active 41 % of the time, 3 % of the DRAM's rate is used.
+// pipe is active 41 % of the time, 3 % of the DRAM's rate is used. Four softmax
+// threads a row (24 warps) took 7 to 11 % longer; two groups that take turns on the
+// tiles with an accumulator each (64-channel heads) 35 %.
 #include <type_traits>
 
 #include "kvb.cuh"
