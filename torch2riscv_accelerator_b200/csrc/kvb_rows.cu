@@ -10,7 +10,7 @@
 // tiles of BN. All units' tiles, in order, are dealt out to the SMs in equal
 // contiguous shares (causal units differ in length, and few rows must still
 // fill the GPU); a CTA leaves at most two partial units, which kvb_rows_finish
-// joins. kvb_rows_plan lists the units, since lengths are device data.
+// joins. plan_rows lists the units on the device, since lengths are device data.
 //
 // Warps of a CTA (one CTA an SM, all 512 TMEM columns):
 //   softmax   8 warps: a row's columns are split between two threads, which meet
@@ -70,7 +70,6 @@ constexpr int kFold = sizeof(T) == 4 ? 3 : 32;   // (16-bit outputs round by 2e-
 // queries and last outputs cost about as much as two tiles (by tiles alone the
 // CTA with a causal prompt's short units took 20 % longer than the others).
 constexpr int kUnitCost = 2;
-constexpr int kPlanThreads = 256;                 // (1,024: 1.8 us longer, in the scans)
 constexpr int kFinishThreads = 256;
 
 template <int HD>
@@ -118,9 +117,10 @@ __host__ __device__ inline int64_t max_units(const KvbCache& c, int heads, int r
 
 __device__ __forceinline__ int live_rows(const KvbSpan& s, int cap) { return s.p < 0 ? 0 : max(min(s.n, cap - s.p), 0); }
 
-// exclusive scan over the CTA's kPlanThreads threads; *sum the total
+// exclusive scan over the CTA's NT threads; *sum the total
+template <int NT>
 __device__ __forceinline__ int block_scan(int x, int* sum) {
-    __shared__ int w[kPlanThreads / 32];
+    __shared__ int w[NT / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     int upto = x;
 #pragma unroll
@@ -132,7 +132,7 @@ __device__ __forceinline__ int block_scan(int x, int* sum) {
     __syncthreads();
     int before = 0, all = 0;
 #pragma unroll
-    for (int i = 0; i < kPlanThreads / 32; ++i) {
+    for (int i = 0; i < NT / 32; ++i) {
         if (i < warp) before += w[i];
         all += w[i];
     }
@@ -141,16 +141,16 @@ __device__ __forceinline__ int block_scan(int x, int* sum) {
     return before + upto - x;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) kvb_rows_plan(const KvbAttnArgs a, RowsPlan plan, int bn, int most) {
-    pdl_wait();
-    pdl_trigger();
+// The plan, by one CTA of NT threads.
+template <int NT>
+__device__ __forceinline__ void plan_rows(const KvbAttnArgs& a, const RowsPlan& plan, int bn, int most) {
     const int tid = threadIdx.x, S = a.c.slots, G = a.heads / a.c.heads;
-    __shared__ int s_before[kPlanThreads];       // the first units' costs before them
+    __shared__ int s_before[NT];       // the first units' costs before them
     int units = 0, sum;
-    for (int b0 = 0; b0 < S; b0 += kPlanThreads) {
+    for (int b0 = 0; b0 < S; b0 += NT) {
         const int b = b0 + tid;
         const int n = b < S ? (live_rows(kvb_span(a.r, b), a.c.cap) * G + kRows - 1) / kRows : 0;
-        const int at = block_scan(n, &sum);
+        const int at = block_scan<NT>(n, &sum);
         if (b < S) plan.first[b] = units + at;
         units += sum;
     }
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kPlanThreads) kvb_rows_plan(const KvbAttnArgs 
     __syncthreads();
     units = min(units, most);                    // more only with offsets out of order: rows are then left out
     int total = 0;
-    for (int u0 = 0; u0 < units; u0 += kPlanThreads) {
+    for (int u0 = 0; u0 < units; u0 += NT) {
         const int u = u0 + tid;
         RowsUnit v{};
         if (u < units) {
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(kPlanThreads) kvb_rows_plan(const KvbAttnArgs 
             v.slot = b, v.m = u - plan.first[b], v.p = sp.p, v.r0 = sp.r0, v.rows = live_rows(sp, a.c.cap) * G;
             v.tiles = (sp.p + min(v.m * kRows + kRows - 1, v.rows - 1) / G) / bn + 1;
         }
-        v.before = total + block_scan(u < units ? v.tiles + kUnitCost : 0, &sum);
+        v.before = total + block_scan<NT>(u < units ? v.tiles + kUnitCost : 0, &sum);
         if (u < units) plan.unit[u] = v;
         if (u0 == 0) s_before[tid] = v.before;
         total += sum;
@@ -182,27 +182,27 @@ __global__ void __launch_bounds__(kPlanThreads) kvb_rows_plan(const KvbAttnArgs 
     __syncthreads();
     // the shares, and where they begin (searched here once: a search through
     // global memory in every CTA of two kernels took 1.5 us in each)
-    if (tid < kSms) {
+    for (int c = tid; c < kSms; c += NT) {
         RowsShare w{};
         w.join = -1;
         const int64_t all = (int64_t)total * a.c.heads, ctas = min(all, (int64_t)kSms);
-        if (tid < ctas) {
-            w.lo = div64(all * tid, ctas), w.hi = div64(all * (tid + 1), ctas);
+        if (c < ctas) {
+            w.lo = div64(all * c, ctas), w.hi = div64(all * (c + 1), ctas);
             w.h = (int)div64(w.lo, total);
             const int at = (int)(w.lo - (int64_t)w.h * total);
             int u = 0, hi = units;               // the last unit that begins at or before `at`
             while (hi - u > 1) {
                 const int mid = (u + hi) >> 1;
-                if ((mid < kPlanThreads ? s_before[mid] : plan.unit[mid].before) <= at) u = mid;
+                if ((mid < NT ? s_before[mid] : plan.unit[mid].before) <= at) u = mid;
                 else hi = mid;
             }
             w.u = u;
-            const int64_t begin = (int64_t)w.h * total + (u < kPlanThreads ? s_before[u] : plan.unit[u].before);
+            const int64_t begin = (int64_t)w.h * total + (u < NT ? s_before[u] : plan.unit[u].before);
             const int64_t end = begin + kUnitCost + plan.unit[u].tiles;
-            if (w.lo > begin + kUnitCost && div64(all * (tid - 1), ctas) <= begin + kUnitCost)
+            if (w.lo > begin + kUnitCost && div64(all * (c - 1), ctas) <= begin + kUnitCost)
                 w.join = (int)div64(end * ctas - 1, all);
         }
-        plan.share[tid] = w;
+        plan.share[c] = w;
     }
 }
 
@@ -301,19 +301,72 @@ __device__ __forceinline__ float row_factor(uint32_t top, float scale, float* up
     return *bad ? NAN : fabsf(scale) * kLog2e * __int_as_float((127 - e) << 23);
 }
 
+// The plan alone: where the query rows need no preparation, or the slots are many.
+constexpr int kPlanThreads = 256;
+// A few slots: the plan in the queries' kernel, whose CTAs then each count the
+// slots (1 slot, 32 rows of 16 heads 14.9 -> 13.3 us and a launch less of the host;
+// 64 slots 37.3 -> 36.0, 128 slots 57.8 -> 58.7, 512 slots 204 -> 250).
+constexpr int kFoldSlots = 64;
+__global__ void __launch_bounds__(kPlanThreads) kvb_rows_plan(const KvbAttnArgs a, const RowsPlan plan, int bn, int most) {
+    pdl_wait();
+    pdl_trigger();
+    plan_rows<kPlanThreads>(a, plan, bn, most);
+}
+
 // The units' query rows as the products take them, 32 rows a CTA, a lane per 8
 // channels: halves in unit order, so that a stage of the main kernel's ring is
 // one run of memory. (Converted there, row by row, they cost each unit 12,000
 // cycles of cold code and scattered loads between two streams of products.)
+// With bn (tokens of a tile) the first CTA makes the plan and the others find
+// their unit by themselves; else the plan is there.
 template <int HD, typename T>
 __global__ void __launch_bounds__(HD / 8 * 32) kvb_rows_queries(const KvbAttnArgs a, const RowsPlan plan,
-                                                              unsigned char* out, int units) {
+                                                              unsigned char* out, int units, int bn) {
     pdl_wait();
     pdl_trigger();
     constexpr int RS = RowsCfg<HD>::qrow(sizeof(T)), LPR = HD / 8;       // bytes, lanes of a row
-    const int u = blockIdx.x / 4, part = blockIdx.x % 4, h = blockIdx.y, G = a.heads / a.c.heads;
-    if (u >= plan.head[1]) return;
-    const RowsUnit v = plan.unit[u];
+    const int x0 = (int)blockIdx.x - (bn > 0), u = x0 / 4, part = x0 % 4, h = blockIdx.y, G = a.heads / a.c.heads;
+    if (x0 < 0) {
+        if (h == 0) plan_rows<HD / 8 * 32>(a, plan, bn, units);
+        return;
+    }
+    __shared__ int s_slot, s_m;
+    if (bn == 0) {
+        if (threadIdx.x == 0) {
+            const bool ok = u < plan.head[1];
+            s_slot = ok ? plan.unit[u].slot : -1, s_m = ok ? plan.unit[u].m : 0;
+        }
+    } else if (threadIdx.x < 32) {               // unit u: the slots' units counted through
+        const int lane = threadIdx.x;
+        if (lane == 0) s_slot = -1;
+        __syncwarp();
+        int before = 0;
+        for (int b0 = 0; b0 < a.c.slots && before <= u; b0 += 128) {     // four slots a lane in flight
+            int n[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int b = b0 + 32 * i + lane;
+                n[i] = b < a.c.slots ? (live_rows(kvb_span(a.r, b), a.c.cap) * G + kRows - 1) / kRows : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                int upto = n[i];
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int o = __shfl_up_sync(0xffffffffu, upto, d);
+                    if (lane >= d) upto += o;
+                }
+                const int at = u - before - (upto - n[i]);
+                if (at >= 0 && at < n[i]) s_slot = b0 + 32 * i + lane, s_m = at;
+                before += __shfl_sync(0xffffffffu, upto, 31);
+            }
+        }
+    }
+    __syncthreads();
+    if (s_slot < 0) return;
+    const KvbSpan sp = kvb_span(a.r, s_slot);
+    RowsUnit v{};
+    v.m = s_m, v.r0 = sp.r0, v.rows = live_rows(sp, a.c.cap) * G;
     const int r = threadIdx.x / LPR, d = threadIdx.x % LPR * 8, f = v.m * kRows + part * 32 + r;
     float x[8];
     uint32_t top = 0u;
@@ -1208,14 +1261,19 @@ cudaError_t rows_launch(const KvbAttnArgs& a, cudaStream_t st) {
                         reinterpret_cast<RowsShare*>(s + L.share)};
     float* parts = reinterpret_cast<float*>(s + L.parts);
     float2* stats = a.mass ? reinterpret_cast<float2*>(s + L.stats) : nullptr;
-    cudaError_t e = launch_k(kvb_rows_plan, dim3(1), dim3(kPlanThreads), 0, st, a, plan, C::BN, units);
-    if (e != cudaSuccess) return e;
     unsigned char* queries = reinterpret_cast<unsigned char*>(s + L.queries);
-    if (C::QT || a.mass) {
+    const bool prepared = C::QT || a.mass, fold = prepared && a.c.slots <= kFoldSlots;
+    if (!fold) {
+        const cudaError_t e = launch_k(kvb_rows_plan, dim3(1), dim3(kPlanThreads), 0, st, a, plan, C::BN, units);
+        if (e != cudaSuccess) return e;
+    }
+    cudaError_t e = cudaSuccess;
+    if (prepared) {
         const auto prep = a.type == KVB_F32    ? kvb_rows_queries<HD, float>
                           : a.type == KVB_BF16 ? kvb_rows_queries<HD, __nv_bfloat16>
                                                : kvb_rows_queries<HD, __half>;
-        e = launch_k(prep, dim3(units * 4, a.c.heads), dim3(HD / 8 * 32), 0, st, a, plan, queries, units);
+        e = launch_k(prep, dim3(units * 4 + fold, a.c.heads), dim3(HD / 8 * 32), 0, st, a, plan, queries, units,
+                     fold ? C::BN : 0);
         if (e != cudaSuccess) return e;
     }
     const auto kern = a.type == KVB_F32    ? kvb_rows_kernel<HD, float>
