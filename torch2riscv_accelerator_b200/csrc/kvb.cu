@@ -415,7 +415,9 @@ cudaError_t launch_kvb_read(const KvbReadArgs& a, cudaStream_t st) {
 
 cudaError_t launch_kvb_evict(const KvbEvictArgs& a, cudaStream_t st) {
     const int cached = a.src.cap < kSelKeys ? a.src.cap : kSelKeys;
-    cudaError_t e = cudaFuncSetAttribute(kvb_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelKeys * 4);
+    cudaError_t e = cudaSuccess;
+    if (cached * 4 > 40960)                      // what a CTA may have anyway, less the static arrays
+        e = cudaFuncSetAttribute(kvb_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelKeys * 4);
     if (e != cudaSuccess) return e;
     e = launch_k(kvb_select_kernel, dim3(a.src.heads, a.src.slots), dim3(kSelThreads), (size_t)cached * 4, st, a, cached);
     if (e != cudaSuccess) return e;

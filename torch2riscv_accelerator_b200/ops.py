@@ -525,7 +525,7 @@ def kvb_read(cache, pos, start, rows, dtype=F32, k=None, v=None):
                               t.dtype != dtype):
             raise ValueError(f"{name}: a contiguous {dtype} {(rows, H, D)} tensor is required")
     k = torch.empty_strided((rows, H, D), (H * D, D, 1), dtype=dtype, device=dev) if k is None else k
-    v = torch.empty_strided((rows, H, D), (H * D, D, 1), dtype=dtype, device=dev) if v is None else v
+    v = torch.empty_like(k) if v is None else v
     _kvb_call("w8a8_kvb_read", dev, ctypes.byref(c), rows, pos.data_ptr(),
               None if start is None else start.data_ptr(), k.data_ptr(), v.data_ptr(), _KVB_TYPES[dtype])
     return k, v
