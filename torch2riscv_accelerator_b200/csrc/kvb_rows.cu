@@ -801,9 +801,7 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                 tc_fence_before();
                 mbar_arrive(&p_full[tl & 1]);
             }
-            // the unit's rows
-            wait(&o_full, sn & 1);
-            tc_fence_after();
+            // the unit's rows; what needs no outputs while the last products run
             barrier_any(1, C::SOFT, false);      // s_half is free
             s_half[w][row] = l;
             named_barrier_sync(2, C::SOFT);
@@ -812,6 +810,8 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
             const float fo = ex2(lr - kWeightLog) * (whole ? 1.0f / l : 1.0f);
             const int64_t orow = (int64_t)(seg.r0 + f / G) * a.heads + seg.h * G + f % G;
             float* pt = parts + ((int64_t)blockIdx.x * 2 + (seg.j == 0)) * C::PART;
+            wait(&o_full, sn & 1);
+            tc_fence_after();
 #pragma unroll 1
             for (int c = w * (HD / 2); c < (w + 1) * (HD / 2); c += 16) {
                 int o[16];
