@@ -350,6 +350,7 @@ __global__ void __launch_bounds__(HD / 8 * 32) kvb_rows_queries(const KvbAttnArg
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
+                if (b0 + 32 * i >= a.c.slots) break;
                 int upto = n[i];
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) {
