@@ -520,7 +520,8 @@ def test_step_attention_of_many_slots_and_long_ones(heads, kv_heads, hd, block, 
 
 @pytest.mark.parametrize("heads,kv_heads,hd,block,dt,S,cap", [
     (4, 2, 64, 64, "fp32", 160, 128), (6, 2, 128, 32, "bf16", 150, 160), (3, 3, 80, 16, "fp32", 110, 144),
-    (2, 1, 256, 64, "fp16", 80, 256), (2, 1, 32, 16, "fp32", 700, 48)])
+    (2, 1, 256, 64, "fp16", 80, 256), (2, 1, 32, 16, "fp32", 700, 48),
+    (24, 12, 48, 16, "bf16", 48, 64)])
 def test_prompt_attention_of_many_slots(heads, kv_heads, hd, block, dt, S, cap):
     """Prompts of a few rows each, idle and empty ones between them."""
     rng = np.random.default_rng(heads * hd + S)

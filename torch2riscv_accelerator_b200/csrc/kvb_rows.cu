@@ -307,13 +307,14 @@ constexpr int kPlanThreads = 256;
 // slots (1 slot, 32 rows of 16 heads 14.9 -> 13.3 us and a launch less of the host;
 // 64 slots 37.3 -> 36.0, 128 slots 57.8 -> 58.7, 512 slots 204 -> 250).
 constexpr int kFoldSlots = 64;
+constexpr int kFullUnits = 4 * kSms;
 __global__ void __launch_bounds__(kPlanThreads) kvb_rows_plan(const KvbAttnArgs a, const RowsPlan plan, int bn, int most) {
     pdl_wait();
     pdl_trigger();
     plan_rows<kPlanThreads>(a, plan, bn, most);
 }
 
-// The units' query rows as the products take them, 32 rows a CTA, a lane per 8
+// The units' query rows as the products take them, 32 rows at a time, a lane per 8
 // channels: halves in unit order, so that a stage of the main kernel's ring is
 // one run of memory. (Converted there, row by row, they cost each unit 12,000
 // cycles of cold code and scattered loads between two streams of products.)
@@ -321,11 +322,11 @@ __global__ void __launch_bounds__(kPlanThreads) kvb_rows_plan(const KvbAttnArgs 
 // their unit by themselves; else the plan is there.
 template <int HD, typename T>
 __global__ void __launch_bounds__(HD / 8 * 32) kvb_rows_queries(const KvbAttnArgs a, const RowsPlan plan,
-                                                              unsigned char* out, int units, int bn) {
+                                                              unsigned char* out, int units, int bn, int per) {
     pdl_wait();
     pdl_trigger();
     constexpr int RS = RowsCfg<HD>::qrow(sizeof(T)), LPR = HD / 8;       // bytes, lanes of a row
-    const int x0 = (int)blockIdx.x - (bn > 0), u = x0 / 4, part = x0 % 4, h = blockIdx.y, G = a.heads / a.c.heads;
+    const int x0 = ((int)blockIdx.x - (bn > 0)) * per, u = x0 / 4, h = blockIdx.y, G = a.heads / a.c.heads;
     if (x0 < 0) {
         if (h == 0) plan_rows<HD / 8 * 32>(a, plan, bn, units);
         return;
@@ -366,34 +367,35 @@ __global__ void __launch_bounds__(HD / 8 * 32) kvb_rows_queries(const KvbAttnArg
     __syncthreads();
     if (s_slot < 0) return;
     const KvbSpan sp = kvb_span(a.r, s_slot);
-    RowsUnit v{};
-    v.m = s_m, v.r0 = sp.r0, v.rows = live_rows(sp, a.c.cap) * G;
-    const int r = threadIdx.x / LPR, d = threadIdx.x % LPR * 8, f = v.m * kRows + part * 32 + r;
-    float x[8];
-    uint32_t top = 0u;
+    const int rows = live_rows(sp, a.c.cap) * G, r = threadIdx.x / LPR, d = threadIdx.x % LPR * 8;
+    for (int part = x0 % 4; part < x0 % 4 + per; ++part) {
+        const int f = s_m * kRows + part * 32 + r;
+        float x[8];
+        uint32_t top = 0u;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.0f;
-    if (f < v.rows && d < a.c.hd)
-        kvb_load8<T>(static_cast<const T*>(a.q) + (int64_t)(v.r0 + f / G) * a.q_stride + (int64_t)(h * G + f % G) * a.c.hd + d, x);
+        for (int i = 0; i < 8; ++i) x[i] = 0.0f;
+        if (f < rows && d < a.c.hd)
+            kvb_load8<T>(static_cast<const T*>(a.q) + (int64_t)(sp.r0 + f / G) * a.q_stride + (int64_t)(h * G + f % G) * a.c.hd + d, x);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
 #pragma unroll
-    for (int i = 1; i < LPR; i <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, i));
-    float up;
-    bool bad;
-    const float factor = row_factor(top, a.scale, &up, &bad);
-    uint32_t hi[4], lo[4];
+        for (int i = 1; i < LPR; i <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, i));
+        float up;
+        bool bad;
+        const float factor = row_factor(top, a.scale, &up, &bad);
+        uint32_t hi[4], lo[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float y0 = bad ? 0.0f : x[2 * i] * up, y1 = bad ? 0.0f : x[2 * i + 1] * up;
-        const __half2 h2 = __floats2half2_rn(y0, y1);
-        const float2 b2 = __half22float2(h2);
-        hi[i] = bits(h2), lo[i] = bits(__floats2half2_rn(y0 - b2.x, y1 - b2.y));
+        for (int i = 0; i < 4; ++i) {
+            const float y0 = bad ? 0.0f : x[2 * i] * up, y1 = bad ? 0.0f : x[2 * i + 1] * up;
+            const __half2 h2 = __floats2half2_rn(y0, y1);
+            const float2 b2 = __half22float2(h2);
+            hi[i] = bits(h2), lo[i] = bits(__floats2half2_rn(y0 - b2.x, y1 - b2.y));
+        }
+        unsigned char* to = out + ((((int64_t)h * units + u) * 4 + part) * 32 + r) * RS;
+        *reinterpret_cast<uint4*>(to + d * 2) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if (sizeof(T) == 4) *reinterpret_cast<uint4*>(to + HD * 2 + d * 2) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if (d == 0) *reinterpret_cast<float*>(to + HD * (int)sizeof(T)) = factor;
     }
-    unsigned char* to = out + ((((int64_t)h * units + u) * 4 + part) * 32 + r) * RS;
-    *reinterpret_cast<uint4*>(to + d * 2) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    if (sizeof(T) == 4) *reinterpret_cast<uint4*>(to + HD * 2 + d * 2) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    if (d == 0) *reinterpret_cast<float*>(to + HD * (int)sizeof(T)) = factor;
 }
 
 // HD: padded head size. Queries enter as hi + lo for fp32 (Q2), the weights
@@ -1273,8 +1275,10 @@ cudaError_t rows_launch(const KvbAttnArgs& a, cudaStream_t st) {
         const auto prep = a.type == KVB_F32    ? kvb_rows_queries<HD, float>
                           : a.type == KVB_BF16 ? kvb_rows_queries<HD, __nv_bfloat16>
                                                : kvb_rows_queries<HD, __half>;
-        e = launch_k(prep, dim3(units * 4 + fold, a.c.heads), dim3(HD / 8 * 32), 0, st, a, plan, queries, units,
-                     fold ? C::BN : 0);
+        // a unit a CTA once that fills the SMs (3,000 units of 64 channels 25.7 -> 19.4 us), else a quarter
+        const int per = (int64_t)units * a.c.heads >= kFullUnits ? 4 : 1;
+        e = launch_k(prep, dim3(units * (4 / per) + fold, a.c.heads), dim3(HD / 8 * 32), 0, st, a, plan, queries, units,
+                     fold ? C::BN : 0, per);
         if (e != cudaSuccess) return e;
     }
     const auto kern = a.type == KVB_F32    ? kvb_rows_kernel<HD, float>
