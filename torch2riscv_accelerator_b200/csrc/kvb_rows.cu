@@ -769,6 +769,7 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                             for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * eo);
                             tmem_st16(to + c * 16, v);
                         }
+                        tmem_st_wait();          // a tile that moves the accumulator out reads these columns below
                     }
                     l *= el, acc_f *= eo, m = xm, lr = xr;
                 }
