@@ -1,78 +1,14 @@
 """Prompt attention over the block-scaled 8-bit KV cache where one CTA takes many
 tiles of one unit: accumulators that are moved out and begun anew, rescaled on
 the way, scores and V scales that jump in the middle of a unit. Compared with
-float64 on the same device.
-
-The bound, from the kernel's arithmetic, all of it over the tokens that a row
-sees. A query enters with an error of at most 2^-22 of itself, the products are
-exact and summed in fp32, the result is scaled and taken from the maximum (two
-roundings): |dz| <= (2^-21 + (D / 16 + 2) 2^-23) max_t sum|q k_t| scale. A weight
-is off by 2 |dz|, and so is the sum that divides it; the exponential, V's scale in
-it and its rounding to 21 bits add 2^-20. The tensor cores round each product's
-running sum towards zero by at most 2^-23: two products for 16 tokens of the
-FOLD tiles between two move-outs, 2 * FOLD * 128 / 16 of them (fewer where a tile
-has 64 tokens); the moved-out sums and the weights' sum are added in fp32 over n
-tokens in at most n / 32 + 16 steps of 2^-24. All are relative to sum p |v|:
-|do| <= (4 |dz| + 2^-20 + 16 FOLD 2^-23 + (n / 32 + 16) 2^-24) sum p |v|, and half
-a step of the output's type relative to it."""
+float64 on the same device (the bound: kvb_ref64.py)."""
 import pytest
 import torch
 
+from kvb_ref64 import DEV, TYPES, attend, check, dz_of, i32, make_cache
 from torch2riscv_accelerator_b200 import ops
 
 pytestmark = pytest.mark.gpu
-DEV = "cuda"
-TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
-FOLD = {"fp32": 3, "bf16": 32, "fp16": 32}
-
-
-def i32(a):
-    return torch.tensor(list(a), dtype=torch.int32, device=DEV)
-
-
-def dz_of(zabs, hd):
-    return (2.0 ** -21 + (hd / 16 + 2) * 2.0 ** -23) * zabs
-
-
-def attend(q, cache, b, p, rows, h, scale=None):
-    """Rows (indices i at positions p + i) of one slot and KV head in float64: q [n, G, D] of these rows -> their
-    outputs, probabilities [n, G, T], sum p |v|, max sum|q k| scale over the tokens that each sees, and what subnormal
-    halves may lose."""
-    k, ks, v, vs = cache
-    B, D = k.shape[2] // ks.shape[2], k.shape[3]
-    T = p + int(rows.max()) + 1
-    of = torch.arange(T, device=DEV) // B
-    sv = vs[b, h].double()[of]
-    kd, vd = k[b, h, :T].double() * ks[b, h].double()[of, None], v[b, h, :T].double() * sv[:, None]
-    hidden = torch.arange(T, device=DEV) > (p + rows).view(-1, 1, 1)
-    q = q.double()
-    scale = D ** -0.5 if scale is None else scale
-    w = torch.softmax((q @ kd.T * scale).masked_fill(hidden, -float("inf")), -1)
-    zabs = ((q.abs() @ kd.abs().T) * abs(scale)).masked_fill(hidden, 0.0).amax(-1, keepdim=True)
-    most = sv.expand_as(w).masked_fill(hidden, 0.0).amax(-1, keepdim=True)
-    lost = torch.minimum(2 * w * sv, 2.0 ** -31 * most).masked_fill(hidden, 0.0) @ v[b, h, :T].double().abs()
-    return w @ vd, w, w @ vd.abs(), zabs, lost
-
-
-def check(got, want, vabs, zabs, lost, n, hd, dt):
-    rel = 4 * dz_of(zabs, hd) + 2.0 ** -20 + 16 * FOLD[dt] * 2.0 ** -23 + (n / 32 + 16) * 2.0 ** -24
-    t = torch.finfo(TYPES[dt])
-    tol = rel * vabs + t.eps / 2 * want.abs() + lost + t.smallest_normal * t.eps / 2
-    off = (got.double() - want).abs()
-    assert got.isfinite().all()
-    assert (off <= tol).all(), (off.max().item(), tol.flatten()[(off - tol).argmax()].item(), (off / tol).max().item())
-
-
-def make_cache(g, S, H, cap, hd, block, k_std=None, v_scale=None):
-    """Codes over the whole range; k_std, v_scale [H, blocks]: a head's scores' spread for unit queries, its V scales."""
-    code = lambda: (torch.randn(S, H, cap, hd, generator=g, device=DEV) * 36).round().clamp(-127, 127).to(torch.int8)
-    nb = cap // block
-    plain = torch.exp(0.25 * torch.randn(S, H, nb, generator=g, device=DEV)) / 36
-    ks = plain if k_std is None else (k_std / 36).expand(S, H, nb).contiguous()
-    vs = torch.exp(0.25 * torch.randn(S, H, nb, generator=g, device=DEV)) / 36
-    if v_scale is not None:
-        vs = vs * v_scale
-    return ops.KvBlocks(code(), ks.float(), code(), vs.float().contiguous())
 
 
 def rising(H, cap, block, every):

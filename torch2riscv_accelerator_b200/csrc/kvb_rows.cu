@@ -25,9 +25,11 @@
 //             TMEM, written over S: hi in columns 0-7, lo in 8-15 of every 16;
 //             V as it lies, its rows being the contraction).
 // Block scales do not touch the codes: K's multiplies the scores of its 16
-// columns, V's goes into the weights, exp(z - m) sv / sv_ref 2^7 by one
-// exponential, with the lazily moved references of the one-row kernel
-// (kvb_attn.cu), so that the accumulator is rescaled rarely.
+// columns, V's goes into the weights, exp(z - m) sv / 2^lr 2^7 by one
+// exponential. m is the row's largest score and 2^lr its largest exp(z - m) sv,
+// both over the tokens that it sees and lazily moved, so that the accumulator is
+// rescaled rarely; blocks that the row does not see, or gives no weight, leave the
+// others' halves their bits, however large their values are.
 //
 // Bound by two chains that run beside each other: the softmax warps (wait, read 64
 // scores, exponentials, write the weights; two warps a scheduler, half of all issue
@@ -58,7 +60,10 @@ namespace {
 constexpr int kRows = 128;                       // rows of a unit (TMEM lanes)
 constexpr int kSms = 148;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLazyScore = 6.0f, kLazyLog = 2.0f, kWeightLog = 7.0f;   // log2: see kvb_attn.cu
+// log2 of: how far a score may pass m, a weight its reference (2^15 is the most that a half should hold),
+// and the reference's place
+constexpr float kLazyScore = 6.0f, kLazyWeight = 8.0f, kWeightLog = 7.0f;
+constexpr float kLeastLog = -126.0f;             // the least reference: 2^lr is a normal number
 constexpr unsigned int kErrWait = 256u;          // error bit 8: a pipeline wait gave up
 // The tensor cores round each product's running sum towards zero: an accumulator
 // is moved out and begun anew every kFold tiles (fp32, relative error of an output over
@@ -280,6 +285,19 @@ __device__ __noinline__ void wait_long(uint64_t* bar, uint32_t parity, int* dead
     }
 }
 
+// log2 of a scale, its exponent and its mantissa (in [1, 2)) apart: off by 2^-22 and the
+// rounding of the sum (for scales from 2^-16 to 2^16 2^-21, at most 2^-18), where the
+// logarithm of the whole may be off by 2 ulp. (As an integer with 22 bits behind the point
+// it would keep 2^-22 at any size: 4 % of the time, in registers that spill.)
+__device__ __forceinline__ float log2_scale(float s) {
+    const bool small = s < 1.17549435e-38f;      // subnormal
+    const uint32_t u = __float_as_uint(small ? s * 16777216.0f : s);
+    const float y = (float)((int)(u >> 23) - (small ? 151 : 127)) + __log2f(__uint_as_float((u & 0x7fffffu) | 0x3f800000u));
+    return u ? y : -INFINITY;
+}
+
+__device__ __forceinline__ float exp2_int(float e) { return __int_as_float((127 + (int)e) << 23); }   // -126 .. 127
+
 // Barrier `id` among n threads, and whether x holds for any of them.
 __device__ __forceinline__ bool barrier_any(int id, int n, bool x) {
     uint32_t r;
@@ -420,7 +438,8 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
     __shared__ uint32_t tmem_base;
     __shared__ int dead;
     __shared__ float s_row[2][kRows];            // score factors of the unit's rows
-    __shared__ float s_half[2][kRows];           // a row's half, for its other thread: largest score, at the end the sum
+    // a row's half, for its other thread: largest score (at the end the sum), largest log2 of a weight
+    __shared__ float s_half[2][kRows], s_top[2][kRows];
     const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
     const int hd = a.c.hd, G = a.heads / a.c.heads;
     if (tid == 0) {
@@ -661,7 +680,7 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
             const bool live = f < seg.rows;
             const int lim = seg.p + (live ? f : seg.rows - 1) / G;       // the last token that the row sees
             const int all_see = seg.p + seg.m * kRows / G;               // ... that every row sees
-            float m = -INFINITY, l = 0.0f, lr = -200.0f;                 // lr: log2 of the V scale reference
+            float m = -INFINITY, l = 0.0f, lr = 0.0f;                    // lr: an integer
             float acc_f = 1.0f;                  // rescaling of the moved-out accumulator since it was moved
             float4* acc = reinterpret_cast<float4*>(accs + (int64_t)blockIdx.x * C::ACC) + w * (HD / 8) * kRows + row;
             // scales of a tile's 16-token groups, loaded a tile ahead: lanes 0-15
@@ -676,26 +695,31 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
             for (int jj = 0; jj < seg.n; ++jj) {
                 const int tl = J + jj, t0 = (seg.j + jj) * BN;
                 const uint32_t ts = tmem + lanes + (tl & 1) * BN + w * HC;
+                // this half's groups: K's scales, log2 of V's; ready before the scores are
+                const float scale = lane < 16 ? coming : log2_scale(coming);
+                if (jj + 1 < seg.n) coming = scale_of(t0 + BN);
+                float fk[NG / 2], fv[NG / 2];
+#pragma unroll
+                for (int g = 0; g < NG / 2; ++g) {
+                    fk[g] = __shfl_sync(0xffffffffu, scale, w * (NG / 2) + g);
+                    fv[g] = __shfl_sync(0xffffffffu, scale, 16 + w * (NG / 2) + g);
+                }
+                float most = fv[0];
+#pragma unroll
+                for (int g = 1; g < NG / 2; ++g) most = fmaxf(most, fv[g]);
                 wait(&s_full[tl & 1], (tl >> 1) & 1);
                 tc_fence_after();
                 const float qs = s_row[sn & 1][row];
-                const float scale = lane < 16 ? coming : __log2f(fmaxf(coming, 1.17549435e-38f));
-                if (jj + 1 < seg.n) coming = scale_of(t0 + BN);
-                float fk[NG / 2], fv[NG / 2];    // this half's groups: score factors, log2 of V's scales
 #pragma unroll
-                for (int g = 0; g < NG / 2; ++g) {
-                    fk[g] = __shfl_sync(0xffffffffu, scale, w * (NG / 2) + g) * qs;
-                    fv[g] = __shfl_sync(0xffffffffu, scale, 16 + w * (NG / 2) + g);
-                }
-                const float lv_here = lane >= 16 ? scale : -200.0f;
+                for (int g = 0; g < NG / 2; ++g) fk[g] *= qs;            // score factors
                 // the scores are read once (a TMEM load waits long while products run)
                 uint32_t v[HC];
 #pragma unroll
                 for (int c = 0; c < HC / 32; ++c) tmem_ld32(ts + c * 32, v + c * 32);
                 tmem_ld_wait();
+                float z[NG / 2], x = -INFINITY;  // the groups' largest scores, and theirs
                 // seen: how many of this thread's columns the row sees, where some row does not see all
                 auto largest = [&](auto cut, int seen) {
-                    float x = -INFINITY;
 #pragma unroll
                     for (int g = 0; g < HC / 16; ++g) {
                         if (cut) {
@@ -708,15 +732,15 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                         for (int i = 1; i < 15; i += 2)
                             y = fmaxf(fmaxf(y, __uint_as_float(v[16 * g + i])), __uint_as_float(v[16 * g + i + 1]));
                         y = fmaxf(y, __uint_as_float(v[16 * g + 15]));
-                        if (y != -INFINITY) x = fmaxf(x, y * fk[g]);
+                        z[g] = y != -INFINITY ? y * fk[g] : y;
+                        x = fmaxf(x, z[g]);
                     }
-                    return x;
                 };
                 auto weights = [&](auto cut, int seen) {
 #pragma unroll
                     for (int g = 0; g < HC / 16; ++g) {
                         uint32_t p[16];          // hi, lo
-                        // 2^7 sv / sv_ref joins the exponent; the sum of the weights without it
+                        // 2^7 sv / 2^lr joins the exponent; the sum of the weights without it
                         const float lv = fmaxf(fv[g] - lr + kWeightLog, -40.0f), fz = fk[g], off = lv - m;
                         const uint64_t fz2 = pack2(fz, fz), off2 = pack2(off, off);
                         uint64_t sum = 0;
@@ -748,15 +772,23 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                 };
                 const bool cut = t0 + BN - 1 > all_see;
                 const int seen = lim + 1 - t0 - w * HC;
-                const float x = cut ? largest(std::true_type{}, seen) : largest(std::false_type{}, 0);
-                if (barrier_any(1, C::SOFT, x > m + kLazyScore || lv_here > lr + kLazyLog)) {
+                if (cut) largest(std::true_type{}, seen);
+                else largest(std::false_type{}, 0);
+                // (x - m + most is no less than what the reference goes by; all of it relative to a
+                // maximum, since scores may be so large that a scale is lost in them)
+                if (barrier_any(1, C::SOFT, x > m + kLazyScore || x - m + most > lr + kLazyWeight)) {
                     s_half[w][row] = x;
                     named_barrier_sync(2, C::SOFT);
-                    float xs = lv_here;
+                    const float xm = fmaxf(fmaxf(x, s_half[w ^ 1][row]), m);
+                    float top = -INFINITY;       // log2 of the largest weight times V's scale (a NaN, -inf less -inf, is passed over)
 #pragma unroll
-                    for (int d = 16; d; d >>= 1) xs = fmaxf(xs, __shfl_xor_sync(0xffffffffu, xs, d));
-                    const float xm = fmaxf(fmaxf(x, s_half[w ^ 1][row]), m), xr = fmaxf(xs, lr);
-                    const float el = xm == m ? 1.0f : ex2(m - xm), eo = el * ex2(lr - xr);
+                    for (int g = 0; g < NG / 2; ++g) top = fmaxf(top, z[g] - xm + fv[g]);
+                    s_top[w][row] = top;
+                    named_barrier_sync(2, C::SOFT);
+                    top = fmaxf(fmaxf(top, s_top[w ^ 1][row]), m - xm + lr);
+                    // (a row that has seen nothing yet stays as it is)
+                    const float xr = xm == -INFINITY ? lr : fminf(fmaxf(ceilf(top), kLeastLog), 127.0f);
+                    const float dm = xm == m ? 0.0f : m - xm, el = ex2(dm), eo = ex2(dm + (lr - xr));
                     if (jj > 0) {                // the products of the tile before are in
                         wait(&v_free[(tl - 1) % C::NBUF], ((tl - 1) / C::NBUF) & 1);
                         tc_fence_after();
@@ -811,7 +843,9 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
             named_barrier_sync(2, C::SOFT);
             l += s_half[w ^ 1][row];
             const bool whole = seg.j == 0 && seg.n == seg.tiles;
-            const float fo = ex2(lr - kWeightLog) * (whole ? 1.0f / l : 1.0f);
+            // parts are divided by their own sums, so that none passes the largest value
+            // (a part that the row sees nothing of: 0; 1 / NaN stays)
+            const float fo = exp2_int(-kWeightLog) * (l == 0.0f ? 0.0f : 1.0f / l), fr = exp2_int(lr);
             const int64_t orow = (int64_t)(seg.r0 + f / G) * a.heads + seg.h * G + f % G;
             float* pt = parts + ((int64_t)blockIdx.x * 2 + (seg.j == 0)) * C::PART;
             wait(&o_full, sn & 1);
@@ -832,7 +866,7 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 16; ++i) y[i] *= fo;
+                for (int i = 0; i < 16; ++i) y[i] = y[i] * fo * fr;
                 if (!whole) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
@@ -893,7 +927,7 @@ __global__ void __launch_bounds__(kFinishThreads) kvb_rows_finish(const KvbAttnA
     const RowsUnit s = plan.unit[w.u];
     const int c0 = blockIdx.x - 1;
     const int r0 = blockIdx.y * kJoinRows;
-    __shared__ float s_m[kJoinRows], s_i[kJoinRows], s_o[kJoinRows][HD + 1];
+    __shared__ float s_m[kJoinRows], s_i[kJoinRows], s_o[kJoinRows][HD + 1];   // maxima, 1 / sums
     auto at = [&](int c) { return parts + ((int64_t)c * 2 + (c == c0)) * C::PART; };
     {
         static_assert(kFinishThreads == 16 * kJoinRows, "16 threads a row");
@@ -925,12 +959,13 @@ __global__ void __launch_bounds__(kFinishThreads) kvb_rows_finish(const KvbAttnA
         float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
         for (int c = c0; c <= last; ++c) {
-            const float mc = at(c)[kRows * HD + row], e = mc == -INFINITY ? 0.0f : ex2(mc - m);
+            const float mc = at(c)[kRows * HD + row], lc = at(c)[kRows * (HD + 1) + row];
+            const float e = (mc == -INFINITY ? 0.0f : ex2(mc - m) * lc) * inv;
             const float4 x = reinterpret_cast<const float4*>(at(c))[d4 * kRows + row];
             y.x = fmaf(x.x, e, y.x), y.y = fmaf(x.y, e, y.y), y.z = fmaf(x.z, e, y.z), y.w = fmaf(x.w, e, y.w);
         }
         float* o = &s_o[r][4 * d4];
-        o[0] = y.x * inv, o[1] = y.y * inv, o[2] = y.z * inv, o[3] = y.w * inv;
+        o[0] = y.x, o[1] = y.y, o[2] = y.z, o[3] = y.w;
     }
     __syncthreads();
     for (int i = tid; i < kJoinRows * HD; i += kFinishThreads) {
