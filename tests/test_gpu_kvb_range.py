@@ -125,3 +125,32 @@ def test_scores_in_which_a_scale_is_lost(hd, dt, size):
             off = (out[6 * b:6 * b + 6].double() - want).abs()
             assert (off <= (2.0 ** -18 + 2.0 ** -20 + torch.finfo(TYPES[dt]).eps / 2) * want.abs()).all(), (b, t, off.max())
         cache.k[:, :, t] = 0
+
+
+@pytest.mark.parametrize("rows", [False, True])
+@pytest.mark.parametrize("tiny", [1e-18, 1e-25, 1e-33, 1e-36])
+@pytest.mark.parametrize("heads,kv_heads,hd,block,dt", [
+    (4, 2, 64, 16, "fp32"), (16, 2, 128, 64, "fp32"), (3, 1, 256, 32, "fp32"), (8, 2, 48, 32, "bf16"),
+    (24, 2, 128, 32, "bf16")])
+def test_tiny_queries(heads, kv_heads, hd, block, dt, tiny, rows):
+    """Queries of any size against keys, or a scale, that bring the scores back; one head of another size beside them,
+    zeros in the rows."""
+    g = torch.Generator(device=DEV).manual_seed(hd)
+    cache = make_cache(g, 3, kv_heads, 512, hd, block)
+    counts = [40, 1, 9] if rows else [1, 1, 1]
+    start, pos = [0, counts[0], counts[0] + counts[1], sum(counts)], [300, 17, 500]
+    q = torch.randn(start[-1], heads, hd, generator=g, device=DEV) * tiny
+    q[:, :, 1::3] = 0
+    q[:, 1] *= 2.0 ** -12
+    q = q.to(TYPES[dt])
+    compare(q, cache, pos, start, dt, hd, 512, scale=0.25 / tiny, rows=rows)
+    cache.k_scale.mul_(0.1 / tiny)
+    compare(q, cache, pos, start, dt, hd, 512, scale=1.0, rows=rows)
+
+
+def test_subnormal_queries_of_single_tokens():
+    g = torch.Generator(device=DEV).manual_seed(3)
+    cache = make_cache(g, 2, 2, 256, 64, 32)
+    q = torch.randn(2, 8, 64, generator=g, device=DEV) * 1e-38 * 2.0 ** -torch.arange(0, 16, 2, device=DEV).view(8, 1)
+    assert (q != 0).any(-1).all()
+    compare(q, cache, [255, 100], None, "fp32", 64, 256, scale=1e38, rows=False)

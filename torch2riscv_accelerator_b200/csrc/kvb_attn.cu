@@ -45,6 +45,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 //            channels). The query row is taken to 24-bit fixed point of its
 //            largest element; its three signed 8-bit digits make three
 //            products (column n: head n % GC), whose integer sums are exact.
+//            (A row below 2^-64 is taken up by 2^64 for it; its factor has 2^11
+//            that K's scales give, so that rows down to 1e-33 and scales down to
+//            1e-34 keep all their bits.)
 //   outputs  mma m16n8k16 in fp16 with fp32 sums (16 channels x 16 tokens): the
 //            codes become halves exactly (byte permutes and one subtraction),
 //            the weights enter as hi + lo halves (22 bits), in columns of
@@ -301,8 +304,10 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD, GC>::CTAS) kvb_step_kern
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             const unsigned int bad = __ballot_sync(0xffffffffu, nan);
+            const float pre = mx < 0x1p-64f ? 0x1p64f : 1.0f;
+            mx *= pre;
             const float up = mx > 0.0f ? 8355711.0f / mx : 0.0f;         // 0x7F7F7F: the largest three digits
-            float qs = mx * (1.0f / 8355711.0f) * a.scale * kLog2e;
+            float qs = mx * (2048.0f / 8355711.0f) * a.scale * kLog2e * (1.0f / pre);
             if (bad >> (lane & ~3) & 15u) qs = NAN;                      // a NaN or infinite row gives NaN
             qsa = __shfl_sync(0xffffffffu, qs, (2 * t) % GC * 4);
             qsb = __shfl_sync(0xffffffffu, qs, (2 * t + 1) % GC * 4);
@@ -317,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD, GC>::CTAS) kvb_step_kern
                     uint32_t v[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float x = fminf(fmaxf(y[w * 4 + i] * up, -8355711.0f), 8355711.0f);
+                        const float x = fminf(fmaxf(y[w * 4 + i] * pre * up, -8355711.0f), 8355711.0f);
                         v[i] = ((uint32_t)__float2int_rn(x) + 0x808080u) ^ 0x808080u;   // three signed digits
                     }
                     const uint32_t x01 = __byte_perm(v[0], v[1], 0x5140), x23 = __byte_perm(v[2], v[3], 0x5140);
@@ -351,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD, GC>::CTAS) kvb_step_kern
             const int t0 = (first + n) * C::TILE + warp * C::TOK;
             float fk[KT], fs[KT];
 #pragma unroll
-            for (int k = 0; k < KT; ++k) fk[k] = sk[k], fs[k] = sv[k];
+            for (int k = 0; k < KT; ++k) fk[k] = sk[k] * 0x1p-11f, fs[k] = sv[k];
             if (n + 1 < n_it) scales(t0 + C::TILE);
             cp_wait<C::NST - 2>();
             __syncwarp();                        // this stage has landed, the one before it is free
