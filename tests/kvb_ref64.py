@@ -11,11 +11,12 @@ move-outs, 2 * FOLD * 128 / 16 of them; the moved-out sums and the weights' sum 
 added in fp32 over n tokens in at most n / 32 + 16 steps of 2^-24. All are relative
 to sum p |v|: (4 |dz| + 2^-20 + 2^-18 + 16 FOLD 2^-23 + (n / 32 + 16) 2^-24) sum p |v|.
 
-A weight times V's scale, over a reference of at most twice the row's largest such
-(2^-126 of the largest weight at least), enters as two halves that stand for 2^7 of it.
-Where they are subnormal each is off by half a step of 2^-24, 2^-24 / 2^7 of the
-reference together (but a weight by no more than itself):
-sum_t min(2^-30 max_t p_t s_t, 2 p_t s_t) |code_t|. (A channel where the heaviest token
+A weight times V's scale, over a reference of at most four times the row's largest
+such (twice in prompts; at least 2^-126 of the largest weight, for single tokens 2^-119 and
+2^-120 of the largest weight times the largest scale),
+enters as two halves that stand for 2^5 of it (2^7). Where they are subnormal each is off
+by half a step of 2^-24, 2^-24 / 2^5 of the reference together (but a weight by no more
+than itself): sum_t min(2^-27 max_t p_t s_t, 2 p_t s_t) |code_t| (2^-30). (A channel where the heaviest token
 holds 0 has nothing but such weights.) The output's type rounds by half a step, relative
 to it and of its smallest subnormal; parts of a row that are joined round once more."""
 import torch
@@ -35,7 +36,7 @@ def dz_of(zabs, hd):
     return (2.0 ** -21 + (hd / 16 + 2) * 2.0 ** -23) * zabs
 
 
-def attend(q, cache, b, p, rows, h, scale=None):
+def attend(q, cache, b, p, rows, h, scale=None, single=False):
     """Rows (indices i at positions p + i) of one slot and KV head in float64: q [n, G, D] of these rows -> their
     outputs, probabilities [n, G, T], sum p |v|, max sum|q k| scale, and what subnormal halves may lose."""
     k, ks, v, vs = cache
@@ -49,8 +50,11 @@ def attend(q, cache, b, p, rows, h, scale=None):
     scale = D ** -0.5 if scale is None else scale
     w = torch.softmax((q @ kd.T * scale).masked_fill(hidden, -float("inf")), -1)
     zabs = ((q.abs() @ kd.abs().T) * abs(scale)).masked_fill(hidden, 0.0).amax(-1, keepdim=True)
-    ref = torch.maximum((w * sv).amax(-1, keepdim=True), 2.0 ** -126 * w.amax(-1, keepdim=True))
-    lost = torch.minimum(2 * w * sv, 2.0 ** -30 * ref) @ v[b, h, :T].double().abs()
+    least, step = (2.0 ** -119, 2.0 ** -27) if single else (2.0 ** -126, 2.0 ** -30)
+    ref = torch.maximum((w * sv).amax(-1, keepdim=True), least * w.amax(-1, keepdim=True))
+    if single:
+        ref = torch.maximum(ref, 2.0 ** -120 * sv.max() * w.amax(-1, keepdim=True))
+    lost = torch.minimum(2 * w * sv, step * ref) @ v[b, h, :T].double().abs()
     return w @ vd, w, w @ vd.abs(), zabs, lost
 
 

@@ -24,7 +24,7 @@ def compare(q, cache, pos, start, dt, hd, n, scale=None, rows=True):
             continue
         at = torch.arange(e - a, device=DEV)
         for h in range(H):
-            want, _, vabs, zabs, lost = attend(q[a:e, h * G:h * G + G], cache, b, p, at, h, scale)
+            want, _, vabs, zabs, lost = attend(q[a:e, h * G:h * G + G], cache, b, p, at, h, scale, not rows)
             check(out[a:e, h * G:h * G + G], want, vabs, zabs, lost, n, hd, dt)
     return out
 
@@ -65,64 +65,75 @@ def test_an_infinity_in_the_last_value_leaves_earlier_rows():
 
 @pytest.mark.parametrize("heads,kv_heads,hd,block,dt", [
     (4, 2, 64, 64, "fp32"), (16, 2, 128, 16, "fp32"), (2, 1, 256, 64, "fp32"), (8, 2, 64, 32, "bf16")])
+@pytest.mark.parametrize("rows", [False, True])
 @pytest.mark.parametrize("big", [2.0 ** 30, 2.0 ** 100])
-def test_a_large_block_without_weight_does_not_count(heads, kv_heads, hd, block, dt, big):
+def test_a_large_block_without_weight_does_not_count(heads, kv_heads, hd, block, dt, big, rows):
     """Every row sees the large block, but its scores lie so far below the others that its weights are 0."""
     g = torch.Generator(device=DEV).manual_seed(hd)
     cap = 640
     cache = make_cache(g, 2, kv_heads, cap, hd, block)
-    q = torch.rand(2 * 70, heads, hd, generator=g, device=DEV).add_(0.5).to(TYPES[dt])
+    n = 70 if rows else 1
+    q = torch.rand(2 * n, heads, hd, generator=g, device=DEV).add_(0.5).to(TYPES[dt])
     for j in (1, 7):                                          # keys against the queries, all other scores near 0
         cache.k[:, :, j * block:(j + 1) * block] = -127
         cache.k_scale[:, :, j] = 2.0
         cache.v_scale[:, :, j] *= big
-    compare(q, cache, [500, 512], [0, 70, 140], dt, hd, cap)
+    compare(q, cache, [500, 512], [0, n, 2 * n], dt, hd, cap, rows=rows)
 
 
+@pytest.mark.parametrize("rows", [False, True])
 @pytest.mark.parametrize("tiny", [1e-30, 1e-34, 1e-36, 1e-38, 1e-41, 1e-42])
 @pytest.mark.parametrize("heads,kv_heads,hd,block,dt", [
     (4, 2, 64, 16, "fp32"), (16, 2, 128, 64, "fp32"), (2, 2, 256, 32, "fp32"), (8, 2, 64, 32, "bf16")])
-def test_tiny_values(heads, kv_heads, hd, block, dt, tiny):
+def test_tiny_values(heads, kv_heads, hd, block, dt, tiny, rows):
     """V of any size comes back at its size, subnormal scales too; a scale of 0 is no value at all."""
     g = torch.Generator(device=DEV).manual_seed(hd)
     cache = make_cache(g, 2, kv_heads, 256, hd, block)
     cache.v_scale.mul_(tiny)
     cache.v_scale[:, :, 1] = 0                                # a block of zeros
-    q = torch.randn(140, heads, hd, generator=g, device=DEV).to(TYPES[dt])
-    out = compare(q, cache, [180, 5], [0, 70, 140], dt, hd, 256)
+    n = 70 if rows else 1
+    q = torch.randn(2 * n, heads, hd, generator=g, device=DEV).to(TYPES[dt])
+    out = compare(q, cache, [180, 5], [0, n, 2 * n], dt, hd, 256, rows=rows)
     t = torch.finfo(TYPES[dt])
     assert out.abs().max() > tiny / 100 or tiny < 100 * t.smallest_normal * t.eps      # (the type's own end)
 
 
-@pytest.mark.parametrize("hd,dt", [(64, "fp32"), (128, "fp32"), (256, "fp32"), (128, "bf16")])
-def test_huge_values(hd, dt):
-    """V up to the largest that append writes: finite outputs, wherever a row's parts are joined."""
+@pytest.mark.parametrize("rows", [False, True])
+@pytest.mark.parametrize("hd,dt,cap", [(64, "fp32", 2048), (128, "fp32", 2048), (256, "fp32", 2048),
+                                       (128, "bf16", 2048), (64, "fp32", 17024), (128, "fp32", 8256)])
+def test_huge_values(hd, dt, cap, rows):
+    """V up to the largest that append writes: finite outputs, wherever a row's parts are joined (single tokens: in a
+    cluster, for the long caches by a second kernel)."""
     g = torch.Generator(device=DEV).manual_seed(hd)
-    cache = make_cache(g, 1, 8, 2048, hd, 64)
+    cache = make_cache(g, 1, 8, cap, hd, 64)
     cache.v_scale.fill_(2.6e36)
-    cache.k_scale.mul_(torch.linspace(0.1, 3.0, 32, device=DEV))         # maxima that rise
-    q = torch.randn(70, 16, hd, generator=g, device=DEV).to(TYPES[dt])
-    compare(q, cache, [1978], [0, 70], dt, hd, 2048)
+    cache.k_scale.mul_(torch.linspace(0.1, 3.0, cap // 64, device=DEV))  # maxima that rise
+    n = 70 if rows else 1
+    q = torch.randn(n, 16, hd, generator=g, device=DEV).to(TYPES[dt])
+    compare(q, cache, [cap - n], [0, n], dt, hd, cap, rows=rows)
 
 
+@pytest.mark.parametrize("rows", [False, True])
 @pytest.mark.parametrize("size", [1e2, 1e4, 2e5])
 @pytest.mark.parametrize("hd,dt", [(64, "fp32"), (128, "bf16"), (256, "fp32")])
-def test_scores_in_which_a_scale_is_lost(hd, dt, size):
+def test_scores_in_which_a_scale_is_lost(hd, dt, size, rows):
     """One token far above all others, scores of up to 2^24, V scales of very different sizes: that token's values. Its weight
     cancels but for the logarithm of V's scale (at most 2^-18 off), the exponential and two halves (2^-20)."""
     g = torch.Generator(device=DEV).manual_seed(hd)
     cache = make_cache(g, 2, 2, 256, hd, 16)
-    q = torch.ones(12, 4, hd, device=DEV, dtype=TYPES[dt])
+    n = 6 if rows else 1
+    q = torch.ones(2 * n, 4, hd, device=DEV, dtype=TYPES[dt])
     cache.k.clamp_(-20, 20)
     cache.k_scale.fill_(size / 36)
     cache.v_scale.mul_(2.0 ** torch.linspace(-60, 60, 16, device=DEV))
     cache.v_scale[1] = cache.v_scale[1].flip(-1)
     for t in (40, 130):                                       # the other tokens' sums are below hd * 20
         cache.k[:, :, t] = 127
-        out = ops.kvb_attn_rows(q, cache, i32([200, 150]), i32([0, 6, 12]))
+        pos = i32([200, 150])
+        out = ops.kvb_attn_rows(q, cache, pos, i32([0, n, 2 * n])) if rows else ops.kvb_attn(q, cache, pos)
         for b in range(2):
             want = (cache.v[b, :, t].double() * cache.v_scale[b, :, t // 16, None].double()).repeat_interleave(2, 0)
-            off = (out[6 * b:6 * b + 6].double() - want).abs()
+            off = (out[n * b:n * b + n].double() - want).abs()
             assert (off <= (2.0 ** -18 + 2.0 ** -20 + torch.finfo(TYPES[dt]).eps / 2) * want.abs()).all(), (b, t, off.max())
         cache.k[:, :, t] = 0
 

@@ -52,14 +52,18 @@ constexpr float kLog2e = 1.4426950408889634f;
 //            codes become halves exactly (byte permutes and one subtraction),
 //            the weights enter as hi + lo halves (22 bits), in columns of
 //            their own where GC leaves room.
-// Maxima move lazily: a warp rescales when a score passes its head's reference
-// by 2^6 or a block's V scale its reference by 2^2; the weights
-// exp(z - m) sv / sv_ref 2^7 then stay below 2^15.
+// The weights are exp(z - m) sv / 2^r 2^5: m is the warp's largest score of the head,
+// 2^r its largest exp(z - m) sv, an integer power of two, so that a block without weight
+// leaves the others' halves their bits, however large its values are. Both move lazily:
+// a warp looks when a score passes m by 2^5 or a block's V scale 2^r by 2^5, and rescales;
+// the weights then stay below 2^15. A warp's outputs are divided by its own sum before
+// they are joined, so that none passes the largest value.
 namespace cg = cooperative_groups;
 constexpr int kStepWarps = 4;
 constexpr int kClusterMost = 16;                 // CTAs of a cluster
 constexpr int kMaxParts = 2;                     // partial units per CTA
-constexpr float kLazyScore = 6.0f, kLazyScale = 4.0f, kWeightScale = 128.0f;
+constexpr float kLazyScore = 5.0f, kLazyScale = 1024.0f;   // 2^5, and the weights' 2^5
+constexpr int kWeightLog = 5, kLeastLog = -119, kMostLog = 122;   // the references' range: 2^(5 - r) and its inverse are normal
 
 template <int HD, int GC>
 struct StepCfg {
@@ -101,6 +105,44 @@ __device__ __forceinline__ int64_t step_scan(const KvbAttnArgs& a, int tile, int
     for (int w = 0; w < kThreads / 32; ++w) x += s_sum[0][w], y += s_sum[1][w];
     *before = y;
     return x;
+}
+
+// 2^(5 - r) of a reference r, and back
+__device__ __forceinline__ float ref_factor(int r) { return __int_as_float((127 + kWeightLog - r) << 23); }
+__device__ __forceinline__ int ref_of(float factor) { return 127 + kWeightLog - (__float_as_int(factor) >> 23); }
+__device__ __forceinline__ float inverse_of(float factor) { return __int_as_float((254 << 23) - __float_as_int(factor)); }
+// 1 / x within 2^-23, for the sums of weights (a division is a subroutine)
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// An integer above log2(s)
+__device__ __forceinline__ float log2_above(float s) { return (float)(max(__float_as_int(s) >> 23, 1) - 126); }
+
+// A head's maximum m and reference (as factor) moved for a tile whose 16 KT tokens' largest
+// scores on this lane are x[k]: what the sums and the outputs are to be multiplied by.
+template <int KT>
+__device__ __forceinline__ float2 move_refs(const float (&x)[KT], const float (&fs)[KT], float& m, float& factor) {
+    float xm = x[0];
+    if constexpr (KT == 2) xm = fmaxf(xm, x[1]);
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) xm = fmaxf(xm, __shfl_xor_sync(0xffffffffu, xm, d));
+    xm = fmaxf(xm, m);
+    float top = -INFINITY;                       // (-inf less -inf, a NaN, is passed over)
+#pragma unroll
+    for (int k = 0; k < KT; ++k) {               // (a scale over 2^r 2^5 stays below 2^126)
+        const float e = log2_above(fs[k]);
+        top = fmaxf(top, fmaxf(x[k] - xm + e, e - 121.0f));
+    }
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const int r = ref_of(factor);
+    top = fmaxf(top, m - xm + (float)r);
+    const int to = xm == -INFINITY ? r : min(max(__float2int_ru(top), kLeastLog), kMostLog);
+    const float dm = xm == m ? 0.0f : m - xm;
+    m = xm, factor = ref_factor(to);
+    return make_float2(ex2(dm), ex2(dm + (float)(r - to)));
 }
 
 __device__ __forceinline__ void mma_s8(int* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -335,7 +377,8 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD, GC>::CTAS) kvb_step_kern
         }
 
         // outputs: channel tile i, column tile; maxima and sums of the lane's two heads
-        float o[MT][C::NP][4], ma = -INFINITY, mb = -INFINITY, la = 0.0f, lb = 0.0f, svr = 0.0f, rsv = 0.0f;
+        float o[MT][C::NP][4], ma = -INFINITY, mb = -INFINITY, la = 0.0f, lb = 0.0f;
+        float ra = 1.0f, rb = 1.0f;              // the references as factors 2^(5 - r)
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -409,33 +452,27 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD, GC>::CTAS) kvb_step_kern
                     xa = fmaxf(xa, fmaxf(z[1][0], z[1][2])), xb = fmaxf(xb, fmaxf(z[1][1], z[1][3]));
                     xs = fmaxf(xs, fs[1]);
                 }
-                if (__any_sync(0xffffffffu, xa > ma + kLazyScore || xb > mb + kLazyScore || xs > svr * kLazyScale)) {
+                if (__any_sync(0xffffffffu, xa > ma + kLazyScore || xb > mb + kLazyScore || xs * fmaxf(ra, rb) > kLazyScale)) {
+                    float ya[KT], yb[KT];
 #pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) {
-                        xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, d));
-                        xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, d));
-                    }
-                    xa = fmaxf(xa, ma), xb = fmaxf(xb, mb), xs = fmaxf(xs, svr);
-                    const float ea = xa == ma ? 1.0f : ex2(ma - xa), eb = xb == mb ? 1.0f : ex2(mb - xb);
-                    const float es = xs > 0.0f ? svr / xs : 0.0f, oa = ea * es, ob = eb * es;
-                    la *= ea, lb *= eb;
+                    for (int k = 0; k < KT; ++k) ya[k] = fmaxf(z[k][0], z[k][2]), yb[k] = fmaxf(z[k][1], z[k][3]);
+                    const float2 ea = move_refs<KT>(ya, fs, ma, ra), eb = move_refs<KT>(yb, fs, mb, rb);
+                    la *= ea.x, lb *= eb.x;
 #pragma unroll
                     for (int i = 0; i < MT; ++i)
 #pragma unroll
                         for (int x = 0; x < C::NP; ++x)
-                            o[i][x][0] *= oa, o[i][x][1] *= ob, o[i][x][2] *= oa, o[i][x][3] *= ob;
-                    ma = xa, mb = xb, svr = xs;
-                    rsv = svr > 1e-33f ? kWeightScale / svr : 0.0f;      // values below count as 0
+                            o[i][x][0] *= ea.y, o[i][x][1] *= eb.y, o[i][x][2] *= ea.y, o[i][x][3] *= eb.y;
                 }
 #pragma unroll
                 for (int k = 0; k < KT; ++k) {
-                    const float fv = fs[k] * rsv;
+                    const float fa = fs[k] * ra, fb = fs[k] * rb;
                     uint32_t pb[C::NP][2];       // the weights as the products' columns
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {                        // tokens g, then g + 8
                         const float ea = ex2(z[k][2 * j] - ma), eb = ex2(z[k][2 * j + 1] - mb);
                         la += ea, lb += eb;
-                        const float wa = ea * fv, wb = eb * fv;
+                        const float wa = ea * fa, wb = eb * fb;
                         const __half2 hi = __floats2half2_rn(wa, wb);
                         const float2 back = __half22float2(hi);
                         const __half2 lo = __floats2half2_rn(wa - back.x, wb - back.y);
@@ -495,7 +532,8 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD, GC>::CTAS) kvb_step_kern
         }
         __syncthreads();                         // the last unit's readers are done
         {
-            const float f = svr * (1.0f / kWeightScale);
+            // 1 / sum (no tokens: 0; 1 / NaN stays), then 2^(r - 5)
+            const float ia = la == 0.0f ? 0.0f : rcp(la), ib = lb == 0.0f ? 0.0f : rcp(lb), fa = inverse_of(ra), fb = inverse_of(rb);
             constexpr int RUN = HD == 64 ? 8 : 16;
             float* wa = merge + (warp * GC + (2 * t) % GC) * (HD + 2);
             const bool mine = 2 * t < GC;        // the columns of the lo halves are added to the hi ones'
@@ -509,8 +547,8 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD, GC>::CTAS) kvb_step_kern
                 }
                 float* w = wa + (i / 8) * 128 + RUN * g + 2 * (i % 8);
                 if (mine) {
-                    *reinterpret_cast<float2*>(w) = make_float2(y[0] * f, y[2] * f);
-                    *reinterpret_cast<float2*>(w + HD + 2) = make_float2(y[1] * f, y[3] * f);
+                    *reinterpret_cast<float2*>(w) = make_float2(y[0] * ia * fa, y[2] * ia * fa);
+                    *reinterpret_cast<float2*>(w + HD + 2) = make_float2(y[1] * ib * fb, y[3] * ib * fb);
                 }
             }
             if (mine && g == 0) wa[HD] = ma, wa[HD + 1] = la, wa[2 * HD + 2] = mb, wa[2 * HD + 3] = lb;
@@ -524,12 +562,15 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD, GC>::CTAS) kvb_step_kern
             float mm = w[HD];
 #pragma unroll
             for (int x = 1; x < kStepWarps; ++x) mm = fmaxf(mm, w[x * WS + HD]);
-            float acc = 0.0f, ll = 0.0f;
+            float acc = 0.0f, ll = 0.0f, f[kStepWarps];
 #pragma unroll
             for (int x = 0; x < kStepWarps; ++x) {
-                const float f = w[x * WS + HD] == -INFINITY ? 0.0f : ex2(w[x * WS + HD] - mm);
-                acc = fmaf(w[x * WS + d], f, acc), ll = fmaf(w[x * WS + HD + 1], f, ll);
+                f[x] = w[x * WS + HD] == -INFINITY ? 0.0f : ex2(w[x * WS + HD] - mm);
+                f[x] *= w[x * WS + HD + 1], ll += f[x];
             }
+            const float inv = ll == 0.0f ? 0.0f : rcp(ll);
+#pragma unroll
+            for (int x = 0; x < kStepWarps; ++x) acc = fmaf(w[x * WS + d], f[x] * inv, acc);
             const int64_t row = (int64_t)b * a.heads + h * G + j0 + j;
             if constexpr (CLUSTER) {
                 float* p = merge + kStepWarps * C::PART + j * (HD + 2);
@@ -539,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD, GC>::CTAS) kvb_step_kern
                 pt[j * (HD + 2) + d] = acc;
                 if (d == 0) pt[j * (HD + 2) + HD] = mm, pt[j * (HD + 2) + HD + 1] = ll;
             } else {
-                if (d < hd) store1(a.out, a.type, row * hd + d, acc / ll);
+                if (d < hd) store1(a.out, a.type, row * hd + d, acc);
                 if (scores && d == 0) {
                     float* ml = scores + (int64_t)a.c.slots * a.heads * a.c.cap + 2 * row;
                     ml[0] = mm, ml[1] = ll;
@@ -553,22 +594,26 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD, GC>::CTAS) kvb_step_kern
             const int n = cl.num_blocks();
             for (int i = cl.block_rank() * kThreads + tid; i < live * hd; i += n * kThreads) {
                 const int j = i / hd, d = i - j * hd;
-                float mr[kClusterMost], mm = -INFINITY, acc = 0.0f, ll = 0.0f;
+                float2 ml[kClusterMost];         // the CTAs' maxima and sums
+                float mm = -INFINITY, acc = 0.0f, ll = 0.0f;
 #pragma unroll
                 for (int r = 0; r < kClusterMost; ++r) {
-                    mr[r] = r < n ? cl.map_shared_rank(own, r)[j * (HD + 2) + HD] : -INFINITY;
-                    mm = fmaxf(mm, mr[r]);
+                    ml[r] = make_float2(-INFINITY, 0.0f);
+                    if (r < n) ml[r] = *reinterpret_cast<const float2*>(cl.map_shared_rank(own, r) + j * (HD + 2) + HD);
+                    mm = fmaxf(mm, ml[r].x);
                 }
 #pragma unroll
+                for (int r = 0; r < kClusterMost; ++r) {
+                    ml[r].y *= ml[r].x == -INFINITY ? 0.0f : ex2(ml[r].x - mm);
+                    ll += ml[r].y;
+                }
+                const float inv = rcp(ll);
+#pragma unroll
                 for (int r = 0; r < kClusterMost; ++r)
-                    if (r < n) {
-                        const float* p = cl.map_shared_rank(own, r) + j * (HD + 2);
-                        const float f = mr[r] == -INFINITY ? 0.0f : ex2(mr[r] - mm);
-                        acc = fmaf(p[d], f, acc), ll = fmaf(p[HD + 1], f, ll);
-                    }
+                    if (r < n) acc = fmaf(cl.map_shared_rank(own, r)[j * (HD + 2) + d], ml[r].y * inv, acc);
                 // a slot without tokens: zeros
                 const int64_t row = (int64_t)b * a.heads + h * G + j0 + j;
-                store1(a.out, a.type, row * hd + d, len > 0 ? acc / ll : 0.0f);
+                store1(a.out, a.type, row * hd + d, len > 0 ? acc : 0.0f);
                 if (scores && GT > 1 && d == 0) {
                     float* ml = scores + (int64_t)a.c.slots * a.heads * a.c.cap + 2 * row;
                     ml[0] = mm, ml[1] = ll;
@@ -636,7 +681,7 @@ __global__ void __launch_bounds__(kThreads) kvb_step_finish(const KvbAttnArgs a,
     const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, hd = a.c.hd;
     const int j = blockIdx.x * (kThreads / 32 / W) + warp / W, b = blockIdx.y;
     if (j >= a.heads) return;
-    __shared__ float s_o[W > 1 ? kThreads / 32 : 1][W > 1 ? HD + 1 : 1];
+    __shared__ float s_o[W > 1 ? kThreads / 32 : 1][W > 1 ? HD : 1];
     const int G = a.heads / a.c.heads, GT = (G + GC - 1) / GC, units = a.c.heads * GT;
     int all = 0, pre = 0;
     for (int i = lane; i < a.c.slots; i += 32) {
@@ -661,15 +706,29 @@ __global__ void __launch_bounds__(kThreads) kvb_step_finish(const KvbAttnArgs a,
     const float* p0 = parts + row * (HD + 2);
     auto at = [&](int c) { return p0 + ((int64_t)c * kMaxParts + (c == c0)) * C::PART; };
     float m = -INFINITY, l = 0.0f, o[V];
-    for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, at(c)[HD]);
+    for (int c = c0 + lane; c <= c1; c += 32) {
+        const float2 x = *reinterpret_cast<const float2*>(at(c) + HD);   // maximum, sum
+        const float top = fmaxf(m, x.x);
+        l = (m == -INFINITY ? l : l * ex2(m - top)) + x.y * ex2(x.x - top);
+        m = top;
+    }
+    float top = m;
 #pragma unroll
-    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    if (m != -INFINITY) l *= ex2(m - top);
+    m = top;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    const float inv = rcp(l);
 #pragma unroll
     for (int v = 0; v < V; ++v) o[v] = 0.0f;
     for (int cc = c0 + warp % W; cc <= c1; cc += 32 * W) {               // this warp: every W-th part
         const int n = min(32, (c1 - cc) / W + 1);
         float w = 0.0f;
-        if (lane < n) w = ex2(at(cc + lane * W)[HD] - m), l = fmaf(at(cc + lane * W)[HD + 1], w, l);
+        if (lane < n) {
+            const float2 x = *reinterpret_cast<const float2*>(at(cc + lane * W) + HD);
+            w = ex2(x.x - m) * x.y * inv;
+        }
 #pragma unroll 8
         for (int i = 0; i < n; ++i) {
             const float* p = at(cc + i * W) + lane * V;
@@ -681,29 +740,21 @@ __global__ void __launch_bounds__(kThreads) kvb_step_finish(const KvbAttnArgs a,
             }
         }
     }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
     if constexpr (W > 1) {
 #pragma unroll
         for (int v = 0; v < V; ++v) s_o[warp][lane * V + v] = o[v];
-        if (lane == 0) s_o[warp][HD] = l;
         __syncthreads();                         // one row per CTA: every warp comes here
-        l = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) l += s_o[w][HD];
-        const float r = 1.0f / l;
         for (int d = threadIdx.x; d < hd; d += kThreads) {
             float y = 0.0f;
 #pragma unroll
             for (int w = 0; w < W; ++w) y += s_o[w][d];
-            store1(a.out, a.type, out + d, y * r);
+            store1(a.out, a.type, out + d, y);
         }
         if (warp) return;
     } else {
-        const float r = 1.0f / l;
 #pragma unroll
         for (int v = 0; v < V; ++v)
-            if (lane * V + v < hd) store1(a.out, a.type, out + lane * V + v, o[v] * r);
+            if (lane * V + v < hd) store1(a.out, a.type, out + lane * V + v, o[v]);
     }
     if (scores && lane == 0) {
         float* ml = scores + (int64_t)a.c.slots * a.heads * a.c.cap + 2 * ((int64_t)b * a.heads + j);
