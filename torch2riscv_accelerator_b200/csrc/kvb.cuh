@@ -7,6 +7,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include "kvb_plan.cuh"
 #include "pdl.cuh"
 
 namespace w8a8 {
@@ -185,11 +186,6 @@ __device__ __forceinline__ void cp16z(uint32_t dst, const void* src, bool in) {
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-// x / y for y > 0; 32-bit where it fits (a 64-bit division is a subroutine)
-__device__ __forceinline__ int64_t div64(int64_t x, int64_t y) {
-    return x >> 32 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
-}
 
 // pairs of floats in one instruction
 __device__ __forceinline__ uint64_t pack2(float x, float y) {

@@ -71,10 +71,6 @@ constexpr unsigned int kErrWait = 256u;          // error bit 8: a pipeline wait
 // 6.4e-7 every 2; moving out every 2 tiles instead of 4 costs 11 % of the time).
 template <typename T>
 constexpr int kFold = sizeof(T) == 4 ? 3 : 32;   // (16-bit outputs round by 2e-4 and more)
-// Shares are equal in tiles plus kUnitCost for each unit begun: a unit's first
-// queries and last outputs cost about as much as two tiles (by tiles alone the
-// CTA with a causal prompt's short units took 20 % longer than the others).
-constexpr int kUnitCost = 2;
 constexpr int kFinishThreads = 256;
 
 template <int HD>
@@ -101,16 +97,8 @@ struct RowsCfg {
     static constexpr size_t PART = (size_t)kRows * (HD + 2), ACC = (size_t)kRows * HD;
 };
 
-struct __align__(16) RowsUnit {
-    int slot, m, before, tiles;                  // 128-row tile of the slot, cost of the units before, tiles
-    int p, r0, rows, pad;                        // position of the slot's first row, its row, the slot's n * G live rows
-};
-struct __align__(16) RowsShare {                 // a CTA's share [lo, hi) of the cost
-    int64_t lo, hi;
-    int h, u, join, pad;                         // KV head and unit where it begins; if that unit is cut there for the
-};                                               // first time, the last share with a part of it, else -1
 struct RowsPlan {                                // in scratch
-    int* head;                                   // [4]: cost of all units of one KV head, units
+    int64_t* head;                               // [2]: cost of all units of one KV head, units
     RowsUnit* unit;
     int* first;                                  // [slots + 1]: the slots' first units
     RowsShare* share;                            // [kSms]
@@ -124,18 +112,18 @@ __device__ __forceinline__ int live_rows(const KvbSpan& s, int cap) { return s.p
 
 // exclusive scan over the CTA's NT threads; *sum the total
 template <int NT>
-__device__ __forceinline__ int block_scan(int x, int* sum) {
-    __shared__ int w[NT / 32];
+__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* sum) {
+    __shared__ int64_t w[NT / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-    int upto = x;
+    int64_t upto = x;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, upto, d);
+        const int64_t o = __shfl_up_sync(0xffffffffu, upto, d);
         if (lane >= d) upto += o;
     }
     if (lane == 31) w[warp] = upto;
     __syncthreads();
-    int before = 0, all = 0;
+    int64_t before = 0, all = 0;
 #pragma unroll
     for (int i = 0; i < NT / 32; ++i) {
         if (i < warp) before += w[i];
@@ -150,19 +138,20 @@ __device__ __forceinline__ int block_scan(int x, int* sum) {
 template <int NT>
 __device__ __forceinline__ void plan_rows(const KvbAttnArgs& a, const RowsPlan& plan, int bn, int most) {
     const int tid = threadIdx.x, S = a.c.slots, G = a.heads / a.c.heads;
-    __shared__ int s_before[NT];       // the first units' costs before them
-    int units = 0, sum;
+    __shared__ int64_t s_before[NT];             // the first units' costs before them
+    int64_t counted = 0, sum;
+    // (offsets out of order may count more than `most` units: rows are then left out)
     for (int b0 = 0; b0 < S; b0 += NT) {
         const int b = b0 + tid;
         const int n = b < S ? (live_rows(kvb_span(a.r, b), a.c.cap) * G + kRows - 1) / kRows : 0;
-        const int at = block_scan<NT>(n, &sum);
-        if (b < S) plan.first[b] = units + at;
-        units += sum;
+        const int64_t at = block_scan<NT>(n, &sum);
+        if (b < S) plan.first[b] = (int)min(counted + at, (int64_t)most + 1);
+        counted += sum;
     }
+    const int units = (int)min(counted, (int64_t)most);
     if (tid == 0) plan.first[S] = units;
     __syncthreads();
-    units = min(units, most);                    // more only with offsets out of order: rows are then left out
-    int total = 0;
+    int64_t total = 0;
     for (int u0 = 0; u0 < units; u0 += NT) {
         const int u = u0 + tid;
         RowsUnit v{};
@@ -187,28 +176,9 @@ __device__ __forceinline__ void plan_rows(const KvbAttnArgs& a, const RowsPlan& 
     __syncthreads();
     // the shares, and where they begin (searched here once: a search through
     // global memory in every CTA of two kernels took 1.5 us in each)
-    for (int c = tid; c < kSms; c += NT) {
-        RowsShare w{};
-        w.join = -1;
-        const int64_t all = (int64_t)total * a.c.heads, ctas = min(all, (int64_t)kSms);
-        if (c < ctas) {
-            w.lo = div64(all * c, ctas), w.hi = div64(all * (c + 1), ctas);
-            w.h = (int)div64(w.lo, total);
-            const int at = (int)(w.lo - (int64_t)w.h * total);
-            int u = 0, hi = units;               // the last unit that begins at or before `at`
-            while (hi - u > 1) {
-                const int mid = (u + hi) >> 1;
-                if ((mid < NT ? s_before[mid] : plan.unit[mid].before) <= at) u = mid;
-                else hi = mid;
-            }
-            w.u = u;
-            const int64_t begin = (int64_t)w.h * total + (u < NT ? s_before[u] : plan.unit[u].before);
-            const int64_t end = begin + kUnitCost + plan.unit[u].tiles;
-            if (w.lo > begin + kUnitCost && div64(all * (c - 1), ctas) <= begin + kUnitCost)
-                w.join = (int)div64(end * ctas - 1, all);
-        }
-        plan.share[c] = w;
-    }
+    auto before = [&](int u) { return u < NT ? s_before[u] : plan.unit[u].before; };
+    auto tiles = [&](int u) { return plan.unit[u].tiles; };
+    for (int c = tid; c < kSms; c += NT) plan.share[c] = share_of(c, kSms, total, a.c.heads, units, before, tiles);
 }
 
 // A run of tiles of one unit within a CTA's share [x, end) of the cost.
@@ -219,7 +189,6 @@ struct Seg {
     __device__ __forceinline__ void unit(const RowsPlan& plan) {
         const RowsUnit v = plan.unit[u];
         slot = v.slot, m = v.m, tiles = v.tiles, p = v.p, r0 = v.r0, rows = v.rows;
-        begin_x = (int64_t)h * plan.head[0] + v.before;
         // a unit's own cost comes before its tiles
         j = (int)max(x - begin_x - kUnitCost, (int64_t)0);
         n = (int)(min(max(end - begin_x - kUnitCost, (int64_t)0), (int64_t)tiles) - j);
@@ -229,6 +198,7 @@ struct Seg {
         x = w.lo, end = w.hi;
         if (x >= end) return false;
         h = w.h, u = w.u;
+        begin_x = h * plan.head[0] + plan.unit[u].before;
         unit(plan);
         return n > 0 || next(plan);              // a share may end before the unit's first tile
     }
@@ -236,7 +206,8 @@ struct Seg {
         do {
             x = begin_x + kUnitCost + tiles;
             if (x >= end) return false;
-            if (++u == plan.head[1]) u = 0, ++h;
+            if (++u == (int)plan.head[1]) u = 0, ++h;
+            begin_x = x;                         // units lie side by side
             unit(plan);
         } while (n <= 0);
         return true;
@@ -1296,7 +1267,7 @@ cudaError_t rows_launch(const KvbAttnArgs& a, cudaStream_t st) {
     const int qbytes = a.type == KVB_F32 ? 4 : 2, units = (int)max_units(a.c, a.heads, a.r.rows);
     const RowsLayout L(a.c, a.heads, a.r.rows, a.mass != nullptr, qbytes);
     char* s = static_cast<char*>(a.scratch);
-    const RowsPlan plan{reinterpret_cast<int*>(s), reinterpret_cast<RowsUnit*>(s + L.unit), reinterpret_cast<int*>(s + L.first),
+    const RowsPlan plan{reinterpret_cast<int64_t*>(s), reinterpret_cast<RowsUnit*>(s + L.unit), reinterpret_cast<int*>(s + L.first),
                         reinterpret_cast<RowsShare*>(s + L.share)};
     float* parts = reinterpret_cast<float*>(s + L.parts);
     float2* stats = a.mass ? reinterpret_cast<float2*>(s + L.stats) : nullptr;
