@@ -25,8 +25,8 @@
 //             TMEM, written over S: hi in columns 0-7, lo in 8-15 of every 16;
 //             V as it lies, its rows being the contraction).
 // Block scales do not touch the codes: K's multiplies the scores of its 16
-// columns, V's goes into the weights, exp(z - m) sv / 2^lr 2^7 by one
-// exponential. m is the row's largest score and 2^lr its largest exp(z - m) sv,
+// columns, V's goes into the weights, exp(z - m) sv / 2^r 2^7 by one
+// exponential. m is the row's largest score and 2^r its largest exp(z - m) sv,
 // both over the tokens that it sees and lazily moved, so that the accumulator is
 // rescaled rarely; blocks that the row does not see, or gives no weight, leave the
 // others' halves their bits, however large their values are.
@@ -60,10 +60,10 @@ namespace {
 constexpr int kRows = 128;                       // rows of a unit (TMEM lanes)
 constexpr int kSms = 148;
 constexpr float kLog2e = 1.4426950408889634f;
-// log2 of: how far a score may pass m, a weight its reference (2^15 is the most that a half should hold),
-// and the reference's place
-constexpr float kLazyScore = 6.0f, kLazyWeight = 8.0f, kWeightLog = 7.0f;
-constexpr float kLeastLog = -126.0f;             // the least reference: 2^lr is a normal number
+// log2 of: how far a score may pass m, the most that a weight as a half should come to, and
+// what its reference stands for
+constexpr float kLazyScore = 6.0f, kMostWeight = 15.0f, kWeightLog = 7.0f;
+constexpr float kLeastLog = -126.0f;             // the least reference: a normal number
 constexpr unsigned int kErrWait = 256u;          // error bit 8: a pipeline wait gave up
 // The tensor cores round each product's running sum towards zero: an accumulator
 // is moved out and begun anew every kFold tiles (fp32, relative error of an output over
@@ -651,7 +651,7 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
             const bool live = f < seg.rows;
             const int lim = seg.p + (live ? f : seg.rows - 1) / G;       // the last token that the row sees
             const int all_see = seg.p + seg.m * kRows / G;               // ... that every row sees
-            float m = -INFINITY, l = 0.0f, lr = 0.0f;                    // lr: an integer
+            float m = -INFINITY, l = 0.0f, lr = 0.0f;                    // lr: an integer, log2 of the reference less kWeightLog
             float acc_f = 1.0f;                  // rescaling of the moved-out accumulator since it was moved
             float4* acc = reinterpret_cast<float4*>(accs + (int64_t)blockIdx.x * C::ACC) + w * (HD / 8) * kRows + row;
             // scales of a tile's 16-token groups, loaded a tile ahead: lanes 0-15
@@ -703,7 +703,7 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                         for (int i = 1; i < 15; i += 2)
                             y = fmaxf(fmaxf(y, __uint_as_float(v[16 * g + i])), __uint_as_float(v[16 * g + i + 1]));
                         y = fmaxf(y, __uint_as_float(v[16 * g + 15]));
-                        z[g] = y != -INFINITY ? y * fk[g] : y;
+                        z[g] = cut && y == -INFINITY ? y : y * fk[g];
                         x = fmaxf(x, z[g]);
                     }
                 };
@@ -711,8 +711,8 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
 #pragma unroll
                     for (int g = 0; g < HC / 16; ++g) {
                         uint32_t p[16];          // hi, lo
-                        // 2^7 sv / 2^lr joins the exponent; the sum of the weights without it
-                        const float lv = fmaxf(fv[g] - lr + kWeightLog, -40.0f), fz = fk[g], off = lv - m;
+                        // sv / 2^lr joins the exponent; the sum of the weights without it
+                        const float lv = fmaxf(fv[g] - lr, -40.0f), fz = fk[g], off = lv - m;
                         const uint64_t fz2 = pack2(fz, fz), off2 = pack2(off, off);
                         uint64_t sum = 0;
 #pragma unroll
@@ -747,7 +747,7 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                 else largest(std::false_type{}, 0);
                 // (x - m + most is no less than what the reference goes by; all of it relative to a
                 // maximum, since scores may be so large that a scale is lost in them)
-                if (barrier_any(1, C::SOFT, x > m + kLazyScore || x - m + most > lr + kLazyWeight)) {
+                if (barrier_any(1, C::SOFT, x > m + kLazyScore || x - m + most > lr + kMostWeight)) {
                     s_half[w][row] = x;
                     named_barrier_sync(2, C::SOFT);
                     const float xm = fmaxf(fmaxf(x, s_half[w ^ 1][row]), m);
@@ -756,9 +756,9 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                     for (int g = 0; g < NG / 2; ++g) top = fmaxf(top, z[g] - xm + fv[g]);
                     s_top[w][row] = top;
                     named_barrier_sync(2, C::SOFT);
-                    top = fmaxf(fmaxf(top, s_top[w ^ 1][row]), m - xm + lr);
+                    top = fmaxf(fmaxf(top, s_top[w ^ 1][row]), m - xm + lr + kWeightLog);
                     // (a row that has seen nothing yet stays as it is)
-                    const float xr = xm == -INFINITY ? lr : fminf(fmaxf(ceilf(top), kLeastLog), 127.0f);
+                    const float xr = xm == -INFINITY ? lr : fminf(fmaxf(ceilf(top), kLeastLog), 127.0f) - kWeightLog;
                     const float dm = xm == m ? 0.0f : m - xm, el = ex2(dm), eo = ex2(dm + (lr - xr));
                     if (jj > 0) {                // the products of the tile before are in
                         wait(&v_free[(tl - 1) % C::NBUF], ((tl - 1) / C::NBUF) & 1);
@@ -816,7 +816,7 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
             const bool whole = seg.j == 0 && seg.n == seg.tiles;
             // parts are divided by their own sums, so that none passes the largest value
             // (a part that the row sees nothing of: 0; 1 / NaN stays)
-            const float fo = exp2_int(-kWeightLog) * (l == 0.0f ? 0.0f : 1.0f / l), fr = exp2_int(lr);
+            const float fo = exp2_int(-kWeightLog) * (l == 0.0f ? 0.0f : 1.0f / l), fr = exp2_int(lr + kWeightLog);
             const int64_t orow = (int64_t)(seg.r0 + f / G) * a.heads + seg.h * G + f % G;
             float* pt = parts + ((int64_t)blockIdx.x * 2 + (seg.j == 0)) * C::PART;
             wait(&o_full, sn & 1);
