@@ -146,7 +146,7 @@ def kvb_read(k_codes: torch.Tensor, k_scale: torch.Tensor, v_codes: torch.Tensor
              pos: torch.Tensor, start: torch.Tensor, rows: int) -> tuple[torch.Tensor, torch.Tensor]:
     """The fp32 values held at the rows' positions (ops.kvb_read); rows behind
     the last sequence are zero."""
-    k, v = (torch.zeros(rows, k_codes.shape[1], k_codes.shape[3], device=k_codes.device) for _ in range(2))
+    k, v = (k_scale.new_zeros(rows, k_codes.shape[1], k_codes.shape[3]) for _ in range(2))
     return ops.kvb_read((k_codes, k_scale, v_codes, v_scale), pos, start, rows, k=k, v=v)
 
 
