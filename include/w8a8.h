@@ -536,9 +536,13 @@ int w8a8_kvb_read(const W8A8KvBlocks* cache, int rows, const int32_t* pos, const
  * idle slots and rows past the capacity. heads a multiple of kv_heads. mass (or
  * NULL; 16-byte aligned): [slots][kv_heads][capacity], each token's probabilities,
  * summed over the rows and the query heads of its KV head, are added. start NULL: one row
- * per slot (decode). scratch: w8a8_kvb_attn_scratch_bytes() bytes for at least
- * this many rows (16-byte aligned, contents irrelevant), not shared by calls
- * that can overlap. */
+ * per slot (decode). A row depends on no token that it does not see, and its error is
+ * relative to its own sum of p |v|, whatever the values' size. Prompt rows: scores of up
+ * to 2^24 in size (past 2^27 a row may become NaN: the rounding of an fp32 score
+ * is then larger than a weight's range). scratch: w8a8_kvb_attn_scratch_bytes() bytes
+ * for at least this many rows (16-byte aligned, contents irrelevant), not shared by
+ * calls that can overlap; decode with mass takes 4 bytes for every query head and
+ * place of the capacity of every slot. */
 size_t w8a8_kvb_attn_scratch_bytes(const W8A8KvBlocks* cache, int heads, int rows, int one_row_per_slot,
                                    int with_mass, int dtype);
 int w8a8_kvb_attn(const W8A8KvBlocks* cache, const void* q, int64_t q_stride, int dtype, int heads, int rows,
@@ -551,7 +555,9 @@ int w8a8_kvb_attn(const W8A8KvBlocks* cache, const void* q, int64_t q_stride, in
  * the lower position; NaN counts as -infinity), in their order, at positions
  * 0 .. keep - 1; each block is requantized to its largest value (codes
  * rint((q * s) / s'), s' = max|q * s| * F(1/127)). A slot with n <= keep stays
- * as it is. dst NULL: in place (dst_mass is then ignored, mass is written);
+ * as it is. A place is then not its token's position any more: rows of a cut slot
+ * are appended and attended at places (pos), and carry the encoding of their
+ * positions. dst NULL: in place (dst_mass is then ignored, mass is written);
  * else the result goes to dst / dst_mass (no overlap with cache / mass; its
  * capacity at least keep) and the source stays. kept [slots][kv_heads][keep]:
  * each place's former position, -1 past the new length; count_out [slots]

@@ -27,15 +27,17 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // ---------------------------------------------------------------- one row per slot
 // The cache is streamed once; everything else is small, so DRAM bounds it: 128
-// sequences of 2,032 tokens, 8 KV heads of 128 (535 MB): 91 us, 5.9 TB/s, and 5 us
-// for the joins; 94 MB of four ragged sequences: 22 + 6 us (4.2 TB/s: start and end
-// of the stream). For one sequence of 2,032 tokens the chain of latencies is all.
+// sequences of 2,032 tokens, 8 KV heads of 128 (535 MB): 104 us, 5.1 TB/s, 5 us of it
+// the joins; 94 MB of four ragged sequences: 27.5 us with the joins (start and end
+// of the stream). For one sequence of 2,032 tokens the chain of latencies is all (8.7 us).
 //
 // Work: a unit is one (slot, KV head, group of GC query heads); its tokens come
 // in tiles of 64 KT. All units' tiles, in order, are dealt out in equal
 // contiguous shares to a fixed grid, so that lengths of any mix load every SM
-// alike and the scratch does not grow with the capacity: a CTA leaves at most
-// two partial units (its first and its last), which kvb_step_finish joins.
+// alike and the partial results do not grow with the capacity: a CTA leaves at most
+// two (its first unit and its last), which kvb_step_finish joins. (Weights to gather
+// do take a score for every head and place of the capacity.) Every CTA, and every
+// joined row, counts the slots through by itself: for hundreds of them, not many thousands.
 //
 // A warp takes 16 KT tokens of a tile through its own ring of shared-memory
 // stages (cp.async, no block barrier in the loop) and keeps its own maxima,

@@ -34,11 +34,13 @@
 // Bound by two chains that run beside each other: the softmax warps (wait, read 64
 // scores, exponentials, write the weights; two warps a scheduler, half of all issue
 // slots) and the products' thread (for fp32 2,048 cycles of products a tile, the rest
-// hand-overs). 8,192 causal rows, 16 heads on 8 KV heads of 128, fp32: 610 us, 0.45
-// PFLOP/s of the formula's operations and 0.9 of those done (hi and lo); the tensor
-// pipe is active 41 % of the time, 3 % of the DRAM's rate is used. Four softmax
-// threads a row (24 warps) took 7 to 11 % longer; two groups that take turns on the
-// tiles with an accumulator each (64-channel heads) 35 %.
+// hand-overs). 8,192 causal rows, 16 heads on 8 KV heads of 128, fp32: 650 us of a
+// call's 690, 0.42 PFLOP/s of the formula's operations and 0.84 of those done (hi and
+// lo); the tensor pipe is active 42 % of the time, 2.5 % of the DRAM's rate is used.
+// Four softmax threads a row (24 warps) took 7 to 11 % longer; two groups that take
+// turns on the tiles with an accumulator each (64-channel heads) 35 %. Head sizes above
+// 128 have room for one buffer and one tile on its way: 4,096 fp32 rows, 16 heads on
+// 8 KV heads of 256, 668 us (0.2 PFLOP/s, tensor pipe 19 %).
 #include <type_traits>
 
 #include "kvb.cuh"
@@ -953,7 +955,9 @@ __global__ void __launch_bounds__(kFinishThreads) kvb_rows_finish(const KvbAttnA
 // A warp holds 16 TG tokens; with few token tiles the CTA's warps hold the same
 // ones and share out the rows (kvb_rows_mass_few), else four warps hold four tiles
 // and share the queries they read. Sums run in a fixed order: over a warp's rows,
-// then over the warps. Bound by the tensor products and their exponentials.
+// then over the warps. Sixteen prompts of up to 1,500 rows, 9 heads on 3 KV heads of 64:
+// 328 us, issue slots 14 %, warps 10 %: bound by the CTAs of the first tokens, which
+// every row sees, while the others are done.
 constexpr int kMassThreads = 128;
 
 template <int HD, bool Q2>
@@ -1120,8 +1124,8 @@ __global__ void __launch_bounds__(kMassThreads) kvb_rows_mass(const KvbAttnArgs 
 // sixteenth group of STEP rows through a ring of its own, so that no barrier stands
 // in the loop and four warps a scheduler cover the products' latency. 1,500 rows
 // of 9 heads on 3 KV heads of 64, two sequences: 31 us (38 with 8 rows a step, 57 with
-// half the warps) against 100 with four warps that met at each 32 rows. Bound by
-// its instructions, not by the rings.
+// half the warps) against 100 with four warps that met at each 32 rows. Issue slots are
+// 24 % used, the tensor pipe 14 %: bound by latencies and by the second wave of CTAs.
 constexpr int kFewWarps = 16;
 
 template <int HD, bool Q2>

@@ -587,7 +587,8 @@ def kvb_attn_rows(q, cache, pos, start, scale=None, mass=None, out=None, scratch
     """Prompt attention over the cache: slot b's rows start[b] .. start[b + 1]
     - 1 of q [rows, heads, head_dim] stand at positions pos[b], pos[b] + 1, ...
     and attend the tokens up to their own (all appended before). Rows behind
-    the last sequence are left as they are in `out`; the rest as kvb_attn."""
+    the last sequence are left as they are in `out`; the rest as kvb_attn. Scores of
+    up to 2^24 in size (past 2^27 a row may become NaN)."""
     if start is None:
         raise ValueError("start: an int32 [slots + 1] tensor is required")
     return _kvb_attn(q, cache, pos, start, scale, mass, out, scratch)
@@ -597,7 +598,8 @@ def kvb_evict(cache, mass, count, keep, sink=0, recent=0, dst=None, dst_mass=Non
     """Cut every slot that holds more than `keep` tokens (count [slots]) to
     `keep`: the first `sink`, the last `recent` and the heaviest by `mass` of
     those between, moved together in their order; in place, or into dst /
-    dst_mass. Returns (kept [slots, kv_heads, keep] int32: each place's former
+    dst_mass. From then on a token's place is not its position: append and attend
+    at places (the new length is the next one). Returns (kept [slots, kv_heads, keep] int32: each place's former
     position, -1 past the new length; the new lengths [slots] int32)."""
     c, dev = _kvb(cache)
     _kvb_mass(mass, cache[0])
