@@ -165,3 +165,30 @@ def test_subnormal_queries_of_single_tokens():
     q = torch.randn(2, 8, 64, generator=g, device=DEV) * 1e-38 * 2.0 ** -torch.arange(0, 16, 2, device=DEV).view(8, 1)
     assert (q != 0).any(-1).all()
     compare(q, cache, [255, 100], None, "fp32", 64, 256, scale=1e38, rows=False)
+
+
+@pytest.mark.parametrize("rows", [False, True])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_the_largest_scales(hd, rows):
+    """Scales of up to 2^126 with codes whose values are still finite, beside ordinary ones."""
+    g = torch.Generator(device=DEV).manual_seed(hd)
+    cache = make_cache(g, 2, 2, 512, hd, 32)
+    cache.v.clamp_(-2, 2)
+    cache.v_scale[:, :, 1::2] = 2.0 ** 126
+    n = 40 if rows else 1
+    q = torch.randn(2 * n, 4, hd, generator=g, device=DEV)
+    compare(q, cache, [470, 40], [0, n, 2 * n], "fp32", hd, 512, rows=rows)
+
+
+@pytest.mark.parametrize("rows", [False, True])
+@pytest.mark.parametrize("tiny", [1e-2, 1e-4, 1e-7])
+@pytest.mark.parametrize("heads,kv_heads,hd,cap", [(16, 8, 128, 2048), (8, 2, 64, 2048), (8, 2, 64, 17024), (4, 4, 256, 640)])
+def test_a_first_token_that_takes_the_weight(heads, kv_heads, hd, cap, tiny, rows):
+    """Its own values tiny: every other block's scale is far over the heaviest weight's, its weights are not."""
+    g = torch.Generator(device=DEV).manual_seed(hd)
+    cache = make_cache(g, 2, kv_heads, cap, hd, 64)
+    cache.k[:, :, 0] = 127
+    cache.v_scale[:, :, 0] *= tiny
+    n = 33 if rows else 1
+    q = torch.randn(2 * n, heads, hd, generator=g, device=DEV) + 0.5
+    compare(q, cache, [cap - n, cap // 2], [0, n, 2 * n], "fp32", hd, cap, rows=rows)

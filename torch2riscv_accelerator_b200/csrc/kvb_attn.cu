@@ -28,8 +28,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // ---------------------------------------------------------------- one row per slot
 // The cache is streamed once; everything else is small, so DRAM bounds it: 128
 // sequences of 2,032 tokens, 8 KV heads of 128 (535 MB): 104 us, 5.1 TB/s, 5 us of it
-// the joins; 94 MB of four ragged sequences: 27.5 us with the joins (start and end
-// of the stream). For one sequence of 2,032 tokens the chain of latencies is all (8.7 us).
+// the joins; 94 MB of four ragged sequences: 27.7 us with the joins (start and end
+// of the stream). For one sequence of 2,032 tokens the chain of latencies is all (8.9 us).
 //
 // Work: a unit is one (slot, KV head, group of GC query heads); its tokens come
 // in tiles of 64 KT. All units' tiles, in order, are dealt out in equal
@@ -57,15 +57,16 @@ constexpr float kLog2e = 1.4426950408889634f;
 // The weights are exp(z - m) sv / 2^r 2^5: m is the warp's largest score of the head,
 // 2^r its largest exp(z - m) sv, an integer power of two, so that a block without weight
 // leaves the others' halves their bits, however large its values are. Both move lazily:
-// a warp looks when a score passes m by 2^5 or a block's V scale 2^r by 2^5, and rescales;
-// the weights then stay below 2^15. A warp's outputs are divided by its own sum before
+// a warp looks when a score passes m by 2^5 or a block's V scale 2^r by 2^5, and rescales
+// where a weight would pass 2^15. A warp's outputs are divided by its own sum before
 // they are joined, so that none passes the largest value.
 namespace cg = cooperative_groups;
 constexpr int kStepWarps = 4;
 constexpr int kClusterMost = 16;                 // CTAs of a cluster
 constexpr int kMaxParts = 2;                     // partial units per CTA
 constexpr float kLazyScore = 5.0f, kLazyScale = 1024.0f;   // 2^5, and the weights' 2^5
-constexpr int kWeightLog = 5, kLeastLog = -119, kMostLog = 122;   // the references' range: 2^(5 - r) and its inverse are normal
+constexpr float kMostWeight = 32768.0f;
+constexpr int kWeightLog = 5, kLeastLog = -119, kMostLog = 128;   // the references' range: 2^(5 - r) and its inverse are normal
 
 template <int HD, int GC>
 struct StepCfg {
@@ -454,17 +455,27 @@ __global__ void __launch_bounds__(kThreads, StepCfg<HD, GC>::CTAS) kvb_step_kern
                     xa = fmaxf(xa, fmaxf(z[1][0], z[1][2])), xb = fmaxf(xb, fmaxf(z[1][1], z[1][3]));
                     xs = fmaxf(xs, fs[1]);
                 }
-                if (__any_sync(0xffffffffu, xa > ma + kLazyScore || xb > mb + kLazyScore || xs * fmaxf(ra, rb) > kLazyScale)) {
+                const bool up = xa > ma + kLazyScore || xb > mb + kLazyScore;
+                const float over = xs * fmaxf(ra, rb);
+                if (__any_sync(0xffffffffu, up || over > kLazyScale)) {
+                    // a large scale counts only with its weight (a first token that takes most of it, its
+                    // own values tiny, would else have every tile rescaled: 128 sequences 106 -> 117 us)
                     float ya[KT], yb[KT];
+                    bool move = up || over > 0x1p126f;
 #pragma unroll
-                    for (int k = 0; k < KT; ++k) ya[k] = fmaxf(z[k][0], z[k][2]), yb[k] = fmaxf(z[k][1], z[k][3]);
-                    const float2 ea = move_refs<KT>(ya, fs, ma, ra), eb = move_refs<KT>(yb, fs, mb, rb);
-                    la *= ea.x, lb *= eb.x;
+                    for (int k = 0; k < KT; ++k) {
+                        ya[k] = fmaxf(z[k][0], z[k][2]), yb[k] = fmaxf(z[k][1], z[k][3]);
+                        move |= ex2(ya[k] - ma) * (fs[k] * ra) > kMostWeight || ex2(yb[k] - mb) * (fs[k] * rb) > kMostWeight;
+                    }
+                    if (__any_sync(0xffffffffu, move)) {
+                        const float2 ea = move_refs<KT>(ya, fs, ma, ra), eb = move_refs<KT>(yb, fs, mb, rb);
+                        la *= ea.x, lb *= eb.x;
 #pragma unroll
-                    for (int i = 0; i < MT; ++i)
+                        for (int i = 0; i < MT; ++i)
 #pragma unroll
-                        for (int x = 0; x < C::NP; ++x)
-                            o[i][x][0] *= ea.y, o[i][x][1] *= eb.y, o[i][x][2] *= ea.y, o[i][x][3] *= eb.y;
+                            for (int x = 0; x < C::NP; ++x)
+                                o[i][x][0] *= ea.y, o[i][x][1] *= eb.y, o[i][x][2] *= ea.y, o[i][x][3] *= eb.y;
+                    }
                 }
 #pragma unroll
                 for (int k = 0; k < KT; ++k) {
