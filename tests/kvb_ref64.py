@@ -5,20 +5,21 @@ A query enters with an error of at most 2^-22 of itself, the products are exact 
 summed in fp32, the result is scaled and taken from the maximum (two roundings):
 |dz| <= (2^-21 + (D / 16 + 2) 2^-23) max_t sum|q k_t| scale. A weight is off by 2 |dz|,
 and so is the sum that divides it; the exponential and its rounding to 21 bits add
-2^-20, V's scale as a logarithm (up to 128 in size, rounded once) 2^-18. The tensor cores round each product's running sum towards zero
-by at most 2^-23: two products for 16 tokens of the FOLD tiles of 128 between two
-move-outs, 2 * FOLD * 128 / 16 of them; the moved-out sums and the weights' sum are
-added in fp32 over n tokens in at most n / 32 + 16 steps of 2^-24. All are relative
-to sum p |v|: (4 |dz| + 2^-20 + 2^-18 + 16 FOLD 2^-23 + (n / 32 + 16) 2^-24) sum p |v|.
+2^-20, V's scale as a logarithm (up to 128 in size, rounded once) 2^-18. The tensor
+cores round each product's running sum towards zero by at most 2^-23: two products for
+16 tokens of the FOLD tiles of 128 between two move-outs, 2 * FOLD * 128 / 16 of them;
+the moved-out sums and the weights' sum are added in fp32 over n tokens in at most
+n / 32 + 16 steps of 2^-24. All are relative to sum p |v|:
+(4 |dz| + 2^-20 + 2^-18 + 16 FOLD 2^-23 + (n / 32 + 16) 2^-24) sum p |v|.
 
-A weight times V's scale, over a reference of at most four times the row's largest
-such (twice in prompts; at least 2^-126 of the largest weight, for single tokens 2^-119 and
-2^-120 of the largest weight times the largest scale),
-enters as two halves that stand for 2^5 of it (2^7). Where they are subnormal each is off
-by half a step of 2^-24, 2^-24 / 2^5 of the reference together (but a weight by no more
-than itself): sum_t min(2^-27 max_t p_t s_t, 2 p_t s_t) |code_t| (2^-30). (A channel where the heaviest token
-holds 0 has nothing but such weights.) The output's type rounds by half a step, relative
-to it and of its smallest subnormal; parts of a row that are joined round once more."""
+A weight times V's scale, over a reference of at most twice the row's largest such (four
+times for single tokens), enters as two halves that stand for 2^7 of it (2^5). Where they
+are subnormal each is off by half a step of 2^-24, 2^-24 / 2^7 of the reference together,
+but a weight by no more than itself: sum_t min(2^-30 max_t p_t s_t, 2 p_t s_t) |code_t|
+(2^-27). The reference is at least 2^-126 of the largest weight (2^-119, and 2^-120 of it
+times the largest scale). (A channel where the heaviest token holds 0 has nothing but
+such weights.) The output's type rounds by half a step, relative to it and of its
+smallest subnormal; parts of a row that are joined round once more."""
 import torch
 
 from torch2riscv_accelerator_b200 import ops
